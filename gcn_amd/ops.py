@@ -7,6 +7,7 @@ gather (preprocessing), forward (the test loop), sgd, mbgd_grad, update.
 """
 import ctypes as C
 import os
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -341,3 +342,295 @@ def update_adagrad(params, rms, grad, lr, it):
     _req(grad, _F64, "grad", params.numel())
     _l.check(_l.load().ccnn_update_adagrad_f64(_ptr(params), _ptr(rms), _ptr(grad), float(lr), int(it),
                                                params.numel(), _stream()), "ccnn_update_adagrad_f64")
+
+
+# ---- scoring, loss and optimiser on any model's logits, gradients and parameters ----
+
+_TYPES = {_F32: _l.TYPE_F32, _F64: _l.TYPE_F64, torch.bfloat16: _l.TYPE_BF16, torch.float16: _l.TYPE_F16}
+
+
+def _on_device(t, name, dtypes):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError(f"{name} must be a CUDA tensor")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} has dtype {t.dtype}, expected one of {', '.join(str(d) for d in dtypes)}")
+    return t
+
+
+def _same_device(t, name, device):
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+
+
+def _enqueue(device, name, *args):
+    """Calls a library function with `device` current and that device's current stream as its last argument."""
+    fn = getattr(_l.load(), name)
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, C.c_void_p(torch.cuda.current_stream(device).cuda_stream))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, C.c_void_p(torch.cuda.current_stream(device).cuda_stream))
+    if rc:
+        _l.check(rc, name)
+
+
+class LogProbs(NamedTuple):
+    """What log_probs returns; fp64 for fp64 logits, else fp32."""
+    logp: torch.Tensor                   # [rows] log probability of the target
+    entropy: Optional[torch.Tensor]      # [rows] in nats
+    top_logp: Optional[torch.Tensor]     # [rows, top] in falling order
+    top_index: Optional[torch.Tensor]    # [rows, top] int32
+    stats: torch.Tensor                  # [rows, 2] largest logit, log sum exp(x - largest)
+
+
+def _rows(t, name):
+    """(rows, columns, elements from row to row) of a matrix whose rows are contiguous and do not overlap."""
+    if t.dim() != 2 or t.shape[1] < 1:
+        raise ValueError(f"{name} must be [rows, classes] with at least one class, got {list(t.shape)}")
+    rows, classes = t.shape
+    if classes > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name} must be contiguous along its classes")
+    stride = t.stride(0) if rows > 1 else classes
+    if stride < classes:
+        raise ValueError(f"rows of {name} overlap")
+    return rows, classes, stride
+
+
+def _targets(targets, rows, device):
+    _on_device(targets, "targets", (torch.int32, torch.int64))
+    _same_device(targets, "targets", device)
+    if targets.dim() != 1 or targets.shape[0] != rows or (rows > 1 and targets.stride(0) != 1):
+        raise ValueError(f"targets must be contiguous [{rows}], got {list(targets.shape)}")
+    return targets
+
+
+def log_probs(logits, targets, top=0, want_entropy=True):
+    """Scores each row of logits [rows, classes] (fp32, fp64, bf16 or fp16; rows may be strided) at its
+    target, int32 or int64 [rows], counted from 0: log probability of the target, entropy of the row,
+    the `top` (at most 64) most likely classes with their log probabilities, equal logits in the order
+    of their indices.  -> LogProbs.  A negative target gives 0, one of `classes` or more NaN.  -inf
+    logits are classes that are not allowed; a row of nothing else has log probabilities of -inf and
+    entropy 0, a row with a NaN or +inf has NaN everywhere and top_index -1."""
+    _on_device(logits, "logits", tuple(_TYPES))
+    rows, classes, stride = _rows(logits, "logits")
+    _targets(targets, rows, logits.device)
+    top = int(top)
+    if top < 0 or top > min(_l.MAX_TOP, classes):
+        raise ValueError(f"top must be between 0 and {min(_l.MAX_TOP, classes)}, got {top}")
+    dev, wide, kind = logits.device, _F64 if logits.dtype == _F64 else _F32, _TYPES[logits.dtype]
+    stats = torch.empty((rows, 2), dtype=wide, device=dev)
+    logp = torch.empty(rows, dtype=wide, device=dev)
+    entropy = torch.empty(rows, dtype=wide, device=dev) if want_entropy else None
+    top_logp = torch.empty((rows, top), dtype=wide, device=dev) if top else None
+    top_index = torch.empty((rows, top), dtype=torch.int32, device=dev) if top else None
+    if rows:
+        nbytes = _l.load().ccnn_log_probs_workspace_bytes(rows, classes, top, kind)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        _enqueue(dev, "ccnn_log_probs", _ptr(logits), kind, rows, classes, stride, _ptr(targets), targets.element_size(), top,
+                 _ptr(logp), _ptr(entropy), _ptr(top_logp), _ptr(top_index), _ptr(stats), _ptr(ws), nbytes)
+    return LogProbs(logp, entropy, top_logp, top_index, stats)
+
+
+def log_probs_grad(logits, targets, scored, d_logp=None, d_entropy=None, out=None):
+    """Gradient of sum(d_logp * logp) + sum(d_entropy * entropy) to the logits, from what log_probs
+    returned for them.  d_logp / d_entropy: [rows] of the type of scored.logp, one of them at least.
+    out: [rows, classes] of the logits' type (rows may be strided), the logits themselves allowed."""
+    _on_device(logits, "logits", tuple(_TYPES))
+    rows, classes, stride = _rows(logits, "logits")
+    dev, wide = logits.device, _F64 if logits.dtype == _F64 else _F32
+    _targets(targets, rows, dev)
+    if d_logp is None and d_entropy is None:
+        raise ValueError("neither d_logp nor d_entropy given")
+    if d_entropy is not None and scored.entropy is None:
+        raise ValueError("d_entropy needs a log_probs call with want_entropy")
+    for t, name, n in ((scored.stats, "stats", 2 * rows), (d_logp, "d_logp", rows), (d_entropy, "d_entropy", rows),
+                       (scored.entropy, "entropy", rows)):
+        if t is not None:
+            _req(t, wide, name, n)
+            _same_device(t, name, dev)
+    if out is None:
+        out = torch.empty((rows, classes), dtype=logits.dtype, device=dev)
+    _on_device(out, "out", (logits.dtype,))
+    _same_device(out, "out", dev)
+    if out.shape != logits.shape:
+        raise ValueError(f"out is {list(out.shape)}, the logits are {list(logits.shape)}")
+    _, _, out_stride = _rows(out, "out")
+    if rows:
+        size = logits.element_size()
+        a, b = logits.data_ptr(), out.data_ptr()
+        if (a, stride) != (b, out_stride) and a < b + ((rows - 1) * out_stride + classes) * size \
+                and b < a + ((rows - 1) * stride + classes) * size:
+            raise ValueError("out overlaps the logits without being them")
+        _enqueue(dev, "ccnn_log_probs_grad", _ptr(logits), _TYPES[logits.dtype], rows, classes, stride, _ptr(targets),
+                 targets.element_size(), _ptr(scored.stats), _ptr(scored.entropy), _ptr(d_logp), _ptr(d_entropy), _ptr(out),
+                 out_stride)
+    return out
+
+
+def grad_norm(grads, max_norm=float("inf")):
+    """Norm of the list of gradient tensors taken as one vector -> float64 [2] on their device: the norm
+    and the factor min(1, max_norm / norm) that AdamW.step takes as `clip` (NaN if the norm is not
+    finite: that step is then left out).  Nothing is scaled here and nothing comes back to the host."""
+    grads = list(grads)
+    if not grads:
+        raise ValueError("grad_norm needs at least one tensor")
+    if not max_norm > 0:
+        raise ValueError(f"max_norm must be positive, got {max_norm}")
+    dev = grads[0].device if isinstance(grads[0], torch.Tensor) else None
+    table = (_l.Tensor * len(grads))()
+    for i, g in enumerate(grads):
+        _on_device(g, f"gradient {i}", tuple(_TYPES))
+        _same_device(g, f"gradient {i}", dev)
+        if not g.is_contiguous():
+            raise ValueError(f"gradient {i} must be contiguous")
+        table[i] = (g.data_ptr(), g.numel(), _TYPES[g.dtype])
+    out = torch.empty(2, dtype=_F64, device=dev)
+    nbytes = _l.load().ccnn_grad_norm_workspace_bytes(table, len(grads))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _enqueue(dev, "ccnn_grad_norm", table, len(grads), float(max_norm), _ptr(out), _ptr(ws), nbytes)
+    return out
+
+
+class AdamW:
+    """AdamW over a list of parameter tensors, all of them in one step:
+
+        m += (1 - beta1)(g - m);  v += (1 - beta2)(g^2 - v)
+        p -= lr (weight_decay p + m / (1 - beta1^t) / (sqrt(v / (1 - beta2^t)) + eps))
+
+    params: contiguous tensors on one device (views of one flat vector as well, see param_views), fp32,
+    bf16 or fp16 - or all fp64 - changed in place by step().  bf16 and fp16 parameters get an fp32
+    master copy (self.master, flat in the order of the list) that takes the step; the parameter is its
+    rounding, so it must not be changed from outside without load_state_dict.
+    weight_decay: one factor, or one per tensor.
+    state_bits=8 keeps m and sqrt(v) as e4m3 codes with one fp32 scale per 256 elements of a tensor (2.03
+    bytes a parameter instead of 8; not for fp64): moments() gives the values they stand for.
+    The step count lives on the device, so a captured step counts on when the graph is replayed; lr may be
+    a float (kept by a captured step as it was) or a float64 [1] device tensor that is read in the step.
+    Steps of one optimiser must be ordered by one stream."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32):
+        self.params = list(params)
+        if not self.params:
+            raise ValueError("AdamW needs at least one parameter tensor")
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        n = len(self.params)
+        decays = [float(weight_decay)] * n if not hasattr(weight_decay, "__len__") else [float(w) for w in weight_decay]
+        if len(decays) != n:
+            raise ValueError(f"{len(decays)} weight_decay factors for {n} tensors")
+        if not all(0 <= b < 1 for b in betas) or len(betas) != 2 or not eps >= 0:
+            raise ValueError(f"betas must be two numbers in [0, 1) and eps not negative, got {betas}, {eps}")
+        self.device = self.params[0].device if isinstance(self.params[0], torch.Tensor) else None
+        self.betas, self.eps, self.state_bits = (float(betas[0]), float(betas[1])), float(eps), state_bits
+        self.lr = lr
+        self._table = (_l.AdamwTensor * n)()
+        first = block = 0
+        spans = []
+        for i, p in enumerate(self.params):
+            _on_device(p, f"parameter {i}", tuple(_TYPES))
+            _same_device(p, f"parameter {i}", self.device)
+            if not p.is_contiguous():
+                raise ValueError(f"parameter {i} must be contiguous")
+            if (p.dtype == _F64) != (self.params[0].dtype == _F64):
+                raise TypeError("fp64 parameters do not mix with others in one optimiser")
+            if p.dtype == _F64 and state_bits == 8:
+                raise TypeError("moments in 8 bits are not for fp64 parameters")
+            kind = _TYPES[p.dtype]
+            self._table[i] = (p.data_ptr(), 0, p.numel(), first, block, decays[i], kind, kind)
+            if p.numel():
+                spans.append((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()))
+            first += p.numel()
+            block += -(-p.numel() // _l.MOMENT_BLOCK)
+        spans.sort()
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("parameter tensors overlap")
+        self.numel, self.blocks = first, block
+        wide = _F64 if self.params[0].dtype == _F64 else _F32
+        if state_bits == 32:
+            self.m, self.v = (torch.zeros(first, dtype=wide, device=self.device) for _ in range(2))
+            self.m_scale = self.v_scale = None
+        else:
+            self.m, self.v = (torch.zeros(block * _l.MOMENT_BLOCK, dtype=torch.uint8, device=self.device) for _ in range(2))
+            self.m_scale, self.v_scale = (torch.zeros(block, dtype=_F32, device=self.device) for _ in range(2))
+        self.master = None
+        if any(p.element_size() == 2 for p in self.params):
+            self.master = torch.cat([p.detach().reshape(-1).float() for p in self.params])
+        self._clock = torch.zeros(_l.ADAMW_CLOCK, dtype=_F64, device=self.device)
+        self._set_step(0)
+
+    def _set_step(self, t):
+        self._clock.copy_(torch.tensor([t, self.betas[0] ** t, self.betas[1] ** t] + [0.0] * (_l.ADAMW_CLOCK - 3), dtype=_F64))
+
+    @property
+    def step_count(self):
+        """Steps taken so far (waits for the device)."""
+        return int(self._clock[0].item())
+
+    def step(self, grads, lr=None, clip=None):
+        """One step from `grads`, one contiguous tensor per parameter with its size, of its type (or fp32
+        for bf16 / fp16).  lr: instead of self.lr.  clip: grad_norm's result; its factor scales every
+        gradient, and a factor that is not finite leaves everything as it is, the step count too."""
+        grads, table = list(grads), self._table
+        if len(grads) != len(self.params):
+            raise ValueError(f"{len(grads)} gradients for {len(self.params)} parameters")
+        for i, (g, p) in enumerate(zip(grads, self.params)):
+            _on_device(g, f"gradient {i}", (p.dtype, _F32) if p.element_size() == 2 else (p.dtype,))
+            _same_device(g, f"gradient {i}", self.device)
+            if not g.is_contiguous():
+                raise ValueError(f"gradient {i} must be contiguous")
+            if g.numel() != table[i].n:
+                raise ValueError(f"gradient {i} has {g.numel()} elements, its parameter {table[i].n}")
+            table[i].grad, table[i].grad_type = g.data_ptr(), _TYPES[g.dtype]
+        if clip is not None:
+            _req(clip, _F64, "clip", 2)
+            _same_device(clip, "clip", self.device)
+        lr = self.lr if lr is None else lr
+        lr_device = None
+        if isinstance(lr, torch.Tensor):
+            _req(lr, _F64, "lr", 1)
+            _same_device(lr, "lr", self.device)
+            lr, lr_device = 0.0, lr
+        _enqueue(self.device, "ccnn_adamw_step", table, len(grads), self.state_bits, _ptr(self.m), _ptr(self.v),
+                 _ptr(self.m_scale), _ptr(self.v_scale), _ptr(self.master), _ptr(self._clock), float(lr), _ptr(lr_device),
+                 self.betas[0], self.betas[1], self.eps, _ptr(clip))
+
+    def moments(self):
+        """(m, v), flat in the order of the parameters: the optimiser's own tensors with 32 bits, the values
+        the codes stand for (fp32) with 8."""
+        if self.state_bits == 32:
+            return self.m, self.v
+        m, v = (torch.empty(self.numel, dtype=_F32, device=self.device) for _ in range(2))
+        _enqueue(self.device, "ccnn_adamw_moments", self._table, len(self.params), _ptr(self.m), _ptr(self.v),
+                 _ptr(self.m_scale), _ptr(self.v_scale), _ptr(m), _ptr(v))
+        return m, v
+
+    def state_dict(self):
+        """Copies of everything a later run continues from (waits for the device)."""
+        keep = {k: getattr(self, k).clone() for k in ("m", "v", "m_scale", "v_scale", "master") if getattr(self, k) is not None}
+        return {"step": self.step_count, **keep}
+
+    def load_state_dict(self, state):
+        """Continues from a state_dict() of an optimiser over the same tensors with the same state_bits."""
+        for k in ("m", "v", "m_scale", "v_scale", "master"):
+            mine, given = getattr(self, k), state.get(k)
+            if (mine is None) != (given is None):
+                raise ValueError(f"state {'lacks' if given is None else 'has'} {k!r}")
+            if mine is not None and (mine.shape != given.shape or mine.dtype != given.dtype):
+                raise ValueError(f"{k!r} is {given.dtype} {list(given.shape)}, expected {mine.dtype} {list(mine.shape)}")
+        if int(state["step"]) < 0:
+            raise ValueError(f"step must not be negative, got {state['step']}")
+        for k in ("m", "v", "m_scale", "v_scale", "master"):
+            if getattr(self, k) is not None:
+                getattr(self, k).copy_(state[k])
+        if self.master is not None:
+            for p, t in zip(self.params, self._table):
+                p.detach().view(-1).copy_(self.master[t.first:t.first + t.n])
+        self._set_step(int(state["step"]))
+
+
+def param_views(flat, z):
+    """The network's six tensors W0, b0, W1, b1, W2, b2 as views of a flat parameter or gradient vector."""
+    d = _l.dims(z)
+    _req(flat, flat.dtype, "flat", d.nparams)
+    ends = [d.off_w0, d.off_b0, d.off_w1, d.off_b1, d.off_w2, d.off_b2, d.nparams]
+    return [flat[a:b] for a, b in zip(ends, ends[1:])]

@@ -373,6 +373,100 @@ int ccnn_mbgd_step_dp_f64(ccnn_comm_t *comm, double *params, const double *cubes
                           long first, int B, int z, double lr, int divisor, double *loss_values,
                           void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- scoring, loss and optimiser on any model's logits, gradients and parameters --------------
+ * No counterparts in the reference (its softmax, loss and update are fixed to its own network:
+ * output_and_dvalue gcn_mbgd_fp64.cu:307-354, loss_function :559-596, update_params_* :500-557).
+ * Element types, where an entry point takes one as an argument: */
+#define CCNN_TYPE_F32 1
+#define CCNN_TYPE_F64 2
+#define CCNN_TYPE_BF16 3
+#define CCNN_TYPE_F16 4
+
+/* Log probability of one given class per row, the row's entropy and its most likely classes.
+ * logits: rows x classes of `type`, row r at logits + r * stride elements (stride >= classes, any
+ * alignment of an element).  All results are fp64 for fp64 logits and fp32 for the other types.
+ *   targets   int32 or int64 (target_bytes 4 or 8), the class of each row counted from 0; negative =
+ *             none given (logp 0); classes or more = an error the device reports as logp NaN
+ *   logp      [rows] log softmax at the target
+ *   entropy   [rows], optional: -sum p log p in nats
+ *   top_logp, top_index  [rows][top], top <= CCNN_MAX_TOP and <= classes: the most likely classes in
+ *             falling order, equal logits in the order of their indices
+ *   stats     [rows][2]: largest logit m and log sum exp(x - m), for ccnn_log_probs_grad
+ * -inf is a class that is not allowed.  A row of nothing else has logp -inf, entropy 0, stats -inf and
+ * top_logp -inf; a row with a NaN or +inf has NaN everywhere and top_index -1.
+ * workspace: ccnn_log_probs_workspace_bytes() bytes (a function of its arguments only; 0 = none
+ * needed); it need not be initialised, and calls that share one must be ordered by one stream. */
+#define CCNN_MAX_TOP 64
+#define CCNN_MAX_LOGITS (1 << 30)
+size_t ccnn_log_probs_workspace_bytes(long rows, int classes, int top, int type);
+int ccnn_log_probs(const void *logits, int type, long rows, int classes, long stride,
+                   const void *targets, int target_bytes, int top, void *logp, void *entropy,
+                   void *top_logp, int *top_index, void *stats, void *workspace,
+                   size_t workspace_bytes, void *stream);
+
+/* Gradient of sum(d_logp * logp) + sum(d_entropy * entropy) to the logits, from the stats (and, with
+ * d_entropy, the entropy) that ccnn_log_probs left: d_logits rows x classes of the logits' type, row
+ * stride d_stride.  d_logp or d_entropy may be NULL (no such term), not both.  A negative target has no
+ * logp term; rows with nothing allowed get 0; rows with a target of `classes` or more, NaN.  d_logits
+ * may be the logits themselves (same stride); it must not overlap them otherwise. */
+int ccnn_log_probs_grad(const void *logits, int type, long rows, int classes, long stride,
+                        const void *targets, int target_bytes, const void *stats,
+                        const void *entropy, const void *d_logp, const void *d_entropy,
+                        void *d_logits, long d_stride, void *stream);
+
+/* Norm of many gradient tensors taken as one vector, and the factor that limits it.
+ * tensors: HOST array of `count` descriptions (n elements of `type` at `data`, n may be 0).
+ * out [2] device doubles: sqrt(sum g^2), summed in fp64 in a fixed order; and min(1, max_norm / norm),
+ * NaN when the norm is not finite.  workspace: ccnn_grad_norm_workspace_bytes() bytes, not
+ * initialised; calls that share one must be ordered by one stream. */
+typedef struct ccnn_tensor {
+    const void *data;
+    long n;
+    int type;
+} ccnn_tensor_t;
+size_t ccnn_grad_norm_workspace_bytes(const ccnn_tensor_t *tensors, int count);
+int ccnn_grad_norm(const ccnn_tensor_t *tensors, int count, double max_norm, double *out,
+                   void *workspace, size_t workspace_bytes, void *stream);
+
+/* One AdamW step (decoupled weight decay) over `count` parameter tensors:
+ *   g *= clip[1];  m += (1 - beta1)(g - m);  v += (1 - beta2)(g^2 - v)
+ *   p -= lr (decay p + m / (1 - beta1^t) / (sqrt(v / (1 - beta2^t)) + eps))
+ * tensors: HOST array.  `type` of a parameter is F32, F64, BF16 or F16; grad_type the same, or F32 for
+ * BF16 and F16.  F64 does not mix with the others in one call.  `first` is the tensor's place (in
+ * elements) in the flat arrays `master` (fp32, needed for BF16 and F16 parameters: the step is taken
+ * there and p is its rounding) and, with 32-bit moments, m and v (fp32; fp64 for F64 parameters).
+ * moment_bits 8 (not for F64): m and v hold sqrt(v) as one byte per element, in blocks of
+ * CCNN_MOMENT_BLOCK elements of one tensor, `block` being the tensor's first block; a block's
+ * values are code x scale, code an e4m3 number (4 exponent bits, bias 7, 3 fraction bits, the largest
+ * 448), scale = (largest magnitude of the block, rounded to fp32) / 448 in m_scale and v_scale [blocks].  New
+ * moments are computed in fp64 from the old codes, as beta x + (1 - beta) y with each operation rounded by
+ * itself, and then rounded once, to the nearest code (ties to the even one); a sqrt(v) above 0 keeps at
+ * least the smallest code, so a denominator never becomes 0 by rounding.  A block's bytes behind the tensor's end are left 0.  A gradient that is not finite makes
+ * its whole block NaN (with 32 bits: its element).
+ * clock [CCNN_ADAMW_CLOCK] device doubles: clock[0] = t, steps taken so far, clock[1] = beta1^t,
+ * clock[2] = beta2^t (initially 0, 1, 1); the call advances them on the device, so a captured step counts
+ * on when it is replayed.  lr_device, if not NULL, is read instead of lr.  clip, if not NULL, is
+ * ccnn_grad_norm's out: when clip[1] is not finite nothing is changed, t included. */
+#define CCNN_MOMENT_BLOCK 256
+#define CCNN_ADAMW_CLOCK 8
+typedef struct ccnn_adamw_tensor {
+    void *param;
+    const void *grad;
+    long n;
+    long first, block;
+    double decay;
+    int type, grad_type;
+} ccnn_adamw_tensor_t;
+int ccnn_adamw_step(const ccnn_adamw_tensor_t *tensors, int count, int moment_bits, void *m, void *v,
+                    float *m_scale, float *v_scale, float *master, double *clock, double lr,
+                    const double *lr_device, double beta1, double beta2, double eps,
+                    const double *clip, void *stream);
+/* 8-bit moments as the values they stand for: m_out, v_out flat fp32 (v, not its root), tensor i at
+ * tensors[i].first (param and grad are not looked at). */
+int ccnn_adamw_moments(const ccnn_adamw_tensor_t *tensors, int count, const void *m, const void *v,
+                       const float *m_scale, const float *v_scale, float *m_out, float *v_out,
+                       void *stream);
+
 /* Measurement hooks (no counterpart in the reference).  While enabled, every
  * kernel launch of this library carries a start/stop HIP event pair on its own
  * stream (attached to the dispatch, so the interval is the kernel's own).  ccnn_profile_report(i, ...) returns 1 and the i-th kernel's name,

@@ -106,3 +106,58 @@ def test_integration_sketch_compiles_against_the_header(tmp_path):
                             "-I", "/opt/rocm/include", "-I", os.path.join(ROOT, "include"), str(src)],
                            capture_output=True, text=True)
         assert r.returncode == 0, r.stderr
+
+
+def test_scoring_and_optimiser_calls_refuse_bad_arguments():
+    """The argument checks of ccnn_log_probs*, ccnn_grad_norm and ccnn_adamw_* answer before anything is launched."""
+    import ctypes as C
+    lib, ok, nul = L.load(), C.c_void_p(64), C.c_void_p()
+
+    def score(x=ok, kind=1, rows=2, classes=5, stride=5, y=ok, yb=4, top=2, logp=ok, tl=ok, ti=ok, stats=ok):
+        return lib.ccnn_log_probs(x, kind, rows, classes, stride, y, yb, top, logp, nul, tl, ti, stats, nul, 0, nul)
+
+    assert score(rows=0) == 0
+    for bad in (dict(x=nul), dict(kind=0), dict(kind=5), dict(rows=-1), dict(classes=0), dict(stride=4), dict(y=nul),
+                dict(yb=2), dict(top=-1), dict(top=6), dict(logp=nul), dict(tl=nul), dict(ti=nul), dict(stats=nul)):
+        assert score(**bad) == -1, bad
+    assert score(rows=1 << 31) == -3 and score(classes=(1 << 30) + 1, stride=1 << 40) == -3
+    assert score(classes=100, stride=100, top=65) == -1
+
+    def grad(x=ok, kind=1, classes=5, stride=5, stats=ok, h=ok, dl=ok, dh=ok, out=C.c_void_p(4096), ostride=5, rows=2):
+        return lib.ccnn_log_probs_grad(x, kind, rows, classes, stride, ok, 4, stats, h, dl, dh, out, ostride, nul)
+
+    assert grad(rows=0) == 0
+    for bad in (dict(x=nul), dict(kind=9), dict(stats=nul), dict(h=nul), dict(dl=nul, dh=nul), dict(out=nul), dict(ostride=4),
+                dict(out=ok, ostride=6)):
+        assert grad(**bad) == -1, bad
+
+    t = (L.Tensor * 2)((64, 10, 1), (64, 40000, 3))
+    need = lib.ccnn_grad_norm_workspace_bytes(t, 2)
+    assert need >= 16
+    assert lib.ccnn_grad_norm(t, 2, 1.0, ok, ok, need - 1, nul) == -2
+    assert lib.ccnn_grad_norm(t, 2, 0.0, ok, ok, need, nul) == -1
+    assert lib.ccnn_grad_norm(t, 2, float("nan"), ok, ok, need, nul) == -1
+    assert lib.ccnn_grad_norm(t, 2, 1.0, nul, ok, need, nul) == -1
+    assert lib.ccnn_grad_norm(t, -1, 1.0, ok, ok, need, nul) == -1
+    for bad in ((0, 10, 1), (64, -1, 1), (64, 10, 7)):
+        assert lib.ccnn_grad_norm((L.Tensor * 1)(bad), 1, 1.0, ok, ok, 64, nul) == -1
+
+    fine = (64, 64, 10, 0, 0, 0.1, 1, 1)
+
+    def step(*ts, bits=32, m=ok, v=ok, ms=ok, vs=ok, master=ok, clock=ok, b1=0.9, b2=0.999, eps=1e-8):
+        arr = (L.AdamwTensor * max(1, len(ts)))(*ts)
+        return lib.ccnn_adamw_step(arr, len(ts), bits, m, v, ms, vs, master, clock, 1e-3, nul, b1, b2, eps, nul, nul)
+
+    for bad in (dict(bits=16), dict(m=nul), dict(v=nul), dict(clock=nul), dict(b1=1.0), dict(b2=-0.1), dict(eps=-1.0),
+                dict(bits=8, ms=nul), dict(bits=8, vs=nul), dict(b1=float("nan"))):
+        assert step(fine, **bad) == -1, bad
+    assert step((64, 64, 10, 0, 0, 0.1, 3, 3), master=nul) == -1           # half precision without its master copy
+    assert step((64, 64, 10, 0, 0, 0.1, 2, 2), bits=8) == -1               # 8-bit moments of doubles
+    assert step(fine, (64, 64, 10, 0, 0, 0.1, 2, 2)) == -1                 # doubles among others
+    for bad in ((0, 64, 10, 0, 0, 0.1, 1, 1), (64, 0, 10, 0, 0, 0.1, 1, 1), (64, 64, -1, 0, 0, 0.1, 1, 1),
+                (64, 64, 10, -1, 0, 0.1, 1, 1), (64, 64, 10, 0, -1, 0.1, 1, 1), (64, 64, 10, 0, 0, 0.1, 1, 3),
+                (64, 64, 10, 0, 0, 0.1, 3, 4), (64, 64, 10, 0, 0, 0.1, 0, 0)):
+        assert step(bad) == -1, bad
+    arr = (L.AdamwTensor * 1)(fine)
+    assert lib.ccnn_adamw_moments(arr, 1, nul, ok, ok, ok, ok, ok, nul) == -1
+    assert lib.ccnn_adamw_moments(arr, -1, ok, ok, ok, ok, ok, ok, nul) == -1

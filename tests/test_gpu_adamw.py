@@ -1,0 +1,352 @@
+"""GPU: gradient norm and AdamW (moments in 32 and in 8 bits) against their 64-bit restatement."""
+import math
+
+import pytest
+import torch
+
+import wide_ref as ref
+from gcn_amd import lib as L
+from gcn_amd import ops
+
+pytestmark = pytest.mark.gpu
+
+F32, F64, BF16, F16 = torch.float32, torch.float64, torch.bfloat16, torch.float16
+KINDS = [(F32, F32), (BF16, BF16), (BF16, F32), (F16, F16), (F16, F32)]
+SIZES = [1, 255, 256, 257, 0, 1000, 4095, 4096, 4097, 13, 9000, 3, 20001]
+
+
+def tensors(sizes, kind, seed, scale, offset=1):
+    """Views of one flat buffer, the first starting `offset` elements in."""
+    g = torch.Generator().manual_seed(seed)
+    flat = (torch.randn(sum(sizes) + offset, generator=g, dtype=F64) * scale).to(kind).cuda()
+    out, at = [], offset
+    for n in sizes:
+        out.append(flat[at:at + n])
+        at += n
+    return out
+
+
+def mixed_scale_grads(sizes, kind, seed):
+    """Gradients over many orders of magnitude, with zeros."""
+    out = []
+    for i, t in enumerate(tensors(sizes, F64, seed, 1.0)):
+        g = torch.Generator().manual_seed(seed + i)
+        mag = 10.0 ** (torch.rand(t.numel(), generator=g, dtype=F64) * 5 - 6)
+        mag[torch.rand(t.numel(), generator=g) < 0.05] = 0.0
+        out.append((t.cpu() * mag).to(kind).cuda())
+    return out
+
+
+def near(got, want, rel, floor, what):
+    got, want = got.detach().cpu().double(), want.double()
+    off = (got - want).abs()
+    bound = rel * want.abs() + floor
+    assert torch.isfinite(got).all() and (off <= bound).all(), (what, float((off - bound).max()))
+
+
+def check(opt, want, params, steps, u, lr, prev=None):
+    """After `steps` steps: with u half a step, one step rounds g * scale, m, v, the quotient and p.  m is off by at
+    most 4u(|m| + |g|) a step and v by 5u(v + g^2), both weighted down by the betas after; the update lr * m / sqrt(v) is
+    at most lr * C in size (C = 1 / sqrt(1 - beta2) for one step) and off by 16u of itself and u of p each step."""
+    flat_p = torch.cat([p for p in want.p])
+    size = 40 * lr                                   # |update| <= lr (1 / sqrt(1 - beta2) + decay |p|) < 40 lr
+    got = opt.master if opt.master is not None else torch.cat([p.detach().reshape(-1) for p in params])
+    near(got, flat_p, 4 * steps * u, steps * 40 * u * size, "p")
+    if opt.master is not None:
+        at = 0
+        for p in params:
+            assert torch.equal(p.detach().cpu(), opt.master[at:at + p.numel()].cpu().to(p.dtype)), "rounding of the master copy"
+            at += p.numel()
+
+
+@pytest.mark.parametrize("kind,grad_kind", KINDS + [(F64, F64)], ids=str)
+@pytest.mark.parametrize("offset", [0, 1, 3])
+def test_steps_with_32_bit_moments(kind, grad_kind, offset):
+    lr, u = 1e-2, ref.half_step(F64 if kind == F64 else F32)
+    params = tensors(SIZES, kind, 1, 0.5, offset)
+    decays = [0.1 * (i % 3) for i in range(len(SIZES))]
+    want = ref.AdamW(params, lr, decays=decays)
+    opt = ops.AdamW(params, lr=lr, weight_decay=decays)
+    gmax = torch.zeros(sum(SIZES), dtype=F64)
+    for k in range(5):
+        grads = mixed_scale_grads(SIZES, grad_kind, 100 + k)
+        opt.step(grads)
+        want.step(grads)
+        gmax = torch.maximum(gmax, torch.cat([g.cpu().double() for g in grads]).abs())
+    assert opt.step_count == 5
+    check(opt, want, params, 5, u, lr)
+    m, v = opt.moments()
+    tiny = torch.finfo(F64 if kind == F64 else F32).smallest_normal
+    assert ((m.cpu().double() - torch.cat(want.m)).abs() <= 5 * 4 * u * gmax + tiny).all()
+    assert ((v.cpu().double() - torch.cat(want.v)).abs() <= 5 * 5 * u * gmax ** 2 + tiny).all()
+
+
+@pytest.mark.parametrize("kind,grad_kind", KINDS, ids=str)
+def test_steps_with_8_bit_moments(kind, grad_kind):
+    """The codes and scales are those of the 64-bit definition, bit for bit, step after step."""
+    lr, u = 1e-2, ref.half_step(F32)
+    params = tensors(SIZES, kind, 2, 0.5)
+    want = ref.AdamW(params, lr, bits=8)
+    opt = ops.AdamW(params, lr=lr, state_bits=8)
+    for k in range(6):
+        grads = mixed_scale_grads(SIZES, grad_kind, 200 + k)
+        opt.step(grads)
+        want.step(grads)
+        mc, vc, ms, vs = want.codes
+        assert torch.equal(opt.m_scale.cpu(), ms) and torch.equal(opt.v_scale.cpu(), vs), k
+        assert torch.equal(opt.m.cpu() & 127, mc & 127) and torch.equal(opt.v.cpu(), vc), k
+        assert torch.equal(ref.decode(opt.m.cpu().view(-1, 256), opt.m_scale.cpu()), ref.decode(mc.view(-1, 256), ms)), k
+    check(opt, want, params, 6, u, lr)
+    m, v = opt.moments()
+    assert torch.equal(m.cpu(), torch.cat(want.m).float()) and torch.equal(v.cpu(), torch.cat(want.v).float())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_magnitudes_at_the_edges(bits):
+    """Gradients whose squares leave the range of fp32 at either end, next to ordinary ones and zeros, in one block
+    and in blocks of their own."""
+    n = 256 * 6 + 40
+    g = torch.randn(n, generator=torch.Generator().manual_seed(3), dtype=F64)
+    g[:256] *= 1e-30
+    g[256:512] *= 1e-3
+    g[300:310] = 1e-36
+    g[512:768] = 0.0
+    g[768:1024] *= 1e-42                              # subnormal
+    g[1024:1280] *= 1e15
+    g[1100:1200] = 1e-10
+    g = g.float().cuda()
+    p = torch.zeros(n, device="cuda")
+    opt, want = ops.AdamW([p], lr=0.1, state_bits=bits), ref.AdamW([p], 0.1, bits=bits)
+    for _ in range(3):
+        opt.step([g])
+        want.step([g])
+        if bits == 8:
+            mc, vc, ms, vs = want.codes
+            assert torch.equal(opt.m_scale.cpu(), ms) and torch.equal(opt.v_scale.cpu(), vs)
+            assert torch.equal(opt.m.cpu() & 127, mc & 127) and torch.equal(opt.v.cpu(), vc)
+    # roots below sqrt of fp32's smallest squares vanish next to eps = 1e-8 and change p by less than 1e-10
+    assert (p.cpu().double() - want.p[0]).abs().max() < 3 * 0.1 * 1e-5 + 1e-10
+
+
+def test_a_root_above_zero_never_becomes_zero():
+    g = torch.full((256,), 1e-7, device="cuda")
+    g[0] = 1.0
+    p = torch.zeros(256, device="cuda")
+    opt = ops.AdamW([p], state_bits=8)
+    opt.step([g])
+    assert (opt.v.cpu()[1:] == 1).all() and opt.v.cpu()[0] == 0x7e
+    g[5] = 0.0
+    q = ops.AdamW([torch.zeros(256, device="cuda")], state_bits=8)
+    q.step([g])
+    assert q.v[5] == 0 and (q.v.cpu()[6:] == 1).all()
+
+
+def test_ties_go_to_the_even_code():
+    """beta1 = beta2 = 0 and a largest value of 448 * 2^k make the scale a power of two, so that values between two
+    codes are exact ties."""
+    between = (ref.VALUES[1:] + ref.VALUES[:-1]) / 2
+    g = torch.zeros(256, dtype=F64)
+    g[0] = 448.0
+    g[1:127] = between
+    g[128:254] = -between
+    g = (g * 2.0 ** -10).float().cuda()
+    opt = ops.AdamW([torch.zeros(256, device="cuda")], betas=(0.0, 0.0), state_bits=8)
+    opt.step([g])
+    assert opt.m_scale[0] == 2.0 ** -10
+    want = torch.arange(126)
+    want = want + want % 2
+    assert torch.equal(opt.m.cpu()[1:127].long(), want) and torch.equal(opt.m.cpu()[128:254].long() & 127, want)
+    assert torch.equal(opt.v.cpu()[1:127].long(), want.clamp(min=1))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_more_tensors_than_one_launch_lists(bits):
+    sizes = [(i * 37) % 411 for i in range(211)] + [70001]
+    params, lr = tensors(sizes, F32, 5, 0.5), 1e-2
+    want = ref.AdamW(params, lr, bits=bits)
+    opt = ops.AdamW(params, lr=lr, state_bits=bits)
+    for k in range(2):
+        grads = tensors(sizes, F32, 300 + k, 1e-3)
+        opt.step(grads)
+        want.step(grads)
+    check(opt, want, params, 2, ref.half_step(F32), lr)
+    n = ops.grad_norm(grads, 1.0)
+    assert n[0].item() == pytest.approx(float(torch.cat([g.cpu().double() for g in grads]).norm()), rel=1e-13)
+
+
+def test_types_mixed_in_one_list():
+    kinds = [F32, BF16, F16, BF16, F32, F16]
+    params = [tensors([777 + i], k, i, 0.5)[0] for i, k in enumerate(kinds)]
+    gk = [F32, BF16, F32, F32, F32, F16]
+    want = ref.AdamW(params, 1e-2)
+    opt = ops.AdamW(params, lr=1e-2)
+    for s in range(3):
+        grads = [tensors([777 + i], k, 50 + i + s, 1e-2)[0] for i, k in enumerate(gk)]
+        clip = ops.grad_norm(grads, 0.1)
+        assert clip[0].item() == pytest.approx(float(torch.cat([g.cpu().double() for g in grads]).norm()), rel=1e-13)
+        opt.step(grads, clip=clip)
+        want.step(grads, scale=clip[1].item())
+    # fp32 parameters have their place in the master copy too, unused
+    at = 0
+    for p, w in zip(params, want.p):
+        got = p.detach().cpu().double() if p.dtype == F32 else opt.master[at:at + p.numel()].cpu().double()
+        near(got, w, 12 * ref.half_step(F32), 3 * 40 * ref.half_step(F32) * 0.4, "p")
+        at += p.numel()
+
+
+@pytest.mark.parametrize("kind", [F32, F64, BF16, F16], ids=str)
+@pytest.mark.parametrize("sizes", [[1], [0, 5], [16384], [16385, 3, 100000], [3000001]])
+def test_norm(kind, sizes):
+    grads = tensors(sizes, kind, 9, 2.0)
+    want = float(torch.cat([g.cpu().double() for g in grads]).norm())
+    for limit in (want / 3, want * 3, math.inf):
+        got = ops.grad_norm(grads, limit).tolist()
+        # fp64 sums: n/256 additions at most in a row
+        assert got[0] == pytest.approx(want, rel=2.0 ** -53 * (sum(sizes) / 256 + 40))
+        assert got[1] == pytest.approx(min(1.0, limit / want), rel=1e-12)
+    assert torch.equal(ops.grad_norm(grads, 1.0), ops.grad_norm(grads, 1.0))       # the same order every time
+
+
+def test_norm_of_nothing_and_of_what_is_not_finite():
+    z = torch.zeros(100, device="cuda")
+    assert ops.grad_norm([z], 1.0).tolist() == [0.0, 1.0]
+    assert ops.grad_norm([z[:0]], 1.0).tolist() == [0.0, 1.0]
+    for bad in (math.inf, -math.inf, math.nan):
+        g = torch.ones(5000, device="cuda")
+        g[4321] = bad
+        n, s = ops.grad_norm([z, g], 1.0).tolist()
+        assert not math.isfinite(n) and math.isnan(s)
+    big = torch.full((1000,), 3e38, device="cuda")                                     # squares beyond fp32
+    assert ops.grad_norm([big], 1.0)[0].item() == pytest.approx(float(big[0]) * math.sqrt(1000), rel=1e-12)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("kind", [F32, BF16], ids=str)
+def test_a_step_that_is_not_finite_is_left_out(kind, bits):
+    params = tensors([300, 5000], kind, 4, 0.5)
+    opt = ops.AdamW(params, state_bits=bits)
+    opt.step(tensors([300, 5000], kind, 5, 1e-2))
+    before, p0 = opt.state_dict(), [p.clone() for p in params]
+    grads = tensors([300, 5000], kind, 6, 1e-2)
+    grads[1][77] = math.inf
+    opt.step(grads, clip=ops.grad_norm(grads, 1.0))
+    after = opt.state_dict()
+    assert after["step"] == 1 == before["step"]
+    assert all(torch.equal(before[k], after[k]) for k in before if k != "step")
+    assert all(torch.equal(a, b) for a, b in zip(p0, params))
+    grads[1][77] = 0.5
+    opt.step(grads, clip=ops.grad_norm(grads, 1.0))
+    assert opt.step_count == 2 and not torch.equal(p0[1], params[1])
+
+
+def test_without_a_norm_what_is_not_finite_stays_in_its_place():
+    g = torch.full((1000,), 0.1, device="cuda")
+    g[300] = math.nan
+    g[600] = math.inf
+    p32, p8 = torch.zeros(1000, device="cuda"), torch.zeros(1000, device="cuda")
+    a, b = ops.AdamW([p32]), ops.AdamW([p8], state_bits=8)
+    for _ in range(2):
+        a.step([g])
+        b.step([g])
+    off = torch.isnan(p32)
+    assert off.nonzero().flatten().tolist() == [300, 600]
+    off = torch.isnan(b.moments()[0])
+    assert off[256:768].all() and not off[:256].any() and not off[768:].any()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_travels(bits):
+    sizes = [1000, 7]
+    params = tensors(sizes, BF16, 7, 0.5)
+    opt = ops.AdamW(params, state_bits=bits)
+    for k in range(3):
+        opt.step(tensors(sizes, BF16, 70 + k, 1e-2))
+    state = opt.state_dict()
+    other = [torch.zeros_like(p) for p in params]
+    new = ops.AdamW(other, state_bits=bits)
+    new.load_state_dict(state)
+    assert new.step_count == 3 and all(torch.equal(a, b) for a, b in zip(params, other))
+    g = tensors(sizes, BF16, 80, 1e-2)
+    opt.step(g)
+    new.step(g)
+    a, b = opt.state_dict(), new.state_dict()
+    assert a["step"] == b["step"] and all(torch.equal(a[k], b[k]) for k in a if k != "step")
+    assert all(torch.equal(x, y) for x, y in zip(params, other))
+    with pytest.raises(ValueError):
+        ops.AdamW(other, state_bits=40 - bits).load_state_dict(state)
+    with pytest.raises(ValueError):
+        ops.AdamW(other[:1], state_bits=bits).load_state_dict(state)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_captured_steps_count_on(bits):
+    """Norm and step in a graph, replayed between eager work; the count, the rate and the gradients are read on the device."""
+    sizes = [3000, 17, 256]
+    params, eager = tensors(sizes, F32, 8, 0.5), tensors(sizes, F32, 8, 0.5)
+    grads = tensors(sizes, F32, 9, 1e-2)
+    rate = torch.tensor([1e-2], dtype=F64, device="cuda")
+    opt, plain = ops.AdamW(params, lr=rate, state_bits=bits), ops.AdamW(eager, lr=rate, state_bits=bits)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for o in (opt, plain):
+            o.step(grads, clip=ops.grad_norm(grads, 0.3))
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        opt.step(grads, clip=ops.grad_norm(grads, 0.3))
+    assert opt.step_count == 1
+    for k in range(4):
+        for t, new in zip(grads, tensors(sizes, F32, 10 + k, 10.0 ** -k)):
+            t.copy_(new)
+        rate.fill_(10.0 ** -(2 + k))
+        g.replay()
+        plain.step(grads, clip=ops.grad_norm(grads, 0.3))
+        torch.cuda.synchronize()
+        assert opt.step_count == plain.step_count == 2 + k
+        assert all(torch.equal(a, b) for a, b in zip(params, eager))
+        assert all(torch.equal(a, b) for a, b in zip(opt.moments(), plain.moments()))
+
+
+def test_network_views_cover_the_flat_vector():
+    z = L.geometry(103, 9)
+    d = L.dims(z)
+    flat = torch.arange(d.nparams, dtype=F32, device="cuda")
+    views = ops.param_views(flat, z)
+    assert [v.numel() for v in views] == [3420, 20, 100 * d.pout, 100, 900, 9]
+    assert torch.equal(torch.cat(views), flat)
+
+
+def test_refused():
+    p, g = torch.zeros(10, device="cuda"), torch.zeros(10, device="cuda")
+    opt = ops.AdamW([p])
+    two = torch.zeros(4, 6, device="cuda")
+    for call, err in [
+        (lambda: ops.AdamW([]), ValueError),
+        (lambda: ops.AdamW([p.cpu()]), TypeError),
+        (lambda: ops.AdamW([p.int()]), TypeError),
+        (lambda: ops.AdamW([two.t()]), ValueError),
+        (lambda: ops.AdamW([p, p[5:]]), ValueError),
+        (lambda: ops.AdamW([p, p.double()]), TypeError),
+        (lambda: ops.AdamW([p.double()], state_bits=8), TypeError),
+        (lambda: ops.AdamW([p], state_bits=16), ValueError),
+        (lambda: ops.AdamW([p], betas=(0.9, 1.0)), ValueError),
+        (lambda: ops.AdamW([p], eps=-1.0), ValueError),
+        (lambda: ops.AdamW([p], weight_decay=[0.1, 0.1]), ValueError),
+        (lambda: opt.step([]), ValueError),
+        (lambda: opt.step([g[:9]]), ValueError),
+        (lambda: opt.step([g.bfloat16()]), TypeError),
+        (lambda: opt.step([g.cpu()]), TypeError),
+        (lambda: opt.step([torch.zeros(20, device="cuda")[::2]]), ValueError),
+        (lambda: opt.step([g], clip=g), TypeError),
+        (lambda: opt.step([g], lr=g), TypeError),
+        (lambda: opt.load_state_dict({"step": -1, "m": opt.m, "v": opt.v}), ValueError),
+        (lambda: ops.grad_norm([], 1.0), ValueError),
+        (lambda: ops.grad_norm([g], 0.0), ValueError),
+        (lambda: ops.grad_norm([g], math.nan), ValueError),
+        (lambda: ops.grad_norm([g.cpu()], 1.0), TypeError),
+        (lambda: ops.grad_norm([two.t()], 1.0), ValueError),
+    ]:
+        with pytest.raises(err):
+            call()
+    assert opt.step_count == 0 and not p.any()

@@ -9,7 +9,7 @@ OBJ="${CCNN_OBJ_DIR:-/tmp/ccnn_obj}"
 HIPCC="${HIPCC:-/opt/rocm/bin/hipcc}"
 FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wall -Xclang -target-feature -Xclang -packed-fp32-ops $CCNN_EXTRA_FLAGS"
 mkdir -p "$OBJ" "$ROOT/gcn_amd/lib"
-SRCS="gather.hip forward.hip mbgd.hip tile.hip sgd.hip comm.hip host_prep.cpp profile.cpp"
+SRCS="gather.hip forward.hip mbgd.hip tile.hip sgd.hip comm.hip score.hip adamw.hip host_prep.cpp profile.cpp"
 newest_hdr=$(ls -t "$CSRC"/*.h "$ROOT/include/ccnn.h" | head -1)
 pids=()
 for s in $SRCS; do

@@ -62,19 +62,6 @@ __device__ __forceinline__ Sums<A> join(Sums<A> a, Sums<A> b)
 }
 
 template <typename A>
-__device__ __forceinline__ void add_element(Sums<A> &a, A x)
-{
-    if (x > a.m) shift(a, x);
-    if (a.m == ninf(A()) && x == a.m) return;   // nothing allowed so far
-    const A d = x - a.m, e = expw(d);
-    a.s += e;
-    if (e > A(0)) a.t += e * d;                 // -inf and far values weigh nothing, and 0 * inf is not wanted
-}
-
-template <typename A>
-__device__ __forceinline__ bool before(A v, int i, A w, int j) { return v > w || (v == w && i < j); }
-
-template <typename A>
 __device__ __forceinline__ void finish_row(const Sums<A> &a, long r, A given, long y, int classes, const ScoreOut<A> &o)
 {
     const bool empty = a.m == ninf(A()) && a.s == A(0);
@@ -86,84 +73,513 @@ __device__ __forceinline__ void finish_row(const Sums<A> &a, long r, A given, lo
     if (o.entropy) o.entropy[r] = bad ? nan : empty ? A(0) : l - a.t / a.s;
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void log_probs_row(const T *__restrict__ logits, int classes, long stride, Targets targets,
-                                                     ScoreOut<Wide<T>> o)
+// ---------------------------------------------------------------------------- order of the alternatives
+// One whole number per element, larger = earlier: the value's order above the index's complement, so
+// that equal values (both zeros among them) come in the order of their indices.
+template <typename A> struct KeyOf { typedef unsigned long long type; };
+template <> struct KeyOf<double> { typedef unsigned __int128 type; };
+template <typename A> using Key = typename KeyOf<A>::type;
+
+__device__ __forceinline__ unsigned long long key_of(float v, unsigned i)
+{
+    const int u = __float_as_int(v + 0.0f);
+    return (unsigned long long)(unsigned)(u ^ ((u >> 31) | (int)0x80000000)) << 32 | (unsigned)~i;
+}
+__device__ __forceinline__ unsigned __int128 key_of(double v, unsigned i)
+{
+    const long long u = __double_as_longlong(v + 0.0);
+    return (unsigned __int128)(unsigned long long)(u ^ ((u >> 63) | (long long)0x8000000000000000ull)) << 32 | (unsigned)~i;
+}
+__device__ __forceinline__ unsigned key_index(unsigned long long k) { return ~(unsigned)k; }
+__device__ __forceinline__ unsigned key_index(unsigned __int128 k) { return ~(unsigned)k; }
+__device__ __forceinline__ float key_value(unsigned long long k)
+{
+    const int u = (int)(k >> 32);
+    return __int_as_float(u ^ (~(u >> 31) | (int)0x80000000));
+}
+__device__ __forceinline__ double key_value(unsigned __int128 k)
+{
+    const long long u = (long long)(k >> 32);
+    return __longlong_as_double(u ^ (~(u >> 63) | (long long)0x8000000000000000ull));
+}
+__device__ __forceinline__ unsigned long long xor_lane(unsigned long long k, int off) { return __shfl_xor(k, off); }
+__device__ __forceinline__ unsigned __int128 xor_lane(unsigned __int128 k, int off)
+{
+    return (unsigned __int128)__shfl_xor((unsigned long long)(k >> 64), off) << 64 | __shfl_xor((unsigned long long)k, off);
+}
+
+template <typename A>
+__device__ __forceinline__ void put_top(const ScoreOut<A> &o, long r, int place, Key<A> k, A m, A l)
+{
+    const A v = key_value(k);
+    const bool bad = l != l;
+    o.top_index[r * o.top + place] = bad ? -1 : (int)key_index(k);
+    o.top_logp[r * o.top + place] = bad ? nan_of(A()) : v == ninf(A()) ? v : (v - m) - l;
+}
+
+// ---------------------------------------------------------------------------- up to 1024 classes
+// G lanes to a row, E elements to a lane, all of them in registers.  The sums are one pass over the
+// registers; alternatives are taken one after the other, the lane whose best was taken looking for its next.
+template <typename T, int G, int E>
+__global__ __launch_bounds__(256) void log_probs_small(const T *__restrict__ logits, long rows, int classes, long stride,
+                                                       Targets targets, ScoreOut<Wide<T>> o)
 {
     typedef Wide<T> A;
-    __shared__ A sm[256], ss[256], stt[256];
-    __shared__ int si[256];
-    const long r = blockIdx.x;
+    const int lane = threadIdx.x % G;
+    const long r = (long)blockIdx.x * (256 / G) + threadIdx.x / G;
+    if (r >= rows) return;               // whole groups leave: the others' exchanges stay among themselves
     const T *row = logits + r * stride;
-    const int tid = threadIdx.x;
-    Sums<A> a = {ninf(A()), A(0), A(0)};
-    for (int j = tid; j < classes; j += 256) add_element(a, (A)widen(row[j]));
-    sm[tid] = a.m, ss[tid] = a.s, stt[tid] = a.t;
-    __syncthreads();
-    for (int h = 128; h > 0; h >>= 1) {
-        if (tid < h) {
-            a = join(a, {sm[tid + h], ss[tid + h], stt[tid + h]});
-            sm[tid] = a.m, ss[tid] = a.s, stt[tid] = a.t;
-        }
-        __syncthreads();
+    A x[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const int j = e * G + lane;
+        x[e] = j < classes ? (A)widen(row[j]) : ninf(A());
     }
-    a = {sm[0], ss[0], stt[0]};
     const long y = targets.at(r);
-    if (tid == 0) finish_row(a, r, y >= 0 && y < classes ? (A)widen(row[y]) : A(0), y, classes, o);
-    const bool bad = !(a.s == a.s);
-    const A l = a.s == A(0) ? ninf(A()) : logw(a.s);
-    A last = A(0);
-    int lasti = -1;
+    const A given = lane == 0 && y >= 0 && y < classes ? (A)widen(row[y]) : A(0);
+    A m = x[0];
+#pragma unroll
+    for (int e = 1; e < E; e++) m = x[e] > m ? x[e] : m;
+#pragma unroll
+    for (int off = G / 2; off > 0; off >>= 1) {
+        const A w = __shfl_xor(m, off);
+        m = w > m ? w : m;
+    }
+    const A from = m == ninf(A()) ? A(0) : m;
+    A s = 0, t = 0;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const A d = x[e] - from, w = expw(d);
+        s += w;
+        t += w * (d < A(-1e4) ? A(-1e4) : d);       // 0 * inf is not wanted
+    }
+#pragma unroll
+    for (int off = G / 2; off > 0; off >>= 1) {
+        s += __shfl_xor(s, off);
+        t += __shfl_xor(t, off);
+    }
+    const Sums<A> sums = {m, s, t};
+    if (lane == 0) finish_row(sums, r, given, y, classes, o);
+    if (o.top == 0) return;
+    const A l = m == ninf(A()) && s == A(0) ? ninf(A()) : logw(s);
+    Key<A> key[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) key[e] = e * G + lane < classes ? key_of(x[e], e * G + lane) : Key<A>(0);
+    Key<A> best = 0;
+#pragma unroll
+    for (int e = 0; e < E; e++) best = key[e] > best ? key[e] : best;
     for (int k = 0; k < o.top; k++) {
-        __syncthreads();
-        A v = ninf(A());
-        int i = 0x7fffffff;
-        for (int j = tid; j < classes; j += 256) {
-            const A x = widen(row[j]);
-            if ((k == 0 || before(last, lasti, x, j)) && (before(x, j, v, i))) v = x, i = j;
+        Key<A> high = best;
+#pragma unroll
+        for (int off = G / 2; off > 0; off >>= 1) {
+            const Key<A> w = xor_lane(high, off);
+            high = w > high ? w : high;
         }
-        sm[tid] = v, si[tid] = i;
-        __syncthreads();
-        for (int h = 128; h > 0; h >>= 1) {
-            if (tid < h && before(sm[tid + h], si[tid + h], sm[tid], si[tid])) sm[tid] = sm[tid + h], si[tid] = si[tid + h];
-            __syncthreads();
-        }
-        last = sm[0], lasti = si[0];
-        if (tid == 0) {
-            o.top_index[r * o.top + k] = bad ? -1 : lasti;
-            o.top_logp[r * o.top + k] = bad ? nan_of(A()) : last == ninf(A()) ? last : (last - a.m) - l;
+        if (lane == 0) put_top(o, r, k, high, m, l);
+        if (best == high) {
+            best = 0;
+#pragma unroll
+            for (int e = 0; e < E; e++) best = key[e] < high && key[e] > best ? key[e] : best;
         }
     }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void log_probs_grad_row(const T *logits, int classes, long stride, Targets targets,
-                                                          const Wide<T> *__restrict__ stats, const Wide<T> *__restrict__ entropy,
-                                                          const Wide<T> *__restrict__ d_logp,
-                                                          const Wide<T> *__restrict__ d_entropy, T *d_logits, long d_stride)
+// ---------------------------------------------------------------------------- more classes
+// A workgroup streams a slice of a row, 16 bytes a load.  Each thread keeps the running sums and its
+// largest element with the load it came in.  The k-th largest of 64 groups' largest is a bar that the
+// top k elements all reach and few others do; only the threads that hold such an element look at their part
+// again, what reaches the bar is collected in LDS and put in order by counting.
+constexpr int SLICE_THREADS = 512;
+constexpr int CANDIDATES = 1024;
+
+template <typename A>
+struct SliceOut {
+    Sums<A> *sums;    // [rows][slices], null: one slice, results go straight to ScoreOut
+    Key<A> *keys;     // [rows][slices][top]
+    int slices;
+    long length;      // elements of a slice (the last may be shorter), a multiple of the load width
+};
+
+template <typename A>
+struct SliceLds {
+    Key<A> key[SLICE_THREADS];
+    Key<A> found[CANDIDATES];
+    A m[SLICE_THREADS / 64], s[SLICE_THREADS / 64], t[SLICE_THREADS / 64];
+    Key<A> bar;
+    int owners[SLICE_THREADS];
+    int n_owners, n_found;
+};
+
+template <typename K>
+__device__ __forceinline__ K wave_max(K k)
+{
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        const K w = xor_lane(k, off);
+        k = w > k ? w : k;
+    }
+    return k;
+}
+
+// k-th largest (k >= 1) of the wave's 64 keys; equal keys count one by one.
+template <typename K>
+__device__ __forceinline__ K wave_kth(K mine, int k, K *lds)
+{
+    const int lane = threadIdx.x & 63;
+    lds[lane] = mine;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+    int rank = 0;
+    for (int j = 0; j < 64; j++) {
+        const K w = lds[j];
+        rank += w > mine || (w == mine && j < lane);
+    }
+    const unsigned long long at = __ballot(rank == k - 1);
+    return lds[__ffsll((unsigned long long)at) - 1];
+}
+
+// The first `top` of n keys in LDS, handed to put(place, key) in falling order.
+template <typename K, typename Put>
+__device__ __forceinline__ void in_order(const K *keys, int n, int top, Put put)
+{
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+        const K mine = keys[i];
+        int rank = 0;
+        for (int j = 0; j < n; j++) rank += keys[j] > mine;
+        if (rank < top) put(rank, mine);
+    }
+}
+
+// The same from any number of keys, one round over all of them for each place.
+template <typename K, typename Get, typename Put>
+__device__ __forceinline__ void in_rounds(Get get, int n, int top, K *lds, Put put)
+{
+    K last = ~K(0);
+    for (int k = 0; k < top; k++) {
+        K high = 0;
+        for (int j = threadIdx.x; j < n; j += blockDim.x) {
+            const K w = get(j);
+            high = w < last && w > high ? w : high;
+        }
+        high = wave_max(high);
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = high;
+        __syncthreads();
+        high = lds[0];
+        for (int w = 1; w < (int)(blockDim.x >> 6); w++) high = lds[w] > high ? lds[w] : high;
+        if (threadIdx.x == 0) put(k, high);
+        last = high;
+    }
+}
+
+template <typename T, bool ENTROPY>
+__global__ __launch_bounds__(SLICE_THREADS) void log_probs_slice(const T *__restrict__ logits, int classes, long stride,
+                                                                 Targets targets, ScoreOut<Wide<T>> o, SliceOut<Wide<T>> part)
 {
     typedef Wide<T> A;
+    constexpr int W = 16 / sizeof(T), NT = SLICE_THREADS, U = 4;
+    __shared__ SliceLds<A> lds;
+    const long r = blockIdx.y;
+    const int slice = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const long begin = slice * part.length;
+    const int n = (int)min((long)classes - begin, part.length);
+    const T *row = logits + r * stride + begin;
+    const int loads = n / W;                    // whole loads; the rest of the row is one element a thread
+    A m = ninf(A()), s = 0, t = 0, best = ninf(A());
+    int best_at = -1;
+    auto take = [&](const A *x, int count, int at) {
+        A high = x[0];
+        for (int e = 1; e < count; e++) high = x[e] > high ? x[e] : high;
+        if (high > best || best_at < 0) best = high, best_at = at;
+        const A to = high > m ? high : m, from = to == ninf(A()) ? A(0) : to;
+        A f = m - to;
+        f = m == to ? A(1) : expw(f < A(-1e4) ? A(-1e4) : f);
+        if (ENTROPY) t = (t + (m == to ? A(0) : (m - to < A(-1e4) ? A(-1e4) : m - to)) * s) * f;
+        s *= f;
+        m = to;
+        for (int e = 0; e < count; e++) {
+            const A d = x[e] - from, w = expw(d);
+            s += w;
+            if (ENTROPY) t += w * (d < A(-1e4) ? A(-1e4) : d);
+        }
+    };
+    int i = tid;
+    for (; i + (U - 1) * NT < loads; i += U * NT) {
+        Pack<T, W> p[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) p[u] = load_pack<T, W>(row + (long)(i + u * NT) * W);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            A x[W];
+#pragma unroll
+            for (int e = 0; e < W; e++) x[e] = widen(p[u].v[e]);
+            take(x, W, i + u * NT);
+        }
+    }
+    for (; i < loads; i += NT) {
+        const Pack<T, W> p = load_pack<T, W>(row + (long)i * W);
+        A x[W];
+#pragma unroll
+        for (int e = 0; e < W; e++) x[e] = widen(p.v[e]);
+        take(x, W, i);
+    }
+    const int rest = n - loads * W;
+    // the last, partial load belongs to the thread whose turn it is
+    if (rest > 0 && tid == loads % NT) {
+        A x[W];
+#pragma unroll
+        for (int e = 0; e < W; e++) x[e] = e < rest ? (A)widen(row[(long)loads * W + e]) : ninf(A());
+        take(x, W, loads);
+    }
+
+    Sums<A> sums = {m, s, t};
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1)
+        sums = join(sums, {__shfl_xor(sums.m, off), __shfl_xor(sums.s, off), __shfl_xor(sums.t, off)});
+    if (lane == 0) lds.m[wave] = sums.m, lds.s[wave] = sums.s, lds.t[wave] = sums.t;
+    if (o.top) lds.key[tid] = best_at < 0 ? Key<A>(0) : key_of(best, best_at);
+    if (tid == 0) lds.n_owners = lds.n_found = 0;
+    __syncthreads();
+    sums = {lds.m[0], lds.s[0], lds.t[0]};
+    for (int w = 1; w < NT / 64; w++) sums = join(sums, {lds.m[w], lds.s[w], lds.t[w]});
+    if (tid == 0) {
+        if (part.sums) part.sums[r * part.slices + slice] = sums;
+        else {
+            const long y = targets.at(r);
+            finish_row(sums, r, y >= 0 && y < classes ? (A)widen(logits[r * stride + y]) : A(0), y, classes, o);
+        }
+    }
+    if (!o.top) return;
+    const A l = sums.m == ninf(A()) && sums.s == A(0) ? ninf(A()) : logw(sums.s);
+    auto put = [&](int place, Key<A> k) {
+        if (part.sums) part.keys[(r * part.slices + slice) * o.top + place] = k;
+        else put_top(o, r, place, k, sums.m, l);
+    };
+    if (wave == 0) {
+        Key<A> high = lds.key[lane];
+        for (int w = 1; w < NT / 64; w++) high = lds.key[w * 64 + lane] > high ? lds.key[w * 64 + lane] : high;
+        const Key<A> bar = wave_kth(high, o.top, lds.found);
+        if (lane == 0) lds.bar = bar;
+    }
+    __syncthreads();
+    const Key<A> bar = lds.bar;
+    if (best_at >= 0 && key_of(best, best_at) >= bar) lds.owners[atomicAdd(&lds.n_owners, 1)] = tid;
+    __syncthreads();
+    const int turns = (loads + (rest > 0) + NT - 1) / NT;
+    for (int task = tid; task < lds.n_owners * turns; task += NT) {
+        const int at = lds.owners[task / turns] + (task % turns) * NT;
+        const int count = at < loads ? W : at == loads ? rest : 0;
+        for (int e = 0; e < count; e++) {
+            const A x = widen(row[(long)at * W + e]);
+            if (key_of(x, at) >= bar) {
+                const int place = atomicAdd(&lds.n_found, 1);
+                if (place < CANDIDATES) lds.found[place] = key_of(x, (unsigned)(begin + (long)at * W + e));
+            }
+        }
+    }
+    __syncthreads();
+    if (lds.n_found <= CANDIDATES) {
+        in_order(lds.found, lds.n_found, o.top, put);
+        if (part.sums)     // a last slice shorter than the list: nothing behind its elements
+            for (int place = lds.n_found + tid; place < o.top; place += NT) put(place, Key<A>(0));
+    } else   // too many elements of a few threads reach the bar: a row ordered on their stride
+        in_rounds([&](int j) { return key_of((A)widen(row[j]), (unsigned)(begin + j)); }, n, o.top, lds.key, put);
+}
+
+// Joins a row's slices: their sums, and their lists of alternatives through the same bar.
+template <typename T>
+__global__ __launch_bounds__(256) void log_probs_join(const T *__restrict__ logits, int classes, long stride, Targets targets,
+                                                      ScoreOut<Wide<T>> o, SliceOut<Wide<T>> part)
+{
+    typedef Wide<T> A;
+    __shared__ Key<A> found[CANDIDATES], high_of[64];
+    __shared__ Key<A> bar;
+    __shared__ int n_found;
     const long r = blockIdx.x;
-    const long y = targets.at(r);
-    const A m = stats[2 * r], l = stats[2 * r + 1];
-    const A dl = d_logp && y >= 0 ? d_logp[r] : A(0), dh = d_entropy ? d_entropy[r] : A(0), h = d_entropy ? entropy[r] : A(0);
-    const bool empty = m == ninf(A()), bad = y >= classes;
-    for (int j = threadIdx.x; j < classes; j += 256) {
-        const A lp = ((A)widen(logits[r * stride + j]) - m) - l, p = expw(lp);
+    const int tid = threadIdx.x, lane = tid & 63;
+    const Sums<A> *in = part.sums + r * part.slices;
+    Sums<A> sums = {ninf(A()), A(0), A(0)};
+    for (int k = lane; k < part.slices; k += 64) sums = join(sums, in[k]);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1)
+        sums = join(sums, {__shfl_xor(sums.m, off), __shfl_xor(sums.s, off), __shfl_xor(sums.t, off)});
+    // lane 0's: a contracted sum differs in its last bit between the two sides of an exchange
+    sums = {__shfl(sums.m, 0), __shfl(sums.s, 0), __shfl(sums.t, 0)};
+    if (tid == 0) {
+        const long y = targets.at(r);
+        finish_row(sums, r, y >= 0 && y < classes ? (A)widen(logits[r * stride + y]) : A(0), y, classes, o);
+        n_found = 0;
+    }
+    if (!o.top) return;
+    const A l = sums.m == ninf(A()) && sums.s == A(0) ? ninf(A()) : logw(sums.s);
+    const int n = part.slices * o.top;
+    const Key<A> *keys = part.keys + r * n;
+    // groups take the slices' lists place by place, so that a row's first alternatives meet in few of them
+    // only if few slices hold them all
+    auto transposed = [&](int k) { return keys[(k % part.slices) * o.top + k / part.slices]; };
+    if (tid < 64) {
+        Key<A> high = 0;
+        for (int k = lane; k < n; k += 64) {
+            const Key<A> w = transposed(k);
+            high = w > high ? w : high;
+        }
+        const Key<A> b = n < 64 ? Key<A>(0) : wave_kth(high, o.top, high_of);
+        if (lane == 0) bar = b;
+    }
+    __syncthreads();
+    for (int k = tid; k < n; k += 256)
+        if (keys[k] >= bar) {
+            const int place = atomicAdd(&n_found, 1);
+            if (place < CANDIDATES) found[place] = keys[k];
+        }
+    __syncthreads();
+    auto put = [&](int place, Key<A> k) { put_top(o, r, place, k, sums.m, l); };
+    if (n_found <= CANDIDATES) in_order(found, n_found, o.top, put);
+    else in_rounds([&](int j) { return keys[j]; }, n, o.top, high_of, put);
+}
+
+// ---------------------------------------------------------------------------- gradient
+template <typename A>
+struct GradIn {
+    const A *stats, *entropy, *d_logp, *d_entropy;
+};
+
+// What one row's elements have in common.
+template <typename A>
+struct GradRow {
+    A m, l, dl, dh, h;
+    long y;
+    bool empty, bad;
+    __device__ GradRow(const GradIn<A> &in, const Targets &targets, long r, int classes)
+    {
+        y = targets.at(r);
+        m = in.stats[2 * r], l = in.stats[2 * r + 1];
+        dl = in.d_logp && y >= 0 ? in.d_logp[r] : A(0);
+        dh = in.d_entropy ? in.d_entropy[r] : A(0);
+        h = in.d_entropy ? in.entropy[r] : A(0);
+        empty = m == ninf(A());
+        bad = y >= classes;
+    }
+    __device__ __forceinline__ A at(A x, long j) const
+    {
+        const A lp = (x - m) - l, p = expw(lp);
         A g = (y == j ? dl : A(0)) - dl * p;
         if (p > A(0)) g -= dh * p * (lp + h);
-        narrow(bad ? nan_of(A()) : empty ? A(0) : g, d_logits[r * d_stride + j]);
+        return bad ? nan_of(A()) : empty ? A(0) : g;
     }
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void log_probs_grad_small(const T *logits, long rows, int classes, long stride,
+                                                            Targets targets, GradIn<Wide<T>> in, T *d_logits, long d_stride,
+                                                            int lanes)
+{
+    typedef Wide<T> A;
+    const long r = ((long)blockIdx.x * 256 + threadIdx.x) / lanes;
+    if (r >= rows) return;
+    const GradRow<A> row(in, targets, r, classes);
+    for (int j = threadIdx.x % lanes; j < classes; j += lanes)
+        narrow(row.at((A)widen(logits[r * stride + j]), j), d_logits[r * d_stride + j]);
+}
+
+constexpr int GRAD_LOADS = 4;
+
+template <typename T>
+__global__ __launch_bounds__(256) void log_probs_grad_wide(const T *logits, int classes, long stride, Targets targets,
+                                                           GradIn<Wide<T>> in, T *d_logits, long d_stride)
+{
+    typedef Wide<T> A;
+    constexpr int W = 16 / sizeof(T);
+    // rows from the last to the first: those the forward pass read last are still in the memory-side cache
+    const long r = gridDim.y - 1 - blockIdx.y;
+    const T *x = logits + r * stride;
+    T *d = d_logits + r * d_stride;
+    const int first = blockIdx.x * (256 * GRAD_LOADS * W) + threadIdx.x * W;
+    Pack<T, W> p[GRAD_LOADS];
+#pragma unroll
+    for (int u = 0; u < GRAD_LOADS; u++) {
+        const int j = first + u * 256 * W;
+        if (j + W <= classes) p[u] = load_pack<T, W>(x + j);
+    }
+    const GradRow<A> row(in, targets, r, classes);
+#pragma unroll
+    for (int u = 0; u < GRAD_LOADS; u++) {
+        const int j = first + u * 256 * W;
+        if (j + W <= classes) {
+#pragma unroll
+            for (int e = 0; e < W; e++) narrow(row.at((A)widen(p[u].v[e]), j + e), p[u].v[e]);
+            store_pack<T, W>(d + j, p[u]);
+        } else {
+            for (int e = j; e < classes; e++) narrow(row.at((A)widen(x[e]), e), d[e]);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------- host
+constexpr int SMALL_CLASSES = 1024;
+
+// Slices of a row: enough of them to give every CU two workgroups, none shorter than a load per thread.
+inline int slices_of(long rows, int classes, int size, long *length)
+{
+    const long width = 16 / size, turn = width * SLICE_THREADS;
+    long want = (512 + rows - 1) / rows, most = (classes + turn - 1) / turn;
+    if (want > most) want = most;
+    if (want < 1) want = 1;
+    *length = ((classes + want - 1) / want + width - 1) / width * width;
+    return (int)((classes + *length - 1) / *length);
+}
+
+template <typename A>
+size_t slice_bytes(long rows, int classes, int top, int size)
+{
+    long length;
+    if (classes <= SMALL_CLASSES) return 0;
+    const int slices = slices_of(rows, classes, size, &length);
+    if (slices == 1) return 0;
+    return align_up(rows * slices * sizeof(Sums<A>)) + align_up(rows * slices * (size_t)top * sizeof(Key<A>));
 }
 
 template <typename T>
 int score_impl(const void *logits, long rows, int classes, long stride, Targets targets, int top, void *logp, void *entropy,
-               void *top_logp, int *top_index, void *stats, hipStream_t st)
+               void *top_logp, int *top_index, void *stats, void *workspace, hipStream_t st)
 {
     typedef Wide<T> A;
     const ScoreOut<A> o = {(A *)logp, (A *)entropy, (A *)top_logp, (A *)stats, top_index, top};
-    launch("log_probs_row", log_probs_row<T>, dim3((unsigned)rows), dim3(256), 0, st, (const T *)logits, classes, stride, targets, o);
-    CCNN_LAUNCH_CHECK();
+    const T *x = (const T *)logits;
+    if (classes <= SMALL_CLASSES) {
+        typedef void (*Kern)(const T *, long, int, long, Targets, ScoreOut<A>);
+        const int group = classes <= 16 ? 1 : classes <= 256 ? 16 : 64;
+        const Kern kern = classes <= 16    ? log_probs_small<T, 1, 16>
+                          : classes <= 64  ? log_probs_small<T, 16, 4>
+                          : classes <= 256 ? log_probs_small<T, 16, 16>
+                                           : log_probs_small<T, 64, 16>;
+        const long per = 256 / group;
+        launch("log_probs_small", kern, dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, st, x, rows, classes, stride,
+               targets, o);
+        CCNN_LAUNCH_CHECK();
+        return 0;
+    }
+    SliceOut<A> part = {};
+    part.slices = slices_of(rows, classes, sizeof(T), &part.length);
+    if (part.slices > 1) {
+        Carver c(workspace);
+        part.sums = c.take<Sums<A>>(rows * part.slices);
+        part.keys = c.take<Key<A>>(rows * part.slices * (size_t)top);
+    }
+    // 65535 rows at most in a grid's second dimension
+    for (long r0 = 0; r0 < rows; r0 += 65535) {
+        const long nr = rows - r0 < 65535 ? rows - r0 : 65535;
+        ScoreOut<A> os = {o.logp + r0, o.entropy ? o.entropy + r0 : nullptr, top ? o.top_logp + r0 * top : nullptr,
+                          o.stats + 2 * r0, top ? o.top_index + r0 * top : nullptr, top};
+        const Targets ts = {(const char *)targets.p + r0 * targets.bytes, targets.bytes};
+        launch("log_probs_slice", entropy ? log_probs_slice<T, true> : log_probs_slice<T, false>,
+               dim3((unsigned)part.slices, (unsigned)nr), dim3(SLICE_THREADS), 0, st, x + r0 * stride, classes, stride, ts, os, part);
+        CCNN_LAUNCH_CHECK();
+    }
+    if (part.slices > 1) {
+        launch("log_probs_join", log_probs_join<T>, dim3((unsigned)rows), dim3(256), 0, st, x, classes, stride, targets, o, part);
+        CCNN_LAUNCH_CHECK();
+    }
     return 0;
 }
 
@@ -173,10 +589,27 @@ int score_grad_impl(const void *logits, long rows, int classes, long stride, Tar
                     hipStream_t st)
 {
     typedef Wide<T> A;
-    launch("log_probs_grad_row", log_probs_grad_row<T>, dim3((unsigned)rows), dim3(256), 0, st, (const T *)logits, classes,
-           stride, targets, (const A *)stats, (const A *)entropy, (const A *)d_logp, (const A *)d_entropy, (T *)d_logits,
-           d_stride);
-    CCNN_LAUNCH_CHECK();
+    const T *x = (const T *)logits;
+    T *d = (T *)d_logits;
+    const GradIn<A> in = {(const A *)stats, (const A *)entropy, (const A *)d_logp, (const A *)d_entropy};
+    if (classes <= SMALL_CLASSES) {
+        const int lanes = classes <= 16 ? 16 : 64;
+        const long per = 256 / lanes;
+        launch("log_probs_grad_small", log_probs_grad_small<T>, dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, st, x,
+               rows, classes, stride, targets, in, d, d_stride, lanes);
+        CCNN_LAUNCH_CHECK();
+        return 0;
+    }
+    const long tile = 256 * GRAD_LOADS * (16 / sizeof(T));
+    for (long r1 = rows; r1 > 0; r1 -= 65535) {
+        const long r0 = r1 > 65535 ? r1 - 65535 : 0;
+        const GradIn<A> is = {in.stats + 2 * r0, in.entropy ? in.entropy + r0 : nullptr, in.d_logp ? in.d_logp + r0 : nullptr,
+                              in.d_entropy ? in.d_entropy + r0 : nullptr};
+        const Targets ts = {(const char *)targets.p + r0 * targets.bytes, targets.bytes};
+        launch("log_probs_grad_wide", log_probs_grad_wide<T>, dim3((unsigned)((classes + tile - 1) / tile), (unsigned)(r1 - r0)),
+               dim3(256), 0, st, x + r0 * stride, classes, stride, ts, is, d + r0 * d_stride, d_stride);
+        CCNN_LAUNCH_CHECK();
+    }
     return 0;
 }
 
@@ -196,8 +629,8 @@ extern "C" {
 
 size_t ccnn_log_probs_workspace_bytes(long rows, int classes, int top, int type)
 {
-    (void)rows, (void)classes, (void)top, (void)type;
-    return 0;
+    if (!type_bytes(type) || rows <= 0 || classes < 1 || top < 0) return 0;
+    return type == CCNN_TYPE_F64 ? slice_bytes<double>(rows, classes, top, 8) : slice_bytes<float>(rows, classes, top, type_bytes(type));
 }
 
 int ccnn_log_probs(const void *logits, int type, long rows, int classes, long stride, const void *targets, int target_bytes,
@@ -208,13 +641,14 @@ int ccnn_log_probs(const void *logits, int type, long rows, int classes, long st
     if (top < 0 || top > CCNN_MAX_TOP || top > classes) return CCNN_E_INVALID;
     if (rows == 0) return 0;
     if (!logp || !stats || (top > 0 && (!top_logp || !top_index))) return CCNN_E_INVALID;
-    if (workspace_bytes < ccnn_log_probs_workspace_bytes(rows, classes, top, type)) return CCNN_E_WORKSPACE;
+    const size_t need = ccnn_log_probs_workspace_bytes(rows, classes, top, type);
+    if (workspace_bytes < need || (need && !workspace)) return CCNN_E_WORKSPACE;
     const Targets t = {targets, target_bytes};
     switch (type) {
-    case CCNN_TYPE_F32: return score_impl<float>(logits, rows, classes, stride, t, top, logp, entropy, top_logp, top_index, stats, (hipStream_t)stream);
-    case CCNN_TYPE_F64: return score_impl<double>(logits, rows, classes, stride, t, top, logp, entropy, top_logp, top_index, stats, (hipStream_t)stream);
-    case CCNN_TYPE_BF16: return score_impl<Bf16>(logits, rows, classes, stride, t, top, logp, entropy, top_logp, top_index, stats, (hipStream_t)stream);
-    default: return score_impl<F16>(logits, rows, classes, stride, t, top, logp, entropy, top_logp, top_index, stats, (hipStream_t)stream);
+    case CCNN_TYPE_F32: return score_impl<float>(logits, rows, classes, stride, t, top, logp, entropy, top_logp, top_index, stats, workspace, (hipStream_t)stream);
+    case CCNN_TYPE_F64: return score_impl<double>(logits, rows, classes, stride, t, top, logp, entropy, top_logp, top_index, stats, workspace, (hipStream_t)stream);
+    case CCNN_TYPE_BF16: return score_impl<Bf16>(logits, rows, classes, stride, t, top, logp, entropy, top_logp, top_index, stats, workspace, (hipStream_t)stream);
+    default: return score_impl<F16>(logits, rows, classes, stride, t, top, logp, entropy, top_logp, top_index, stats, workspace, (hipStream_t)stream);
     }
 }
 

@@ -5,6 +5,7 @@
 // kernel's arguments (LIST tensors a launch), every tensor is cut into chunks, and a workgroup finds
 // its chunk's tensor by bisection over the chunk counts.
 #include <cmath>
+#include <type_traits>
 
 #include "numeric.h"
 #include "profile.h"
@@ -36,39 +37,58 @@ __device__ __forceinline__ int find(const L &list, int chunk)
     return lo;
 }
 
-// Sum over a workgroup of 256 in a fixed order; the result is in thread 0.
+// Sum over a workgroup of N threads in a fixed order; the result is in every thread.
+template <int N>
 __device__ __forceinline__ double block_sum(double v, double *lds)
 {
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_down(v, off);
+    v = lanes_sum<64>(v);
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
     __syncthreads();
-    return lds[0] + lds[1] + lds[2] + lds[3];
+    v = 0;
+#pragma unroll
+    for (int w = 0; w < N / 64; w++) v += lds[w];
+    return v;
 }
 
 template <typename T>
 __global__ __launch_bounds__(256) void norm_partial(NormList list, double *__restrict__ partial)
 {
+    constexpr int W = 16 / sizeof(T), U = 8;
     __shared__ double lds[4];
     const int i = find(list, blockIdx.x);
-    const T *p = (const T *)list.data[i];
-    const long lo = (long)(blockIdx.x - list.chunk0[i]) * NORM_CHUNK;
-    const long n = min(list.n[i], lo + NORM_CHUNK);
+    const T *p = (const T *)list.data[i] + (long)(blockIdx.x - list.chunk0[i]) * NORM_CHUNK;
+    const int n = (int)min(list.n[i] - (long)(blockIdx.x - list.chunk0[i]) * NORM_CHUNK, NORM_CHUNK);
     double s = 0;
-    for (long k = lo + threadIdx.x; k < n; k += 256) {
-        const double g = widen(p[k]);
-        s += g * g;
+    for (int k = threadIdx.x * W; k < n; k += U * 256 * W) {
+        Pack<T, W> x[U];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (k + u * 256 * W + W <= n) x[u] = load_pack<T, W>(p + k + u * 256 * W);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int at = k + u * 256 * W;
+            if (at + W <= n) {
+#pragma unroll
+                for (int e = 0; e < W; e++) s += (double)widen(x[u].v[e]) * (double)widen(x[u].v[e]);
+            } else {
+                for (int j = at; j < n; j++) s += (double)widen(p[j]) * (double)widen(p[j]);
+            }
+        }
     }
-    s = block_sum(s, lds);
+    s = block_sum<256>(s, lds);
     if (threadIdx.x == 0) partial[blockIdx.x] = s;
 }
 
-__global__ __launch_bounds__(256) void norm_total(const double *__restrict__ partial, int n, double max_norm,
+constexpr int TOTAL_THREADS = 1024;
+
+__global__ __launch_bounds__(TOTAL_THREADS) void norm_total(const double *__restrict__ partial, int n, double max_norm,
                                                   double *__restrict__ out)
 {
-    __shared__ double lds[4];
+    __shared__ double lds[TOTAL_THREADS / 64];
     double s = 0;
-    for (int k = threadIdx.x; k < n; k += 256) s += partial[k];
-    s = block_sum(s, lds);
+#pragma unroll 4
+    for (int k = threadIdx.x; k < n; k += TOTAL_THREADS) s += partial[k];
+    s = block_sum<TOTAL_THREADS>(s, lds);
     if (threadIdx.x == 0) {
         const double norm = sqrt(s);
         out[0] = norm;
@@ -117,11 +137,10 @@ __global__ void adamw_clock(double *clock, double lr, const double *lr_device, d
 template <typename A>
 struct Rates {
     A scale, lr_decay, rate, root, eps;
-    double scale64;
     bool skip;
     __device__ Rates(const StepArgs &a, double decay)
         : scale((A)a.clock[6]), lr_decay((A)(a.clock[3] * decay)), rate((A)a.clock[4]), root((A)a.clock[5]), eps((A)a.eps),
-          scale64(a.clock[6]), skip(!(a.clock[6] == a.clock[6]))
+          skip(!(a.clock[6] == a.clock[6]))
     {
     }
 };
@@ -132,32 +151,77 @@ __device__ __forceinline__ A stepped(A p, A m, A v_root, const Rates<A> &r)
     return p - (r.lr_decay * p + r.rate * m / (v_root * r.root + r.eps));
 }
 
+// N elements at p + k of a tensor of n, zeros behind its end.
+template <int N, typename T>
+__device__ __forceinline__ Pack<T, N> load_some(const T *p, long k, long n)
+{
+    if (k + N <= n) return load_pack<T, N>(p + k);
+    Pack<T, N> r = {};
+#pragma unroll
+    for (int e = 0; e < N; e++)
+        if (k + e < n) r.v[e] = p[k + e];
+    return r;
+}
+template <int N, typename T>
+__device__ __forceinline__ void store_some(T *p, long k, long n, const Pack<T, N> &r)
+{
+    if (k + N <= n) {
+        store_pack<T, N>(p + k, r);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < N; e++)
+        if (k + e < n) p[k + e] = r.v[e];
+}
+
 template <typename P, typename G>
 __global__ __launch_bounds__(256) void adamw_wide(StepList list, StepArgs a)
 {
     typedef Wide<P> A;
     constexpr bool COPY = sizeof(P) == 2;   // the parameter is the rounding of its master copy
+    typedef std::conditional_t<COPY, float, P> S;
+    constexpr int W = 4, U = sizeof(P) == 8 ? 2 : 4;
     const int i = find(list, blockIdx.x);
     const Rates<A> r(a, list.decay[i]);
     if (r.skip) return;
     P *param = (P *)list.param[i];
     const G *grad = (const G *)list.grad[i];
     A *m = (A *)a.m + list.first[i], *v = (A *)a.v + list.first[i];
-    float *master = COPY ? a.master + list.first[i] : nullptr;
+    S *held;
+    if constexpr (COPY) held = a.master + list.first[i];
+    else held = param;
     const long lo = (long)(blockIdx.x - list.chunk0[i]) * STEP_CHUNK;
     const long n = min(list.n[i], lo + STEP_CHUNK);
     const A b1 = (A)(1 - a.beta1), b2 = (A)(1 - a.beta2);
-    for (long k = lo + threadIdx.x; k < n; k += 256) {
-        const A g = (A)widen(grad[k]) * r.scale;
-        const A mk = m[k] + b1 * (g - m[k]), vk = v[k] + b2 * (g * g - v[k]);
-        m[k] = mk;
-        v[k] = vk;
-        A p;
-        if constexpr (COPY) p = master[k];
-        else p = param[k];
-        p = stepped(p, mk, (A)sqrt(vk), r);
-        if constexpr (COPY) master[k] = p;
-        narrow(p, param[k]);
+    for (long k0 = lo + threadIdx.x * W; k0 < n; k0 += U * 256 * W) {
+        Pack<A, W> mk[U], vk[U];
+        Pack<S, W> pk[U];
+        Pack<G, W> gk[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const long k = k0 + u * 256 * W;
+            gk[u] = load_some<W>(grad, k, n);
+            mk[u] = load_some<W>(m, k, n);
+            vk[u] = load_some<W>(v, k, n);
+            pk[u] = load_some<W>(held, k, n);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const long k = k0 + u * 256 * W;
+            Pack<P, W> out;
+#pragma unroll
+            for (int e = 0; e < W; e++) {
+                const A g = (A)widen(gk[u].v[e]) * r.scale;
+                mk[u].v[e] += b1 * (g - mk[u].v[e]);
+                vk[u].v[e] += b2 * (g * g - vk[u].v[e]);
+                pk[u].v[e] = stepped((A)pk[u].v[e], mk[u].v[e], (A)sqrt(vk[u].v[e]), r);
+                narrow(pk[u].v[e], out.v[e]);
+            }
+            store_some<W>(m, k, n, mk[u]);
+            store_some<W>(v, k, n, vk[u]);
+            if constexpr (COPY) store_some<W>(held, k, n, pk[u]);
+            store_some<W>(param, k, n, out);
+        }
     }
 }
 
@@ -175,27 +239,10 @@ __device__ __forceinline__ unsigned encode8(double y)
     return (unsigned)(u >> 49) - ((1023u - 7u) << 3);
 }
 
-// Largest of 64 lanes; any NaN wins (compared as the bits of magnitudes).
-__device__ __forceinline__ float wave_high(double v)
-{
-    unsigned u = __float_as_uint(fabsf((float)v));
-    for (int off = 32; off > 0; off >>= 1) u = max(u, (unsigned)__shfl_xor((int)u, off));
-    return __uint_as_float(u);
-}
-
-// beta old + (1 - beta) new, every product and the sum rounded by itself.  With a beta like 9/10 the result
-// often lies exactly between two fp32 values, so a block's fp32 scale would hang on how the compiler
-// contracts the expression.
-__device__ __forceinline__ double decay_to(double beta, double old, double now)
-{
-#pragma clang fp contract(off)
-    const double a = beta * old, b = (1 - beta) * now;
-    return a + b;
-}
-
 __device__ __forceinline__ unsigned pack_codes(const double (&x)[4], float scale, bool floor)
 {
     unsigned w = 0;
+#pragma unroll
     for (int e = 0; e < 4; e++) {
         const double y = fabs(x[e]);
         unsigned c = scale > 0 ? encode8(fmin(y / scale, 448.0)) : scale == 0 ? 0u : 0x7fu;
@@ -207,72 +254,154 @@ __device__ __forceinline__ unsigned pack_codes(const double (&x)[4], float scale
     return w;
 }
 
-// One wave per block of 256 elements, four to a lane.
+// The same, for all but a few in a hundred blocks: y in fp32 is within 2^-22 of itself, so where it gives the
+// same codes a little larger and a little smaller, no border lies between it and the exact quotient.
+// Scales outside the range where that holds, and blocks with an undecided element, go the way above.
+__device__ __forceinline__ unsigned quick_codes(const double (&x)[4], float scale, bool floor)
+{
+    const float inv = 1.0f / scale;
+    unsigned up = 0, down = 0;
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        y[e] = (float)x[e] * inv;
+        if (floor) y[e] = x[e] > 0 ? fmaxf(y[e], 0x1p-9f) : y[e];
+    }
+    constexpr float MORE = 1.0f + 0x1p-21f, LESS = 1.0f - 0x1p-21f;
+    up = __builtin_amdgcn_cvt_pk_fp8_f32(y[0] * MORE, y[1] * MORE, up, false);
+    up = __builtin_amdgcn_cvt_pk_fp8_f32(y[2] * MORE, y[3] * MORE, up, true);
+    down = __builtin_amdgcn_cvt_pk_fp8_f32(y[0] * LESS, y[1] * LESS, down, false);
+    down = __builtin_amdgcn_cvt_pk_fp8_f32(y[2] * LESS, y[3] * LESS, down, true);
+    if (__any(up != down) || !(scale > 1e-30f && scale < 1e30f)) return pack_codes(x, scale, floor);
+    return up;
+}
+
+// beta old + (1 - beta) new, every product and the sum rounded by itself.  With a beta like 9/10 the result
+// often lies exactly between two fp32 values, so a block's fp32 scale would hang on how the compiler
+// contracts the expression.
+__device__ __forceinline__ double decay_to(double beta, double rest, double old, double now)
+{
+#pragma clang fp contract(off)
+    const double a = beta * old, b = rest * now;
+    return a + b;
+}
+
+// sqrt to the last bit or two: the hardware's 2^-24 start and two corrections.
+__device__ __forceinline__ double root64(double v)
+{
+    const double y = __builtin_amdgcn_rsq(v), h = 0.5 * y;
+    double s = v * y;
+    s = fma(fma(-s, s, v), h, s);
+    s = fma(fma(-s, s, v), h, s);
+    return v == 0 ? 0.0 : s;
+}
+
+// (largest magnitude of the block in fp32) / 448, NaN if one of them is not finite; any NaN's bits are above
+// all others'.
+__device__ __forceinline__ float block_scale(const double (&x)[4])
+{
+    unsigned u = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) u = max(u, __float_as_uint((float)x[e]) & 0x7fffffffu);
+    u = lanes_max<64>(u);
+    return u >= 0x7f800000u ? __builtin_nanf("") : __uint_as_float(u) / 448.0f;
+}
+
+// One wave per block of 256 elements, four to a lane, four blocks in flight.  Moments, root and step in fp64.
 template <typename P, typename G>
 __global__ __launch_bounds__(256) void adamw_coded(StepList list, StepArgs a)
 {
     constexpr bool COPY = sizeof(P) == 2;
+    typedef std::conditional_t<COPY, float, P> S;
+    constexpr int U = STEP_CHUNK / (4 * BLOCK);
     const int i = find(list, blockIdx.x);
-    const Rates<float> r(a, list.decay[i]);
+    const Rates<double> r(a, list.decay[i]);
     if (r.skip) return;
     P *param = (P *)list.param[i];
     const G *grad = (const G *)list.grad[i];
-    float *master = COPY ? a.master + list.first[i] : nullptr;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long lo = (long)(blockIdx.x - list.chunk0[i]) * STEP_CHUNK;
-    const long n = list.n[i], hi = min(n, lo + STEP_CHUNK);
-    for (long b = lo + wave * BLOCK; b < hi; b += 4 * BLOCK) {
-        const long blk = list.block[i] + b / BLOCK;
-        unsigned *mw = (unsigned *)a.m + blk * (BLOCK / 4) + lane, *vw = (unsigned *)a.v + blk * (BLOCK / 4) + lane;
-        const unsigned mc = *mw, vc = *vw;
-        const double ms = a.m_scale[blk], vs = a.v_scale[blk];
-        double m[4], v[4], root[4];
-        double hm = 0, hv = 0;
-        bool nan_m = false, nan_v = false;
+    S *held;
+    if constexpr (COPY) held = a.master + list.first[i];
+    else held = param;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long n = list.n[i], b0 = (long)(blockIdx.x - list.chunk0[i]) * STEP_CHUNK + wave * (U * BLOCK);
+    const long blk0 = list.block[i] + b0 / BLOCK;
+    const double rest1 = 1 - a.beta1, rest2 = 1 - a.beta2;
+    Pack<G, 4> gk[U];
+    Pack<S, 4> pk[U];
+    unsigned mc[U], vc[U];
+    float ms[U], vs[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        if (b0 + u * BLOCK >= n) break;
+        const long k = b0 + u * BLOCK + lane * 4;
+        gk[u] = load_some<4>(grad, k, n);
+        pk[u] = load_some<4>(held, k, n);
+        mc[u] = ((const unsigned *)a.m)[(blk0 + u) * (BLOCK / 4) + lane];
+        vc[u] = ((const unsigned *)a.v)[(blk0 + u) * (BLOCK / 4) + lane];
+        ms[u] = a.m_scale[blk0 + u];
+        vs[u] = a.v_scale[blk0 + u];
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        if (b0 + u * BLOCK >= n) break;
+        const long k = b0 + u * BLOCK + lane * 4;
+        double m[4], root[4];
+        Pack<P, 4> out;
+        const double old_m[4] = {__builtin_amdgcn_cvt_f32_fp8((int)mc[u], 0), __builtin_amdgcn_cvt_f32_fp8((int)mc[u], 1),
+                                 __builtin_amdgcn_cvt_f32_fp8((int)mc[u], 2), __builtin_amdgcn_cvt_f32_fp8((int)mc[u], 3)};
+        const double old_v[4] = {__builtin_amdgcn_cvt_f32_fp8((int)vc[u], 0), __builtin_amdgcn_cvt_f32_fp8((int)vc[u], 1),
+                                 __builtin_amdgcn_cvt_f32_fp8((int)vc[u], 2), __builtin_amdgcn_cvt_f32_fp8((int)vc[u], 3)};
+#pragma unroll
         for (int e = 0; e < 4; e++) {
-            const long k = b + lane * 4 + e;
-            const double g = k < n ? (double)widen(grad[k]) * r.scale64 : 0.0;
-            const double mo = decode8((mc >> (8 * e)) & 255) * ms, vo = decode8((vc >> (8 * e)) & 255) * vs;
-            m[e] = decay_to(a.beta1, mo, g);
-            v[e] = decay_to(a.beta2, vo * vo, g * g);
-            root[e] = sqrt(v[e]);
-            hm = fmax(hm, fabs(m[e]));
-            hv = fmax(hv, root[e]);
-            nan_m |= !(fabs(m[e]) < __builtin_huge_val());
-            nan_v |= !(v[e] < __builtin_huge_val());
+            const double g = (double)widen(gk[u].v[e]) * r.scale, vo = old_v[e] * (double)vs[u];
+            m[e] = decay_to(a.beta1, rest1, old_m[e] * (double)ms[u], g);
+            root[e] = root64(decay_to(a.beta2, rest2, vo * vo, g * g));
+            const double d = fma(root[e], r.root, r.eps);
+            double x = __builtin_amdgcn_rcp(d);
+            x = fma(fma(-d, x, 1.0), x, x);
+            const double p = pk[u].v[e];
+            pk[u].v[e] = (float)(p - fma(r.lr_decay, p, r.rate * m[e] * x));
+            narrow(pk[u].v[e], out.v[e]);
         }
-        const float high_m = wave_high(nan_m ? __builtin_nan("") : hm), high_v = wave_high(nan_v ? __builtin_nan("") : hv);
-        const float sm = high_m / 448.0f, sv = high_v / 448.0f;
-        *mw = pack_codes(m, sm, false);
-        *vw = pack_codes(root, sv, true);
-        if (lane == 0) a.m_scale[blk] = sm, a.v_scale[blk] = sv;
-        for (int e = 0; e < 4; e++) {
-            const long k = b + lane * 4 + e;
-            if (k >= n) break;
-            float p;
-            if constexpr (COPY) p = master[k];
-            else p = param[k];
-            p = stepped(p, (float)m[e], (float)root[e], r);
-            if constexpr (COPY) master[k] = p;
-            narrow(p, param[k]);
-        }
+        if constexpr (COPY) store_some<4>(held, k, n, pk[u]);
+        store_some<4>(param, k, n, out);
+        const float sm = block_scale(m), sv = block_scale(root);
+        ((unsigned *)a.m)[(blk0 + u) * (BLOCK / 4) + lane] = quick_codes(m, sm, false);
+        ((unsigned *)a.v)[(blk0 + u) * (BLOCK / 4) + lane] = quick_codes(root, sv, true);
+        if (lane == 0) a.m_scale[blk0 + u] = sm, a.v_scale[blk0 + u] = sv;
     }
 }
 
-__global__ __launch_bounds__(256) void adamw_decode(StepList list, const unsigned char *__restrict__ m,
-                                                    const unsigned char *__restrict__ v, const float *__restrict__ m_scale,
-                                                    const float *__restrict__ v_scale, float *__restrict__ m_out,
-                                                    float *__restrict__ v_out)
+__global__ __launch_bounds__(256) void adamw_decode(StepList list, const unsigned *__restrict__ m, const unsigned *__restrict__ v,
+                                                    const float *__restrict__ m_scale, const float *__restrict__ v_scale,
+                                                    float *__restrict__ m_out, float *__restrict__ v_out)
 {
+    constexpr int U = STEP_CHUNK / (4 * 256);
     const int i = find(list, blockIdx.x);
-    const long lo = (long)(blockIdx.x - list.chunk0[i]) * STEP_CHUNK;
-    const long n = min(list.n[i], lo + STEP_CHUNK);
-    for (long k = lo + threadIdx.x; k < n; k += 256) {
-        const long at = (long)list.block[i] * BLOCK + k, blk = at / BLOCK;
-        const double root = (double)decode8(v[at]) * v_scale[blk];
-        m_out[list.first[i] + k] = (float)((double)decode8(m[at]) * m_scale[blk]);
-        v_out[list.first[i] + k] = (float)(root * root);
-    }
+    const long n = list.n[i], k0 = (long)(blockIdx.x - list.chunk0[i]) * STEP_CHUNK + threadIdx.x * 4;
+    const long at0 = (long)list.block[i] * BLOCK + k0;
+    unsigned mc[U], vc[U];
+    float ms[U], vs[U];
+#pragma unroll
+    for (int u = 0; u < U; u++)
+        if (k0 + u * 1024 < n) {
+            const long at = at0 + u * 1024;
+            mc[u] = m[at / 4], vc[u] = v[at / 4];
+            ms[u] = m_scale[at / BLOCK], vs[u] = v_scale[at / BLOCK];
+        }
+#pragma unroll
+    for (int u = 0; u < U; u++)
+        if (k0 + u * 1024 < n) {
+            Pack<float, 4> mo, vo;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const double root = (double)decode8((vc[u] >> (8 * e)) & 255) * vs[u];
+                mo.v[e] = (float)((double)decode8((mc[u] >> (8 * e)) & 255) * ms[u]);
+                vo.v[e] = (float)(root * root);
+            }
+            store_some<4>(m_out + list.first[i], k0 + u * 1024, n, mo);
+            store_some<4>(v_out + list.first[i], k0 + u * 1024, n, vo);
+        }
 }
 
 // ---------------------------------------------------------------------------- host
@@ -311,37 +440,41 @@ using namespace ccnn;
 
 extern "C" {
 
-size_t ccnn_grad_norm_workspace_bytes(const ccnn_tensor_t *tensors, int count)
+size_t ccnn_grad_norm_workspace_bytes(const long *n, int count)
 {
-    if (!tensors || count < 0) return 0;
+    if (!n || count < 0) return 0;
     size_t chunks = 1;
     for (int i = 0; i < count; i++)
-        if (tensors[i].n > 0) chunks += (size_t)((tensors[i].n + NORM_CHUNK - 1) / NORM_CHUNK);
+        if (n[i] > 0) chunks += (size_t)((n[i] + NORM_CHUNK - 1) / NORM_CHUNK);
     return chunks * sizeof(double);
 }
 
-int ccnn_grad_norm(const ccnn_tensor_t *tensors, int count, double max_norm, double *out, void *workspace,
-                   size_t workspace_bytes, void *stream)
+int ccnn_grad_norm(const void *const *data, const long *n, const int *types, int count, double max_norm, double *out,
+                   void *workspace, size_t workspace_bytes, void *stream)
 {
-    if (count < 0 || (count > 0 && !tensors) || !out || !(max_norm > 0)) return CCNN_E_INVALID;
-    for (int i = 0; i < count; i++)
-        if (!type_bytes(tensors[i].type) || tensors[i].n < 0 || (tensors[i].n > 0 && !tensors[i].data)) return CCNN_E_INVALID;
-    const size_t need = ccnn_grad_norm_workspace_bytes(tensors, count);
+    if (count < 0 || (count > 0 && (!data || !n || !types)) || !out || !(max_norm > 0)) return CCNN_E_INVALID;
+    bool used[CCNN_TYPE_F16 + 1] = {};
+    for (int i = 0; i < count; i++) {
+        if (!type_bytes(types[i]) || n[i] < 0 || (n[i] > 0 && !data[i])) return CCNN_E_INVALID;
+        used[types[i]] = true;
+    }
+    const size_t need = count > 0 ? ccnn_grad_norm_workspace_bytes(n, count) : sizeof(double);
     if (need / sizeof(double) > 0x7fffffffu) return CCNN_E_RANGE;
     if (!workspace || workspace_bytes < need) return CCNN_E_WORKSPACE;
     hipStream_t st = (hipStream_t)stream;
     double *partial = (double *)workspace;
     int done = 0;
     for (int type = CCNN_TYPE_F32; type <= CCNN_TYPE_F16; type++) {
+        if (!used[type]) continue;
         const int e = in_lists<NormList>(
             count, NORM_CHUNK,
             [&](NormList &list, int i) -> long {
-                if (tensors[i].type != type) return 0;
+                if (types[i] != type) return 0;
                 if (list.count < LIST) {
-                    list.data[list.count] = tensors[i].data;
-                    list.n[list.count] = tensors[i].n;
+                    list.data[list.count] = data[i];
+                    list.n[list.count] = n[i];
                 }
-                return tensors[i].n;
+                return n[i];
             },
             [&](const NormList &list) -> int {
                 const int chunks = list.chunk0[list.count];
@@ -356,24 +489,24 @@ int ccnn_grad_norm(const ccnn_tensor_t *tensors, int count, double max_norm, dou
             });
         if (e) return e;
     }
-    launch("norm_total", norm_total, dim3(1), dim3(256), 0, st, partial, done, max_norm, out);
+    launch("norm_total", norm_total, dim3(1), dim3(TOTAL_THREADS), 0, st, partial, done, max_norm, out);
     CCNN_LAUNCH_CHECK();
     return 0;
 }
 
-int ccnn_adamw_step(const ccnn_adamw_tensor_t *tensors, int count, int moment_bits, void *m, void *v, float *m_scale,
-                    float *v_scale, float *master, double *clock, double lr, const double *lr_device, double beta1,
-                    double beta2, double eps, const double *clip, void *stream)
+int ccnn_adamw_step(const ccnn_adamw_tensor_t *tensors, const void *const *grads, const int *grad_types, int count,
+                    int moment_bits, void *m, void *v, float *m_scale, float *v_scale, float *master, double *clock, double lr,
+                    const double *lr_device, double beta1, double beta2, double eps, const double *clip, void *stream)
 {
-    if (count < 0 || (count > 0 && !tensors) || !clock) return CCNN_E_INVALID;
+    if (count < 0 || (count > 0 && (!tensors || !grads || !grad_types)) || !clock) return CCNN_E_INVALID;
     if (moment_bits != 32 && moment_bits != 8) return CCNN_E_INVALID;
     if (!(beta1 >= 0 && beta1 < 1) || !(beta2 >= 0 && beta2 < 1) || !(eps >= 0)) return CCNN_E_INVALID;
     bool wide = false, other = false, any = false;
     for (int i = 0; i < count; i++) {
         const ccnn_adamw_tensor_t &t = tensors[i];
         const bool half = t.type == CCNN_TYPE_BF16 || t.type == CCNN_TYPE_F16;
-        if (!type_bytes(t.type) || (t.grad_type != t.type && !(half && t.grad_type == CCNN_TYPE_F32))) return CCNN_E_INVALID;
-        if (t.n < 0 || (t.n > 0 && (!t.param || !t.grad || t.first < 0 || t.block < 0))) return CCNN_E_INVALID;
+        if (!type_bytes(t.type) || (grad_types[i] != t.type && !(half && grad_types[i] == CCNN_TYPE_F32))) return CCNN_E_INVALID;
+        if (t.n < 0 || (t.n > 0 && (!t.param || !grads[i] || t.first < 0 || t.block < 0))) return CCNN_E_INVALID;
         if (moment_bits == 8 && t.block > 0x7fffffffL) return CCNN_E_RANGE;
         if (half && t.n > 0 && !master) return CCNN_E_INVALID;
         (t.type == CCNN_TYPE_F64 ? wide : other) = true;
@@ -402,10 +535,10 @@ int ccnn_adamw_step(const ccnn_adamw_tensor_t *tensors, int count, int moment_bi
             count, STEP_CHUNK,
             [&](StepList &list, int i) -> long {
                 const ccnn_adamw_tensor_t &t = tensors[i];
-                if (t.type != kind.type || t.grad_type != kind.grad_type) return 0;
+                if (t.type != kind.type || grad_types[i] != kind.grad_type) return 0;
                 if (const int c = list.count; c < LIST) {
                     list.param[c] = t.param;
-                    list.grad[c] = t.grad;
+                    list.grad[c] = grads[i];
                     list.n[c] = t.n;
                     list.first[c] = t.first;
                     list.block[c] = (int)t.block;
@@ -445,7 +578,7 @@ int ccnn_adamw_moments(const ccnn_adamw_tensor_t *tensors, int count, const void
         },
         [&](const StepList &list) -> int {
             launch("adamw_decode", adamw_decode, dim3((unsigned)list.chunk0[list.count]), dim3(256), 0, (hipStream_t)stream,
-                   list, (const unsigned char *)m, (const unsigned char *)v, m_scale, v_scale, m_out, v_out);
+                   list, (const unsigned *)m, (const unsigned *)v, m_scale, v_scale, m_out, v_out);
             CCNN_LAUNCH_CHECK();
             return 0;
         });

@@ -27,16 +27,65 @@ __device__ __forceinline__ float widen(Bf16 v) { return __uint_as_float((unsigne
 __device__ __forceinline__ void narrow(float v, float &out) { out = v; }
 __device__ __forceinline__ void narrow(double v, double &out) { out = v; }
 __device__ __forceinline__ void narrow(float v, F16 &out) { out = (F16)v; }
-__device__ __forceinline__ void narrow(float v, Bf16 &out)
-{
-    const unsigned u = __float_as_uint(v);
-    out.bits = v != v ? 0x7fc0 : (unsigned short)((u + 0x7fff + ((u >> 16) & 1)) >> 16);
-}
+__device__ __forceinline__ void narrow(float v, Bf16 &out) { out.bits = __builtin_bit_cast(unsigned short, (__bf16)v); }
 
 __device__ __forceinline__ float ninf(float) { return -__builtin_huge_valf(); }
 __device__ __forceinline__ double ninf(double) { return -__builtin_huge_val(); }
 __device__ __forceinline__ float nan_of(float) { return __builtin_nanf(""); }
 __device__ __forceinline__ double nan_of(double) { return __builtin_nan(""); }
+
+// op over all of a group of G lanes (a power of two, aligned), the same result in each.  Lanes meet their
+// neighbours, quads, halves of a row of 16 and rows through the cross-lane paths of the vector unit; no LDS.
+template <int CTRL>
+__device__ __forceinline__ unsigned lane_move(unsigned v)
+{
+    return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+template <int STEP, typename V>
+__device__ __forceinline__ void lane_pair(V v, V &a, V &b)
+{
+    constexpr int N = sizeof(V) / 4;
+    struct Words { unsigned w[N]; };
+    const Words x = __builtin_bit_cast(Words, v);
+    Words p, q;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        if constexpr (STEP == 32) {
+            const auto r = __builtin_amdgcn_permlane32_swap(x.w[i], x.w[i], false, false);
+            p.w[i] = r[0], q.w[i] = r[1];
+        } else if constexpr (STEP == 16) {
+            const auto r = __builtin_amdgcn_permlane16_swap(x.w[i], x.w[i], false, false);
+            p.w[i] = r[0], q.w[i] = r[1];
+        } else {
+            p.w[i] = x.w[i];
+            q.w[i] = lane_move<STEP == 1 ? 0xb1 : STEP == 2 ? 0x4e : STEP == 4 ? 0x141 : 0x140>(x.w[i]);
+        }
+    }
+    a = __builtin_bit_cast(V, p);
+    b = __builtin_bit_cast(V, q);
+}
+template <int G, typename V, typename Op>
+__device__ __forceinline__ V over_lanes(V v, Op op)
+{
+    V a, b;
+    if constexpr (G > 1) lane_pair<1>(v, a, b), v = op(a, b);
+    if constexpr (G > 2) lane_pair<2>(v, a, b), v = op(a, b);
+    if constexpr (G > 4) lane_pair<4>(v, a, b), v = op(a, b);
+    if constexpr (G > 8) lane_pair<8>(v, a, b), v = op(a, b);
+    if constexpr (G > 16) lane_pair<16>(v, a, b), v = op(a, b);
+    if constexpr (G > 32) lane_pair<32>(v, a, b), v = op(a, b);
+    return v;
+}
+template <int G, typename V>
+__device__ __forceinline__ V lanes_max(V v)
+{
+    return over_lanes<G>(v, [](V a, V b) { return a > b ? a : b; });
+}
+template <int G, typename V>
+__device__ __forceinline__ V lanes_sum(V v)
+{
+    return over_lanes<G>(v, [](V a, V b) { return a + b; });
+}
 
 // N consecutive elements in one access.  The type says only what a tensor guarantees (its element's
 // alignment): a view into a flat buffer may start anywhere, and the hardware takes such addresses.

@@ -61,6 +61,14 @@ __device__ __forceinline__ Sums<A> join(Sums<A> a, Sums<A> b)
     return {m, a.s + b.s, a.t + b.t};
 }
 
+// Joined over the wave's lanes, the same in all of them.
+template <typename A>
+__device__ __forceinline__ Sums<A> over_wave(Sums<A> a)
+{
+    shift(a, lanes_max<64>(a.m));
+    return {a.m, lanes_sum<64>(a.s), lanes_sum<64>(a.t)};
+}
+
 template <typename A>
 __device__ __forceinline__ void finish_row(const Sums<A> &a, long r, A given, long y, int classes, const ScoreOut<A> &o)
 {
@@ -102,12 +110,6 @@ __device__ __forceinline__ double key_value(unsigned __int128 k)
     const long long u = (long long)(k >> 32);
     return __longlong_as_double(u ^ (~(u >> 63) | (long long)0x8000000000000000ull));
 }
-__device__ __forceinline__ unsigned long long xor_lane(unsigned long long k, int off) { return __shfl_xor(k, off); }
-__device__ __forceinline__ unsigned __int128 xor_lane(unsigned __int128 k, int off)
-{
-    return (unsigned __int128)__shfl_xor((unsigned long long)(k >> 64), off) << 64 | __shfl_xor((unsigned long long)k, off);
-}
-
 template <typename A>
 __device__ __forceinline__ void put_top(const ScoreOut<A> &o, long r, int place, Key<A> k, A m, A l)
 {
@@ -140,11 +142,7 @@ __global__ __launch_bounds__(256) void log_probs_small(const T *__restrict__ log
     A m = x[0];
 #pragma unroll
     for (int e = 1; e < E; e++) m = x[e] > m ? x[e] : m;
-#pragma unroll
-    for (int off = G / 2; off > 0; off >>= 1) {
-        const A w = __shfl_xor(m, off);
-        m = w > m ? w : m;
-    }
+    m = lanes_max<G>(m);
     const A from = m == ninf(A()) ? A(0) : m;
     A s = 0, t = 0;
 #pragma unroll
@@ -153,33 +151,27 @@ __global__ __launch_bounds__(256) void log_probs_small(const T *__restrict__ log
         s += w;
         t += w * (d < A(-1e4) ? A(-1e4) : d);       // 0 * inf is not wanted
     }
-#pragma unroll
-    for (int off = G / 2; off > 0; off >>= 1) {
-        s += __shfl_xor(s, off);
-        t += __shfl_xor(t, off);
-    }
-    const Sums<A> sums = {m, s, t};
+    const Sums<A> sums = {m, s = lanes_sum<G>(s), t = lanes_sum<G>(t)};
     if (lane == 0) finish_row(sums, r, given, y, classes, o);
     if (o.top == 0) return;
     const A l = m == ninf(A()) && s == A(0) ? ninf(A()) : logw(s);
-    Key<A> key[E];
+    // a lane's next alternative: the first of its largest elements not taken yet
+    unsigned taken = 0;
+    auto next = [&]() {
+        A v = ninf(A());
+        int at = -1;
 #pragma unroll
-    for (int e = 0; e < E; e++) key[e] = e * G + lane < classes ? key_of(x[e], e * G + lane) : Key<A>(0);
-    Key<A> best = 0;
-#pragma unroll
-    for (int e = 0; e < E; e++) best = key[e] > best ? key[e] : best;
+        for (int e = 0; e < E; e++)
+            if (!(taken >> e & 1) && e * G + lane < classes && (at < 0 || x[e] > v)) v = x[e], at = e;
+        return at < 0 ? Key<A>(0) : key_of(v, at * G + lane);
+    };
+    Key<A> best = next();
     for (int k = 0; k < o.top; k++) {
-        Key<A> high = best;
-#pragma unroll
-        for (int off = G / 2; off > 0; off >>= 1) {
-            const Key<A> w = xor_lane(high, off);
-            high = w > high ? w : high;
-        }
+        const Key<A> high = lanes_max<G>(best);
         if (lane == 0) put_top(o, r, k, high, m, l);
-        if (best == high) {
-            best = 0;
-#pragma unroll
-            for (int e = 0; e < E; e++) best = key[e] < high && key[e] > best ? key[e] : best;
+        if (best == high && k + 1 < o.top) {
+            taken |= 1u << (key_index(high) / G);
+            best = next();
         }
     }
 }
@@ -209,17 +201,6 @@ struct SliceLds {
     int owners[SLICE_THREADS];
     int n_owners, n_found;
 };
-
-template <typename K>
-__device__ __forceinline__ K wave_max(K k)
-{
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-        const K w = xor_lane(k, off);
-        k = w > k ? w : k;
-    }
-    return k;
-}
 
 // k-th largest (k >= 1) of the wave's 64 keys; equal keys count one by one.
 template <typename K>
@@ -261,7 +242,7 @@ __device__ __forceinline__ void in_rounds(Get get, int n, int top, K *lds, Put p
             const K w = get(j);
             high = w < last && w > high ? w : high;
         }
-        high = wave_max(high);
+        high = lanes_max<64>(high);
         __syncthreads();
         if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = high;
         __syncthreads();
@@ -284,7 +265,13 @@ __global__ __launch_bounds__(SLICE_THREADS) void log_probs_slice(const T *__rest
     const long begin = slice * part.length;
     const int n = (int)min((long)classes - begin, part.length);
     const T *row = logits + r * stride + begin;
-    const int loads = n / W;                    // whole loads; the rest of the row is one element a thread
+    const int loads = n / W;                    // whole loads; what is left of the row is one more, partial one
+    long y = -1;
+    A given = A(0);
+    if (tid == 0 && !part.sums) {               // under way while the row streams
+        y = targets.at(r);
+        if (y >= 0 && y < classes) given = widen(logits[r * stride + y]);
+    }
     A m = ninf(A()), s = 0, t = 0, best = ninf(A());
     int best_at = -1;
     auto take = [&](const A *x, int count, int at) {
@@ -332,22 +319,25 @@ __global__ __launch_bounds__(SLICE_THREADS) void log_probs_slice(const T *__rest
         take(x, W, loads);
     }
 
-    Sums<A> sums = {m, s, t};
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1)
-        sums = join(sums, {__shfl_xor(sums.m, off), __shfl_xor(sums.s, off), __shfl_xor(sums.t, off)});
+    Sums<A> sums = over_wave(Sums<A>{m, s, t});
     if (lane == 0) lds.m[wave] = sums.m, lds.s[wave] = sums.s, lds.t[wave] = sums.t;
     if (o.top) lds.key[tid] = best_at < 0 ? Key<A>(0) : key_of(best, best_at);
     if (tid == 0) lds.n_owners = lds.n_found = 0;
     __syncthreads();
-    sums = {lds.m[0], lds.s[0], lds.t[0]};
-    for (int w = 1; w < NT / 64; w++) sums = join(sums, {lds.m[w], lds.s[w], lds.t[w]});
+    A all = lds.m[0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; w++) all = lds.m[w] > all ? lds.m[w] : all;
+    sums = {all, A(0), A(0)};
+#pragma unroll
+    for (int w = 0; w < NT / 64; w++) {
+        Sums<A> one = {lds.m[w], lds.s[w], lds.t[w]};
+        shift(one, all);
+        sums.s += one.s;
+        sums.t += one.t;
+    }
     if (tid == 0) {
         if (part.sums) part.sums[r * part.slices + slice] = sums;
-        else {
-            const long y = targets.at(r);
-            finish_row(sums, r, y >= 0 && y < classes ? (A)widen(logits[r * stride + y]) : A(0), y, classes, o);
-        }
+        else finish_row(sums, r, given, y, classes, o);
     }
     if (!o.top) return;
     const A l = sums.m == ninf(A()) && sums.s == A(0) ? ninf(A()) : logw(sums.s);
@@ -369,9 +359,17 @@ __global__ __launch_bounds__(SLICE_THREADS) void log_probs_slice(const T *__rest
     for (int task = tid; task < lds.n_owners * turns; task += NT) {
         const int at = lds.owners[task / turns] + (task % turns) * NT;
         const int count = at < loads ? W : at == loads ? rest : 0;
-        for (int e = 0; e < count; e++) {
-            const A x = widen(row[(long)at * W + e]);
-            if (key_of(x, at) >= bar) {
+        Pack<T, W> p;
+        if (count == W) p = load_pack<T, W>(row + (long)at * W);
+        else {
+#pragma unroll
+            for (int e = 0; e < W; e++)
+                if (e < count) p.v[e] = row[(long)at * W + e];
+        }
+#pragma unroll
+        for (int e = 0; e < W; e++) {
+            const A x = widen(p.v[e]);
+            if (e < count && key_of(x, at) >= bar) {
                 const int place = atomicAdd(&lds.n_found, 1);
                 if (place < CANDIDATES) lds.found[place] = key_of(x, (unsigned)(begin + (long)at * W + e));
             }
@@ -387,42 +385,42 @@ __global__ __launch_bounds__(SLICE_THREADS) void log_probs_slice(const T *__rest
 }
 
 // Joins a row's slices: their sums, and their lists of alternatives through the same bar.
+constexpr int JOIN_KEYS = 2048;   // slices x top, see slices_of
+
 template <typename T>
 __global__ __launch_bounds__(256) void log_probs_join(const T *__restrict__ logits, int classes, long stride, Targets targets,
                                                       ScoreOut<Wide<T>> o, SliceOut<Wide<T>> part)
 {
     typedef Wide<T> A;
-    __shared__ Key<A> found[CANDIDATES], high_of[64];
+    __shared__ Key<A> keys[JOIN_KEYS], found[CANDIDATES], high_of[64];
     __shared__ Key<A> bar;
     __shared__ int n_found;
     const long r = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63;
+    const int n = part.slices * o.top;
+    long y = -1;
+    A given = A(0);
+    if (tid == 0) {
+        y = targets.at(r);
+        if (y >= 0 && y < classes) given = widen(logits[r * stride + y]);
+        n_found = 0;
+    }
+    for (int k = tid; k < n; k += 256) {
+        // place by place of all slices, so that groups of every 64th key share a row's first alternatives
+        // unevenly only if few slices hold them all
+        keys[k % o.top * part.slices + k / o.top] = part.keys[r * n + k];
+    }
     const Sums<A> *in = part.sums + r * part.slices;
     Sums<A> sums = {ninf(A()), A(0), A(0)};
     for (int k = lane; k < part.slices; k += 64) sums = join(sums, in[k]);
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1)
-        sums = join(sums, {__shfl_xor(sums.m, off), __shfl_xor(sums.s, off), __shfl_xor(sums.t, off)});
-    // lane 0's: a contracted sum differs in its last bit between the two sides of an exchange
-    sums = {__shfl(sums.m, 0), __shfl(sums.s, 0), __shfl(sums.t, 0)};
-    if (tid == 0) {
-        const long y = targets.at(r);
-        finish_row(sums, r, y >= 0 && y < classes ? (A)widen(logits[r * stride + y]) : A(0), y, classes, o);
-        n_found = 0;
-    }
+    sums = over_wave(sums);
+    if (tid == 0) finish_row(sums, r, given, y, classes, o);
     if (!o.top) return;
     const A l = sums.m == ninf(A()) && sums.s == A(0) ? ninf(A()) : logw(sums.s);
-    const int n = part.slices * o.top;
-    const Key<A> *keys = part.keys + r * n;
-    // groups take the slices' lists place by place, so that a row's first alternatives meet in few of them
-    // only if few slices hold them all
-    auto transposed = [&](int k) { return keys[(k % part.slices) * o.top + k / part.slices]; };
+    __syncthreads();
     if (tid < 64) {
         Key<A> high = 0;
-        for (int k = lane; k < n; k += 64) {
-            const Key<A> w = transposed(k);
-            high = w > high ? w : high;
-        }
+        for (int k = lane; k < n; k += 64) high = keys[k] > high ? keys[k] : high;
         const Key<A> b = n < 64 ? Key<A>(0) : wave_kth(high, o.top, high_of);
         if (lane == 0) bar = b;
     }
@@ -518,12 +516,15 @@ __global__ __launch_bounds__(256) void log_probs_grad_wide(const T *logits, int 
 // ---------------------------------------------------------------------------- host
 constexpr int SMALL_CLASSES = 1024;
 
-// Slices of a row: enough of them to give every CU two workgroups, none shorter than a load per thread.
-inline int slices_of(long rows, int classes, int size, long *length)
+// Slices of a row: enough of them to give every CU two workgroups, none shorter than a load per thread, and
+// their lists short enough for the LDS of the workgroup that joins them.
+inline int slices_of(long rows, int classes, int top, int size, long *length)
 {
     const long width = 16 / size, turn = width * SLICE_THREADS;
-    long want = (512 + rows - 1) / rows, most = (classes + turn - 1) / turn;
+    long want = (512 + rows - 1) / rows;
+    const long most = (classes + turn - 1) / turn;
     if (want > most) want = most;
+    if (top > 0 && want > JOIN_KEYS / top) want = JOIN_KEYS / top;
     if (want < 1) want = 1;
     *length = ((classes + want - 1) / want + width - 1) / width * width;
     return (int)((classes + *length - 1) / *length);
@@ -534,7 +535,7 @@ size_t slice_bytes(long rows, int classes, int top, int size)
 {
     long length;
     if (classes <= SMALL_CLASSES) return 0;
-    const int slices = slices_of(rows, classes, size, &length);
+    const int slices = slices_of(rows, classes, top, size, &length);
     if (slices == 1) return 0;
     return align_up(rows * slices * sizeof(Sums<A>)) + align_up(rows * slices * (size_t)top * sizeof(Key<A>));
 }
@@ -560,7 +561,7 @@ int score_impl(const void *logits, long rows, int classes, long stride, Targets 
         return 0;
     }
     SliceOut<A> part = {};
-    part.slices = slices_of(rows, classes, sizeof(T), &part.length);
+    part.slices = slices_of(rows, classes, top, sizeof(T), &part.length);
     if (part.slices > 1) {
         Carver c(workspace);
         part.sums = c.take<Sums<A>>(rows * part.slices);

@@ -30,13 +30,9 @@ class LrSched(C.Structure):
     _fields_ = [("fifo", C.c_double * 5), ("cur_min", C.c_double), ("count", C.c_int), ("use_float", C.c_int)]
 
 
-class Tensor(C.Structure):
-    _fields_ = [("data", C.c_void_p), ("n", C.c_long), ("type", C.c_int)]
-
-
 class AdamwTensor(C.Structure):
-    _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("n", C.c_long), ("first", C.c_long), ("block", C.c_long),
-                ("decay", C.c_double), ("type", C.c_int), ("grad_type", C.c_int)]
+    _fields_ = [("param", C.c_void_p), ("n", C.c_long), ("first", C.c_long), ("block", C.c_long), ("decay", C.c_double),
+                ("type", C.c_int)]
 
 
 TYPE_F32, TYPE_F64, TYPE_BF16, TYPE_F16 = 1, 2, 3, 4     # CCNN_TYPE_*
@@ -78,8 +74,8 @@ _SIG = {
     "ccnn_log_probs_grad": (C.c_int, [_P, C.c_int, C.c_long, C.c_int, C.c_long, _P, C.c_int, _P, _P, _P, _P, _P, C.c_long,
                                       _P]),
     "ccnn_grad_norm_workspace_bytes": (C.c_size_t, [_P, C.c_int]),
-    "ccnn_grad_norm": (C.c_int, [_P, C.c_int, C.c_double, _P, _P, C.c_size_t, _P]),
-    "ccnn_adamw_step": (C.c_int, [_P, C.c_int, C.c_int, _P, _P, _P, _P, _P, _P, C.c_double, _P, C.c_double, C.c_double,
+    "ccnn_grad_norm": (C.c_int, [_P, _P, _P, C.c_int, C.c_double, _P, _P, C.c_size_t, _P]),
+    "ccnn_adamw_step": (C.c_int, [_P, _P, _P, C.c_int, C.c_int, _P, _P, _P, _P, _P, _P, C.c_double, _P, C.c_double, C.c_double,
                                   C.c_double, _P, _P]),
     "ccnn_adamw_moments": (C.c_int, [_P, C.c_int, _P, _P, _P, _P, _P, _P, _P]),
     "ccnn_host_scan_labels": (C.c_int, [_P, C.c_int, C.c_int, _P, C.POINTER(C.c_int)]),

@@ -350,7 +350,7 @@ _TYPES = {_F32: _l.TYPE_F32, _F64: _l.TYPE_F64, torch.bfloat16: _l.TYPE_BF16, to
 
 
 def _on_device(t, name, dtypes):
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
         raise TypeError(f"{name} must be a CUDA tensor")
     if t.dtype not in dtypes:
         raise TypeError(f"{name} has dtype {t.dtype}, expected one of {', '.join(str(d) for d in dtypes)}")
@@ -362,14 +362,22 @@ def _same_device(t, name, device):
         raise ValueError(f"{name} is on {t.device}, expected {device}")
 
 
-def _enqueue(device, name, *args):
-    """Calls a library function with `device` current and that device's current stream as its last argument."""
+def _at(t):
+    return t.data_ptr() if t is not None else None
+
+
+_raw_stream, _current = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+
+
+def _enqueue(index, name, *args):
+    """Calls a library function with device `index` current and that device's current stream as its last
+    argument.  Addresses go as plain numbers: the host side of a small call is most of it."""
     fn = getattr(_l.load(), name)
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, C.c_void_p(torch.cuda.current_stream(device).cuda_stream))
+    if index == _current():
+        rc = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, C.c_void_p(torch.cuda.current_stream(device).cuda_stream))
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
     if rc:
         _l.check(rc, name)
 
@@ -385,23 +393,24 @@ class LogProbs(NamedTuple):
 
 def _rows(t, name):
     """(rows, columns, elements from row to row) of a matrix whose rows are contiguous and do not overlap."""
-    if t.dim() != 2 or t.shape[1] < 1:
-        raise ValueError(f"{name} must be [rows, classes] with at least one class, got {list(t.shape)}")
-    rows, classes = t.shape
-    if classes > 1 and t.stride(1) != 1:
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or shape[1] < 1:
+        raise ValueError(f"{name} must be [rows, classes] with at least one class, got {list(shape)}")
+    rows, classes = shape
+    if classes > 1 and stride[1] != 1:
         raise ValueError(f"{name} must be contiguous along its classes")
-    stride = t.stride(0) if rows > 1 else classes
-    if stride < classes:
+    step = stride[0] if rows > 1 else classes
+    if step < classes:
         raise ValueError(f"rows of {name} overlap")
-    return rows, classes, stride
+    return rows, classes, step
 
 
-def _targets(targets, rows, device):
+def _target_bytes(targets, rows, device):
     _on_device(targets, "targets", (torch.int32, torch.int64))
     _same_device(targets, "targets", device)
     if targets.dim() != 1 or targets.shape[0] != rows or (rows > 1 and targets.stride(0) != 1):
         raise ValueError(f"targets must be contiguous [{rows}], got {list(targets.shape)}")
-    return targets
+    return 4 if targets.dtype == torch.int32 else 8
 
 
 def log_probs(logits, targets, top=0, want_entropy=True):
@@ -413,11 +422,12 @@ def log_probs(logits, targets, top=0, want_entropy=True):
     entropy 0, a row with a NaN or +inf has NaN everywhere and top_index -1."""
     _on_device(logits, "logits", tuple(_TYPES))
     rows, classes, stride = _rows(logits, "logits")
-    _targets(targets, rows, logits.device)
+    dev = logits.device
+    target_bytes = _target_bytes(targets, rows, dev)
     top = int(top)
     if top < 0 or top > min(_l.MAX_TOP, classes):
         raise ValueError(f"top must be between 0 and {min(_l.MAX_TOP, classes)}, got {top}")
-    dev, wide, kind = logits.device, _F64 if logits.dtype == _F64 else _F32, _TYPES[logits.dtype]
+    wide, kind = _F64 if logits.dtype == _F64 else _F32, _TYPES[logits.dtype]
     stats = torch.empty((rows, 2), dtype=wide, device=dev)
     logp = torch.empty(rows, dtype=wide, device=dev)
     entropy = torch.empty(rows, dtype=wide, device=dev) if want_entropy else None
@@ -426,8 +436,8 @@ def log_probs(logits, targets, top=0, want_entropy=True):
     if rows:
         nbytes = _l.load().ccnn_log_probs_workspace_bytes(rows, classes, top, kind)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        _enqueue(dev, "ccnn_log_probs", _ptr(logits), kind, rows, classes, stride, _ptr(targets), targets.element_size(), top,
-                 _ptr(logp), _ptr(entropy), _ptr(top_logp), _ptr(top_index), _ptr(stats), _ptr(ws), nbytes)
+        _enqueue(dev.index, "ccnn_log_probs", logits.data_ptr(), kind, rows, classes, stride, targets.data_ptr(), target_bytes,
+                 top, logp.data_ptr(), _at(entropy), _at(top_logp), _at(top_index), stats.data_ptr(), _at(ws), nbytes)
     return LogProbs(logp, entropy, top_logp, top_index, stats)
 
 
@@ -438,7 +448,7 @@ def log_probs_grad(logits, targets, scored, d_logp=None, d_entropy=None, out=Non
     _on_device(logits, "logits", tuple(_TYPES))
     rows, classes, stride = _rows(logits, "logits")
     dev, wide = logits.device, _F64 if logits.dtype == _F64 else _F32
-    _targets(targets, rows, dev)
+    target_bytes = _target_bytes(targets, rows, dev)
     if d_logp is None and d_entropy is None:
         raise ValueError("neither d_logp nor d_entropy given")
     if d_entropy is not None and scored.entropy is None:
@@ -448,22 +458,23 @@ def log_probs_grad(logits, targets, scored, d_logp=None, d_entropy=None, out=Non
         if t is not None:
             _req(t, wide, name, n)
             _same_device(t, name, dev)
-    if out is None:
+    given, out_stride = out is not None, classes
+    if given:
+        _on_device(out, "out", (logits.dtype,))
+        _same_device(out, "out", dev)
+        if out.shape != logits.shape:
+            raise ValueError(f"out is {list(out.shape)}, the logits are {list(logits.shape)}")
+        _, _, out_stride = _rows(out, "out")
+    else:
         out = torch.empty((rows, classes), dtype=logits.dtype, device=dev)
-    _on_device(out, "out", (logits.dtype,))
-    _same_device(out, "out", dev)
-    if out.shape != logits.shape:
-        raise ValueError(f"out is {list(out.shape)}, the logits are {list(logits.shape)}")
-    _, _, out_stride = _rows(out, "out")
     if rows:
         size = logits.element_size()
         a, b = logits.data_ptr(), out.data_ptr()
-        if (a, stride) != (b, out_stride) and a < b + ((rows - 1) * out_stride + classes) * size \
+        if given and (a, stride) != (b, out_stride) and a < b + ((rows - 1) * out_stride + classes) * size \
                 and b < a + ((rows - 1) * stride + classes) * size:
             raise ValueError("out overlaps the logits without being them")
-        _enqueue(dev, "ccnn_log_probs_grad", _ptr(logits), _TYPES[logits.dtype], rows, classes, stride, _ptr(targets),
-                 targets.element_size(), _ptr(scored.stats), _ptr(scored.entropy), _ptr(d_logp), _ptr(d_entropy), _ptr(out),
-                 out_stride)
+        _enqueue(dev.index, "ccnn_log_probs_grad", a, _TYPES[logits.dtype], rows, classes, stride, targets.data_ptr(),
+                 target_bytes, scored.stats.data_ptr(), _at(scored.entropy), _at(d_logp), _at(d_entropy), b, out_stride)
     return out
 
 
@@ -477,17 +488,19 @@ def grad_norm(grads, max_norm=float("inf")):
     if not max_norm > 0:
         raise ValueError(f"max_norm must be positive, got {max_norm}")
     dev = grads[0].device if isinstance(grads[0], torch.Tensor) else None
-    table = (_l.Tensor * len(grads))()
+    count = len(grads)
     for i, g in enumerate(grads):
-        _on_device(g, f"gradient {i}", tuple(_TYPES))
-        _same_device(g, f"gradient {i}", dev)
-        if not g.is_contiguous():
+        _on_device(g, f"gradient {i}", _TYPES)
+        if g.device != dev or not g.is_contiguous():
+            _same_device(g, f"gradient {i}", dev)
             raise ValueError(f"gradient {i} must be contiguous")
-        table[i] = (g.data_ptr(), g.numel(), _TYPES[g.dtype])
+    at = (C.c_void_p * count)(*[g.data_ptr() for g in grads])
+    n = (C.c_long * count)(*[g.numel() for g in grads])
+    kinds = (C.c_int * count)(*[_TYPES[g.dtype] for g in grads])
     out = torch.empty(2, dtype=_F64, device=dev)
-    nbytes = _l.load().ccnn_grad_norm_workspace_bytes(table, len(grads))
+    nbytes = _l.load().ccnn_grad_norm_workspace_bytes(n, count)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _enqueue(dev, "ccnn_grad_norm", table, len(grads), float(max_norm), _ptr(out), _ptr(ws), nbytes)
+    _enqueue(dev.index, "ccnn_grad_norm", at, n, kinds, count, float(max_norm), out.data_ptr(), ws.data_ptr(), nbytes)
     return out
 
 
@@ -536,7 +549,7 @@ class AdamW:
             if p.dtype == _F64 and state_bits == 8:
                 raise TypeError("moments in 8 bits are not for fp64 parameters")
             kind = _TYPES[p.dtype]
-            self._table[i] = (p.data_ptr(), 0, p.numel(), first, block, decays[i], kind, kind)
+            self._table[i] = (p.data_ptr(), p.numel(), first, block, decays[i], kind)
             if p.numel():
                 spans.append((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()))
             first += p.numel()
@@ -545,6 +558,9 @@ class AdamW:
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise ValueError("parameter tensors overlap")
         self.numel, self.blocks = first, block
+        # what each gradient is held against, and the types' table for the usual case that they are the parameters'
+        self._expected = [(p.dtype, p.numel()) for p in self.params]
+        self._kinds = (C.c_int * n)(*[t.type for t in self._table])
         wide = _F64 if self.params[0].dtype == _F64 else _F32
         if state_bits == 32:
             self.m, self.v = (torch.zeros(first, dtype=wide, device=self.device) for _ in range(2))
@@ -570,17 +586,23 @@ class AdamW:
         """One step from `grads`, one contiguous tensor per parameter with its size, of its type (or fp32
         for bf16 / fp16).  lr: instead of self.lr.  clip: grad_norm's result; its factor scales every
         gradient, and a factor that is not finite leaves everything as it is, the step count too."""
-        grads, table = list(grads), self._table
-        if len(grads) != len(self.params):
-            raise ValueError(f"{len(grads)} gradients for {len(self.params)} parameters")
-        for i, (g, p) in enumerate(zip(grads, self.params)):
-            _on_device(g, f"gradient {i}", (p.dtype, _F32) if p.element_size() == 2 else (p.dtype,))
-            _same_device(g, f"gradient {i}", self.device)
-            if not g.is_contiguous():
-                raise ValueError(f"gradient {i} must be contiguous")
-            if g.numel() != table[i].n:
-                raise ValueError(f"gradient {i} has {g.numel()} elements, its parameter {table[i].n}")
-            table[i].grad, table[i].grad_type = g.data_ptr(), _TYPES[g.dtype]
+        grads, kinds, dev = list(grads), self._kinds, self.device
+        count = len(self.params)
+        if len(grads) != count:
+            raise ValueError(f"{len(grads)} gradients for {count} parameters")
+        for i, (g, (dtype, n)) in enumerate(zip(grads, self._expected)):
+            if not (isinstance(g, torch.Tensor) and g.is_cuda and g.dtype == dtype and g.device == dev and g.is_contiguous()
+                    and g.numel() == n):
+                _on_device(g, f"gradient {i}", (dtype, _F32) if dtype.itemsize == 2 else (dtype,))
+                _same_device(g, f"gradient {i}", dev)
+                if not g.is_contiguous():
+                    raise ValueError(f"gradient {i} must be contiguous")
+                if g.numel() != n:
+                    raise ValueError(f"gradient {i} has {g.numel()} elements, its parameter {n}")
+                kinds = None
+        if kinds is None:
+            kinds = (C.c_int * count)(*[_TYPES[g.dtype] for g in grads])
+        at = (C.c_void_p * count)(*[g.data_ptr() for g in grads])
         if clip is not None:
             _req(clip, _F64, "clip", 2)
             _same_device(clip, "clip", self.device)
@@ -590,9 +612,9 @@ class AdamW:
             _req(lr, _F64, "lr", 1)
             _same_device(lr, "lr", self.device)
             lr, lr_device = 0.0, lr
-        _enqueue(self.device, "ccnn_adamw_step", table, len(grads), self.state_bits, _ptr(self.m), _ptr(self.v),
-                 _ptr(self.m_scale), _ptr(self.v_scale), _ptr(self.master), _ptr(self._clock), float(lr), _ptr(lr_device),
-                 self.betas[0], self.betas[1], self.eps, _ptr(clip))
+        _enqueue(dev.index, "ccnn_adamw_step", self._table, at, kinds, count, self.state_bits, self.m.data_ptr(),
+                 self.v.data_ptr(), _at(self.m_scale), _at(self.v_scale), _at(self.master), self._clock.data_ptr(), float(lr),
+                 _at(lr_device), self.betas[0], self.betas[1], self.eps, _at(clip))
 
     def moments(self):
         """(m, v), flat in the order of the parameters: the optimiser's own tensors with 32 bits, the values
@@ -600,8 +622,8 @@ class AdamW:
         if self.state_bits == 32:
             return self.m, self.v
         m, v = (torch.empty(self.numel, dtype=_F32, device=self.device) for _ in range(2))
-        _enqueue(self.device, "ccnn_adamw_moments", self._table, len(self.params), _ptr(self.m), _ptr(self.v),
-                 _ptr(self.m_scale), _ptr(self.v_scale), _ptr(m), _ptr(v))
+        _enqueue(self.device.index, "ccnn_adamw_moments", self._table, len(self.params), self.m.data_ptr(), self.v.data_ptr(),
+                 self.m_scale.data_ptr(), self.v_scale.data_ptr(), m.data_ptr(), v.data_ptr())
         return m, v
 
     def state_dict(self):
@@ -624,7 +646,8 @@ class AdamW:
                 getattr(self, k).copy_(state[k])
         if self.master is not None:
             for p, t in zip(self.params, self._table):
-                p.detach().view(-1).copy_(self.master[t.first:t.first + t.n])
+                if p.element_size() == 2:
+                    p.detach().view(-1).copy_(self.master[t.first:t.first + t.n])
         self._set_step(int(state["step"]))
 
 

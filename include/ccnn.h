@@ -415,25 +415,21 @@ int ccnn_log_probs_grad(const void *logits, int type, long rows, int classes, lo
                         void *d_logits, long d_stride, void *stream);
 
 /* Norm of many gradient tensors taken as one vector, and the factor that limits it.
- * tensors: HOST array of `count` descriptions (n elements of `type` at `data`, n may be 0).
+ * data, n, types: HOST arrays of `count` pointers, element counts (0 allowed) and CCNN_TYPE_*.
  * out [2] device doubles: sqrt(sum g^2), summed in fp64 in a fixed order; and min(1, max_norm / norm),
  * NaN when the norm is not finite.  workspace: ccnn_grad_norm_workspace_bytes() bytes, not
  * initialised; calls that share one must be ordered by one stream. */
-typedef struct ccnn_tensor {
-    const void *data;
-    long n;
-    int type;
-} ccnn_tensor_t;
-size_t ccnn_grad_norm_workspace_bytes(const ccnn_tensor_t *tensors, int count);
-int ccnn_grad_norm(const ccnn_tensor_t *tensors, int count, double max_norm, double *out,
-                   void *workspace, size_t workspace_bytes, void *stream);
+size_t ccnn_grad_norm_workspace_bytes(const long *n, int count);
+int ccnn_grad_norm(const void *const *data, const long *n, const int *types, int count,
+                   double max_norm, double *out, void *workspace, size_t workspace_bytes,
+                   void *stream);
 
 /* One AdamW step (decoupled weight decay) over `count` parameter tensors:
  *   g *= clip[1];  m += (1 - beta1)(g - m);  v += (1 - beta2)(g^2 - v)
  *   p -= lr (decay p + m / (1 - beta1^t) / (sqrt(v / (1 - beta2^t)) + eps))
- * tensors: HOST array.  `type` of a parameter is F32, F64, BF16 or F16; grad_type the same, or F32 for
- * BF16 and F16.  F64 does not mix with the others in one call.  `first` is the tensor's place (in
- * elements) in the flat arrays `master` (fp32, needed for BF16 and F16 parameters: the step is taken
+ * tensors, grads, grad_types: HOST arrays of `count` entries.  `type` of a parameter is F32, F64, BF16 or
+ * F16; its gradient's the same, or F32 for BF16 and F16.  F64 does not mix with the others in one call.
+ * `first` is the tensor's place (in elements) in the flat arrays `master` (fp32, needed for BF16 and F16 parameters: the step is taken
  * there and p is its rounding) and, with 32-bit moments, m and v (fp32; fp64 for F64 parameters).
  * moment_bits 8 (not for F64): m and v hold sqrt(v) as one byte per element, in blocks of
  * CCNN_MOMENT_BLOCK elements of one tensor, `block` being the tensor's first block; a block's
@@ -451,18 +447,18 @@ int ccnn_grad_norm(const ccnn_tensor_t *tensors, int count, double max_norm, dou
 #define CCNN_ADAMW_CLOCK 8
 typedef struct ccnn_adamw_tensor {
     void *param;
-    const void *grad;
     long n;
     long first, block;
     double decay;
-    int type, grad_type;
+    int type;
 } ccnn_adamw_tensor_t;
-int ccnn_adamw_step(const ccnn_adamw_tensor_t *tensors, int count, int moment_bits, void *m, void *v,
+int ccnn_adamw_step(const ccnn_adamw_tensor_t *tensors, const void *const *grads,
+                    const int *grad_types, int count, int moment_bits, void *m, void *v,
                     float *m_scale, float *v_scale, float *master, double *clock, double lr,
                     const double *lr_device, double beta1, double beta2, double eps,
                     const double *clip, void *stream);
 /* 8-bit moments as the values they stand for: m_out, v_out flat fp32 (v, not its root), tensor i at
- * tensors[i].first (param and grad are not looked at). */
+ * tensors[i].first (param and type are not looked at). */
 int ccnn_adamw_moments(const ccnn_adamw_tensor_t *tensors, int count, const void *m, const void *v,
                        const float *m_scale, const float *v_scale, float *m_out, float *v_out,
                        void *stream);

@@ -131,32 +131,36 @@ def test_scoring_and_optimiser_calls_refuse_bad_arguments():
                 dict(out=ok, ostride=6)):
         assert grad(**bad) == -1, bad
 
-    t = (L.Tensor * 2)((64, 10, 1), (64, 40000, 3))
-    need = lib.ccnn_grad_norm_workspace_bytes(t, 2)
-    assert need >= 16
-    assert lib.ccnn_grad_norm(t, 2, 1.0, ok, ok, need - 1, nul) == -2
-    assert lib.ccnn_grad_norm(t, 2, 0.0, ok, ok, need, nul) == -1
-    assert lib.ccnn_grad_norm(t, 2, float("nan"), ok, ok, need, nul) == -1
-    assert lib.ccnn_grad_norm(t, 2, 1.0, nul, ok, need, nul) == -1
-    assert lib.ccnn_grad_norm(t, -1, 1.0, ok, ok, need, nul) == -1
-    for bad in ((0, 10, 1), (64, -1, 1), (64, 10, 7)):
-        assert lib.ccnn_grad_norm((L.Tensor * 1)(bad), 1, 1.0, ok, ok, 64, nul) == -1
+    def norm(at=(64, 64), n=(10, 40000), kinds=(1, 3), limit=1.0, out=ok, ws=ok, short=0, count=None):
+        c = len(at)
+        n = (C.c_long * c)(*n)
+        need = lib.ccnn_grad_norm_workspace_bytes(n, c)
+        assert need >= 8
+        return lib.ccnn_grad_norm((C.c_void_p * c)(*at), n, (C.c_int * c)(*kinds), c if count is None else count, limit, out, ws,
+                                  need - short, nul)
 
-    fine = (64, 64, 10, 0, 0, 0.1, 1, 1)
+    assert norm(short=1) == -2 and norm(ws=nul) == -2
+    for bad in (dict(limit=0.0), dict(limit=float("nan")), dict(out=nul), dict(count=-1), dict(at=(0, 64)), dict(n=(-1, 5)),
+                dict(kinds=(1, 7)), dict(kinds=(0, 1))):
+        assert norm(**bad) == -1, bad
 
-    def step(*ts, bits=32, m=ok, v=ok, ms=ok, vs=ok, master=ok, clock=ok, b1=0.9, b2=0.999, eps=1e-8):
-        arr = (L.AdamwTensor * max(1, len(ts)))(*ts)
-        return lib.ccnn_adamw_step(arr, len(ts), bits, m, v, ms, vs, master, clock, 1e-3, nul, b1, b2, eps, nul, nul)
+    fine = (64, 10, 0, 0, 0.1, 1)
+
+    def step(*ts, grads=None, kinds=None, bits=32, m=ok, v=ok, ms=ok, vs=ok, master=ok, clock=ok, b1=0.9, b2=0.999, eps=1e-8):
+        k = max(1, len(ts))
+        arr = (L.AdamwTensor * k)(*ts)
+        return lib.ccnn_adamw_step(arr, (C.c_void_p * k)(*(grads or [64] * k)), (C.c_int * k)(*(kinds or [t[5] for t in ts])),
+                                   len(ts), bits, m, v, ms, vs, master, clock, 1e-3, nul, b1, b2, eps, nul, nul)
 
     for bad in (dict(bits=16), dict(m=nul), dict(v=nul), dict(clock=nul), dict(b1=1.0), dict(b2=-0.1), dict(eps=-1.0),
-                dict(bits=8, ms=nul), dict(bits=8, vs=nul), dict(b1=float("nan"))):
+                dict(bits=8, ms=nul), dict(bits=8, vs=nul), dict(b1=float("nan")), dict(grads=[0]), dict(kinds=[3])):
         assert step(fine, **bad) == -1, bad
-    assert step((64, 64, 10, 0, 0, 0.1, 3, 3), master=nul) == -1           # half precision without its master copy
-    assert step((64, 64, 10, 0, 0, 0.1, 2, 2), bits=8) == -1               # 8-bit moments of doubles
-    assert step(fine, (64, 64, 10, 0, 0, 0.1, 2, 2)) == -1                 # doubles among others
-    for bad in ((0, 64, 10, 0, 0, 0.1, 1, 1), (64, 0, 10, 0, 0, 0.1, 1, 1), (64, 64, -1, 0, 0, 0.1, 1, 1),
-                (64, 64, 10, -1, 0, 0.1, 1, 1), (64, 64, 10, 0, -1, 0.1, 1, 1), (64, 64, 10, 0, 0, 0.1, 1, 3),
-                (64, 64, 10, 0, 0, 0.1, 3, 4), (64, 64, 10, 0, 0, 0.1, 0, 0)):
+    assert step((64, 10, 0, 0, 0.1, 3), master=nul) == -1                  # half precision without its master copy
+    assert step((64, 10, 0, 0, 0.1, 2), bits=8) == -1                      # 8-bit moments of doubles
+    assert step(fine, (64, 10, 0, 0, 0.1, 2)) == -1                        # doubles among others
+    assert step((64, 10, 0, 0, 0.1, 3), kinds=[4]) == -1
+    for bad in ((0, 10, 0, 0, 0.1, 1), (64, -1, 0, 0, 0.1, 1), (64, 10, -1, 0, 0.1, 1), (64, 10, 0, -1, 0.1, 1),
+                (64, 10, 0, 0, 0.1, 0)):
         assert step(bad) == -1, bad
     arr = (L.AdamwTensor * 1)(fine)
     assert lib.ccnn_adamw_moments(arr, 1, nul, ok, ok, ok, ok, ok, nul) == -1

@@ -63,7 +63,7 @@ __global__ __launch_bounds__(256) void norm_partial(NormList list, double *__res
         Pack<T, W> x[U];
 #pragma unroll
         for (int u = 0; u < U; u++)
-            if (k + u * 256 * W + W <= n) x[u] = load_pack<T, W>(p + k + u * 256 * W);
+            if (k + u * 256 * W + W <= n) x[u] = load_pack<W>(p + k + u * 256 * W);
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int at = k + u * 256 * W;
@@ -155,7 +155,7 @@ __device__ __forceinline__ A stepped(A p, A m, A v_root, const Rates<A> &r)
 template <int N, typename T>
 __device__ __forceinline__ Pack<T, N> load_some(const T *p, long k, long n)
 {
-    if (k + N <= n) return load_pack<T, N>(p + k);
+    if (k + N <= n) return load_pack<N>(p + k);
     Pack<T, N> r = {};
 #pragma unroll
     for (int e = 0; e < N; e++)
@@ -166,7 +166,7 @@ template <int N, typename T>
 __device__ __forceinline__ void store_some(T *p, long k, long n, const Pack<T, N> &r)
 {
     if (k + N <= n) {
-        store_pack<T, N>(p + k, r);
+        store_pack<N>(p + k, r);
         return;
     }
 #pragma unroll

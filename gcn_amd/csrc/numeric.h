@@ -89,21 +89,33 @@ __device__ __forceinline__ V lanes_sum(V v)
 
 // N consecutive elements in one access.  The type says only what a tensor guarantees (its element's
 // alignment): a view into a flat buffer may start anywhere, and the hardware takes such addresses.
+// What streams past once is read and written past the caches' order of use (nontemporal): of the loss over
+// 4096 x 128000 bf16 logits both together took 606 us to 501, the step with 8-bit moments 593 to 462.
 template <typename T, int N>
 struct Pack {
     T v[N];
 };
-template <typename T, int N>
+template <int BYTES> struct Words;
+template <> struct Words<8> { typedef unsigned type __attribute__((ext_vector_type(2), aligned(2))); };
+template <> struct Words<16> { typedef unsigned type __attribute__((ext_vector_type(4), aligned(2))); };
+template <> struct Words<32> { typedef unsigned type __attribute__((ext_vector_type(8), aligned(2))); };
+
+template <int N, typename T>
 __device__ __forceinline__ Pack<T, N> load_pack(const T *p)
 {
+    typedef typename Words<sizeof(Pack<T, N>)>::type V;
+    const V w = __builtin_nontemporal_load(reinterpret_cast<const V *>(p));
     Pack<T, N> r;
-    __builtin_memcpy(&r, p, sizeof(r));
+    __builtin_memcpy(&r, &w, sizeof(r));
     return r;
 }
-template <typename T, int N>
+template <int N, typename T>
 __device__ __forceinline__ void store_pack(T *p, const Pack<T, N> &r)
 {
-    __builtin_memcpy(p, &r, sizeof(r));
+    typedef typename Words<sizeof(Pack<T, N>)>::type V;
+    V w;
+    __builtin_memcpy(&w, &r, sizeof(r));
+    __builtin_nontemporal_store(w, reinterpret_cast<V *>(p));
 }
 #endif
 

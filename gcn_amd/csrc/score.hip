@@ -61,6 +61,27 @@ __device__ __forceinline__ Sums<A> join(Sums<A> a, Sums<A> b)
     return {m, a.s + b.s, a.t + b.t};
 }
 
+// The largest of a load's elements (a NaN is passed over: the sums carry it), and a distance that times 0 is 0.
+template <int W>
+__device__ __forceinline__ float max_of(const float (&x)[W])
+{
+    float m = x[0];
+#pragma unroll
+    for (int e = 1; e < W - 1; e += 2) asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(m), "v"(x[e]), "v"(x[e + 1]));
+    asm("v_max_f32 %0, %1, %2" : "=v"(m) : "v"(m), "v"(x[W - 1]));
+    return m;
+}
+template <int W>
+__device__ __forceinline__ double max_of(const double (&x)[W])
+{
+    double m = x[0];
+#pragma unroll
+    for (int e = 1; e < W; e++) m = fmax(m, x[e]);
+    return m;
+}
+__device__ __forceinline__ float floor_of(float d) { return fmaxf(d, -1e4f); }
+__device__ __forceinline__ double floor_of(double d) { return fmax(d, -1e4); }
+
 // Joined over the wave's lanes, the same in all of them.
 template <typename A>
 __device__ __forceinline__ Sums<A> over_wave(Sums<A> a)
@@ -149,7 +170,7 @@ __global__ __launch_bounds__(256) void log_probs_small(const T *__restrict__ log
     for (int e = 0; e < E; e++) {
         const A d = x[e] - from, w = expw(d);
         s += w;
-        t += w * (d < A(-1e4) ? A(-1e4) : d);       // 0 * inf is not wanted
+        t += w * floor_of(d);       // 0 * inf is not wanted
     }
     const Sums<A> sums = {m, s = lanes_sum<G>(s), t = lanes_sum<G>(t)};
     if (lane == 0) finish_row(sums, r, given, y, classes, o);
@@ -272,43 +293,48 @@ __global__ __launch_bounds__(SLICE_THREADS) void log_probs_slice(const T *__rest
         y = targets.at(r);
         if (y >= 0 && y < classes) given = widen(logits[r * stride + y]);
     }
-    A m = ninf(A()), s = 0, t = 0, best = ninf(A());
+    // Sums about `from`, which follows the largest element so far at a distance of up to LAG: e^LAG costs the sums
+    // nothing, and only a wave that meets a larger element moves them.
+    constexpr A LAG = 4;
+    A from = 0, limit = ninf(A()), s = 0, t = 0, best = ninf(A());
     int best_at = -1;
-    auto take = [&](const A *x, int count, int at) {
-        A high = x[0];
-        for (int e = 1; e < count; e++) high = x[e] > high ? x[e] : high;
+    auto take = [&](const A (&x)[W], int at) {
+        const A high = max_of(x);
         if (high > best || best_at < 0) best = high, best_at = at;
-        const A to = high > m ? high : m, from = to == ninf(A()) ? A(0) : to;
-        A f = m - to;
-        f = m == to ? A(1) : expw(f < A(-1e4) ? A(-1e4) : f);
-        if (ENTROPY) t = (t + (m == to ? A(0) : (m - to < A(-1e4) ? A(-1e4) : m - to)) * s) * f;
-        s *= f;
-        m = to;
-        for (int e = 0; e < count; e++) {
+        if (__any(high > limit)) {
+            if (high > limit) {
+                const A d = from - high, f = d < A(-1e4) ? A(0) : expw(d);
+                if (limit > ninf(A())) t = f > A(0) ? (t + d * s) * f : t * f, s *= f;
+                from = high;
+                limit = high + LAG;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < W; e++) {
             const A d = x[e] - from, w = expw(d);
             s += w;
-            if (ENTROPY) t += w * (d < A(-1e4) ? A(-1e4) : d);
+            if (ENTROPY) t += w * floor_of(d);       // 0 * inf is not wanted
         }
     };
     int i = tid;
     for (; i + (U - 1) * NT < loads; i += U * NT) {
         Pack<T, W> p[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) p[u] = load_pack<T, W>(row + (long)(i + u * NT) * W);
+        for (int u = 0; u < U; u++) p[u] = load_pack<W>(row + (long)(i + u * NT) * W);
 #pragma unroll
         for (int u = 0; u < U; u++) {
             A x[W];
 #pragma unroll
             for (int e = 0; e < W; e++) x[e] = widen(p[u].v[e]);
-            take(x, W, i + u * NT);
+            take(x, i + u * NT);
         }
     }
     for (; i < loads; i += NT) {
-        const Pack<T, W> p = load_pack<T, W>(row + (long)i * W);
+        const Pack<T, W> p = load_pack<W>(row + (long)i * W);
         A x[W];
 #pragma unroll
         for (int e = 0; e < W; e++) x[e] = widen(p.v[e]);
-        take(x, W, i);
+        take(x, i);
     }
     const int rest = n - loads * W;
     // the last, partial load belongs to the thread whose turn it is
@@ -316,10 +342,12 @@ __global__ __launch_bounds__(SLICE_THREADS) void log_probs_slice(const T *__rest
         A x[W];
 #pragma unroll
         for (int e = 0; e < W; e++) x[e] = e < rest ? (A)widen(row[(long)loads * W + e]) : ninf(A());
-        take(x, W, loads);
+        take(x, loads);
     }
 
-    Sums<A> sums = over_wave(Sums<A>{m, s, t});
+    Sums<A> sums = {limit > ninf(A()) ? from : ninf(A()), s, t};
+    shift(sums, best);
+    sums = over_wave(sums);
     if (lane == 0) lds.m[wave] = sums.m, lds.s[wave] = sums.s, lds.t[wave] = sums.t;
     if (o.top) lds.key[tid] = best_at < 0 ? Key<A>(0) : key_of(best, best_at);
     if (tid == 0) lds.n_owners = lds.n_found = 0;
@@ -360,7 +388,7 @@ __global__ __launch_bounds__(SLICE_THREADS) void log_probs_slice(const T *__rest
         const int at = lds.owners[task / turns] + (task % turns) * NT;
         const int count = at < loads ? W : at == loads ? rest : 0;
         Pack<T, W> p;
-        if (count == W) p = load_pack<T, W>(row + (long)at * W);
+        if (count == W) p = load_pack<W>(row + (long)at * W);
         else {
 #pragma unroll
             for (int e = 0; e < W; e++)
@@ -480,7 +508,7 @@ __global__ __launch_bounds__(256) void log_probs_grad_small(const T *logits, lon
         narrow(row.at((A)widen(logits[r * stride + j]), j), d_logits[r * d_stride + j]);
 }
 
-constexpr int GRAD_LOADS = 4;
+constexpr int GRAD_LOADS = 2;   // 1 and 4 are a few per cent slower over 1 GB of logits
 
 template <typename T>
 __global__ __launch_bounds__(256) void log_probs_grad_wide(const T *logits, int classes, long stride, Targets targets,
@@ -488,8 +516,7 @@ __global__ __launch_bounds__(256) void log_probs_grad_wide(const T *logits, int 
 {
     typedef Wide<T> A;
     constexpr int W = 16 / sizeof(T);
-    // rows from the last to the first: those the forward pass read last are still in the memory-side cache
-    const long r = gridDim.y - 1 - blockIdx.y;
+    const long r = blockIdx.y;
     const T *x = logits + r * stride;
     T *d = d_logits + r * d_stride;
     const int first = blockIdx.x * (256 * GRAD_LOADS * W) + threadIdx.x * W;
@@ -497,7 +524,7 @@ __global__ __launch_bounds__(256) void log_probs_grad_wide(const T *logits, int 
 #pragma unroll
     for (int u = 0; u < GRAD_LOADS; u++) {
         const int j = first + u * 256 * W;
-        if (j + W <= classes) p[u] = load_pack<T, W>(x + j);
+        if (j + W <= classes) p[u] = load_pack<W>(x + j);
     }
     const GradRow<A> row(in, targets, r, classes);
 #pragma unroll
@@ -506,7 +533,7 @@ __global__ __launch_bounds__(256) void log_probs_grad_wide(const T *logits, int 
         if (j + W <= classes) {
 #pragma unroll
             for (int e = 0; e < W; e++) narrow(row.at((A)widen(p[u].v[e]), j + e), p[u].v[e]);
-            store_pack<T, W>(d + j, p[u]);
+            store_pack<W>(d + j, p[u]);
         } else {
             for (int e = j; e < classes; e++) narrow(row.at((A)widen(x[e]), e), d[e]);
         }
@@ -602,12 +629,12 @@ int score_grad_impl(const void *logits, long rows, int classes, long stride, Tar
         return 0;
     }
     const long tile = 256 * GRAD_LOADS * (16 / sizeof(T));
-    for (long r1 = rows; r1 > 0; r1 -= 65535) {
-        const long r0 = r1 > 65535 ? r1 - 65535 : 0;
+    for (long r0 = 0; r0 < rows; r0 += 65535) {
+        const long nr = rows - r0 < 65535 ? rows - r0 : 65535;
         const GradIn<A> is = {in.stats + 2 * r0, in.entropy ? in.entropy + r0 : nullptr, in.d_logp ? in.d_logp + r0 : nullptr,
                               in.d_entropy ? in.d_entropy + r0 : nullptr};
         const Targets ts = {(const char *)targets.p + r0 * targets.bytes, targets.bytes};
-        launch("log_probs_grad_wide", log_probs_grad_wide<T>, dim3((unsigned)((classes + tile - 1) / tile), (unsigned)(r1 - r0)),
+        launch("log_probs_grad_wide", log_probs_grad_wide<T>, dim3((unsigned)((classes + tile - 1) / tile), (unsigned)nr),
                dim3(256), 0, st, x + r0 * stride, classes, stride, ts, is, d + r0 * d_stride, d_stride);
         CCNN_LAUNCH_CHECK();
     }

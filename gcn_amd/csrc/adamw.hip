@@ -2,8 +2,7 @@
 // with moments in 32 bits or in 8.  They stand beside the update rules of forward.hip (plain and AdaGrad).
 //
 // Both read a list of tensors of any sizes in as few launches as possible: the list travels in the
-// kernel's arguments (LIST tensors a launch), every tensor is cut into chunks, and a workgroup finds
-// its chunk's tensor by bisection over the chunk counts.
+// kernel's arguments, every tensor is cut into chunks, and a workgroup finds its chunk's tensor there.
 #include <cmath>
 #include <type_traits>
 
@@ -12,29 +11,32 @@
 
 namespace ccnn {
 
-constexpr int LIST = 64;          // tensors per launch: the argument block stays under 4 KB
+// tensors per launch: the argument block stays under 4 KB
+constexpr int NORM_TENSORS = 192, STEP_TENSORS = 64;
 constexpr int BLOCK = CCNN_MOMENT_BLOCK;
 
 // ---------------------------------------------------------------------------- gradient norm
 constexpr long NORM_CHUNK = 16384;
 
 struct NormList {
-    const void *data[LIST];
-    long n[LIST];
-    int chunk0[LIST + 1];   // first chunk of each tensor; [count] = all
+    static constexpr int MOST = NORM_TENSORS;
+    const void *data[MOST];
+    long n[MOST];
+    int chunk0[MOST + 1];   // first chunk of each tensor; [count] = all
     int count;
 };
 
+// The tensor of a chunk: how many of the list's first chunks are not behind it, 64 looked at at once (a bisection
+// is six loads after each other).
 template <typename L>
 __device__ __forceinline__ int find(const L &list, int chunk)
 {
-    int lo = 0, hi = list.count;   // chunk0[lo] <= chunk < chunk0[hi]
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (list.chunk0[mid] <= chunk) lo = mid;
-        else hi = mid;
+    int before = -1;
+    for (int base = 0; base < list.count; base += 64) {
+        const int i = base + (threadIdx.x & 63);
+        before += __popcll(__ballot(i < list.count && list.chunk0[i] <= chunk));
     }
-    return lo;
+    return __builtin_amdgcn_readfirstlane(before);
 }
 
 // Sum over a workgroup of N threads in a fixed order; the result is in every thread.
@@ -79,6 +81,13 @@ __global__ __launch_bounds__(256) void norm_partial(NormList list, double *__res
     if (threadIdx.x == 0) partial[blockIdx.x] = s;
 }
 
+__device__ __forceinline__ void put_norm(double squares, double max_norm, double *out)
+{
+    const double norm = sqrt(squares);
+    out[0] = norm;
+    out[1] = !(norm < __builtin_huge_val()) ? __builtin_nan("") : norm > max_norm ? max_norm / norm : 1.0;
+}
+
 constexpr int TOTAL_THREADS = 1024;
 
 __global__ __launch_bounds__(TOTAL_THREADS) void norm_total(const double *__restrict__ partial, int n, double max_norm,
@@ -89,23 +98,46 @@ __global__ __launch_bounds__(TOTAL_THREADS) void norm_total(const double *__rest
 #pragma unroll 4
     for (int k = threadIdx.x; k < n; k += TOTAL_THREADS) s += partial[k];
     s = block_sum<TOTAL_THREADS>(s, lds);
-    if (threadIdx.x == 0) {
-        const double norm = sqrt(s);
-        out[0] = norm;
-        out[1] = !(norm < __builtin_huge_val()) ? __builtin_nan("") : norm > max_norm ? max_norm / norm : 1.0;
+    if (threadIdx.x == 0) put_norm(s, max_norm, out);
+}
+
+// Few gradients: one workgroup for all of them, each of its waves taking every 16th piece, in place of two launches.
+constexpr long PIECE = 2048, ONE_PIECES = 64;
+
+template <typename T>
+__global__ __launch_bounds__(TOTAL_THREADS) void norm_one(NormList list, double max_norm, double *__restrict__ out)
+{
+    constexpr int W = 16 / sizeof(T), U = PIECE / (64 * W);
+    __shared__ double lds[TOTAL_THREADS / 64];
+    const int lane = threadIdx.x & 63;
+    double s = 0;
+    for (int c = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); c < list.chunk0[list.count]; c += TOTAL_THREADS / 64) {
+        const int i = find(list, c);
+        const T *p = (const T *)list.data[i];
+        const long n = list.n[i], lo = (c - list.chunk0[i]) * PIECE + lane * W;
+        Pack<T, W> x[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) x[u] = load_some<W>(p, lo + u * 64 * W, n);
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int e = 0; e < W; e++) s += (double)widen(x[u].v[e]) * (double)widen(x[u].v[e]);
     }
+    s = block_sum<TOTAL_THREADS>(s, lds);
+    if (threadIdx.x == 0) put_norm(s, max_norm, out);
 }
 
 // ---------------------------------------------------------------------------- AdamW
-constexpr long STEP_CHUNK = 4096;
+constexpr long CODED_CHUNK = 2048, DECODE_CHUNK = 4096;
 
 struct StepList {
-    void *param[LIST];
-    const void *grad[LIST];
-    long n[LIST], first[LIST];
-    int block[LIST];
-    double decay[LIST];
-    int chunk0[LIST + 1];
+    static constexpr int MOST = STEP_TENSORS;
+    void *param[MOST];
+    const void *grad[MOST];
+    long n[MOST], first[MOST];
+    int block[MOST];
+    double decay[MOST];
+    int chunk0[MOST + 1];
     int count;
 };
 
@@ -151,77 +183,52 @@ __device__ __forceinline__ A stepped(A p, A m, A v_root, const Rates<A> &r)
     return p - (r.lr_decay * p + r.rate * m / (v_root * r.root + r.eps));
 }
 
-// N elements at p + k of a tensor of n, zeros behind its end.
-template <int N, typename T>
-__device__ __forceinline__ Pack<T, N> load_some(const T *p, long k, long n)
-{
-    if (k + N <= n) return load_pack<N>(p + k);
-    Pack<T, N> r = {};
-#pragma unroll
-    for (int e = 0; e < N; e++)
-        if (k + e < n) r.v[e] = p[k + e];
-    return r;
-}
-template <int N, typename T>
-__device__ __forceinline__ void store_some(T *p, long k, long n, const Pack<T, N> &r)
-{
-    if (k + N <= n) {
-        store_pack<N>(p + k, r);
-        return;
-    }
-#pragma unroll
-    for (int e = 0; e < N; e++)
-        if (k + e < n) p[k + e] = r.v[e];
-}
-
-template <typename P, typename G>
+// U packs of four elements in flight per thread.
+template <typename P, typename G, int U>
 __global__ __launch_bounds__(256) void adamw_wide(StepList list, StepArgs a)
 {
     typedef Wide<P> A;
     constexpr bool COPY = sizeof(P) == 2;   // the parameter is the rounding of its master copy
     typedef std::conditional_t<COPY, float, P> S;
-    constexpr int W = 4, U = sizeof(P) == 8 ? 2 : 4;
+    constexpr int W = 4;
     const int i = find(list, blockIdx.x);
-    const Rates<A> r(a, list.decay[i]);
-    if (r.skip) return;
     P *param = (P *)list.param[i];
     const G *grad = (const G *)list.grad[i];
     A *m = (A *)a.m + list.first[i], *v = (A *)a.v + list.first[i];
     S *held;
     if constexpr (COPY) held = a.master + list.first[i];
     else held = param;
-    const long lo = (long)(blockIdx.x - list.chunk0[i]) * STEP_CHUNK;
-    const long n = min(list.n[i], lo + STEP_CHUNK);
+    const long k0 = (long)(blockIdx.x - list.chunk0[i]) * (U * 256 * W) + threadIdx.x * W, n = list.n[i];
+    Pack<A, W> mk[U], vk[U];
+    Pack<S, W> pk[U];
+    Pack<G, W> gk[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const long k = k0 + u * 256 * W;
+        gk[u] = load_some<W>(grad, k, n);
+        mk[u] = load_some<W>(m, k, n);
+        vk[u] = load_some<W>(v, k, n);
+        pk[u] = load_some<W>(held, k, n);
+    }
+    const Rates<A> r(a, list.decay[i]);
+    if (r.skip) return;
     const A b1 = (A)(1 - a.beta1), b2 = (A)(1 - a.beta2);
-    for (long k0 = lo + threadIdx.x * W; k0 < n; k0 += U * 256 * W) {
-        Pack<A, W> mk[U], vk[U];
-        Pack<S, W> pk[U];
-        Pack<G, W> gk[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const long k = k0 + u * 256 * W;
-            gk[u] = load_some<W>(grad, k, n);
-            mk[u] = load_some<W>(m, k, n);
-            vk[u] = load_some<W>(v, k, n);
-            pk[u] = load_some<W>(held, k, n);
+    for (int u = 0; u < U; u++) {
+        const long k = k0 + u * 256 * W;
+        Pack<P, W> out;
+#pragma unroll
+        for (int e = 0; e < W; e++) {
+            const A g = (A)widen(gk[u].v[e]) * r.scale;
+            mk[u].v[e] += b1 * (g - mk[u].v[e]);
+            vk[u].v[e] += b2 * (g * g - vk[u].v[e]);
+            pk[u].v[e] = stepped((A)pk[u].v[e], mk[u].v[e], (A)sqrt(vk[u].v[e]), r);
+            narrow(pk[u].v[e], out.v[e]);
         }
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const long k = k0 + u * 256 * W;
-            Pack<P, W> out;
-#pragma unroll
-            for (int e = 0; e < W; e++) {
-                const A g = (A)widen(gk[u].v[e]) * r.scale;
-                mk[u].v[e] += b1 * (g - mk[u].v[e]);
-                vk[u].v[e] += b2 * (g * g - vk[u].v[e]);
-                pk[u].v[e] = stepped((A)pk[u].v[e], mk[u].v[e], (A)sqrt(vk[u].v[e]), r);
-                narrow(pk[u].v[e], out.v[e]);
-            }
-            store_some<W>(m, k, n, mk[u]);
-            store_some<W>(v, k, n, vk[u]);
-            if constexpr (COPY) store_some<W>(held, k, n, pk[u]);
-            store_some<W>(param, k, n, out);
-        }
+        store_some<W>(m, k, n, mk[u]);
+        store_some<W>(v, k, n, vk[u]);
+        if constexpr (COPY) store_some<W>(held, k, n, pk[u]);
+        store_some<W>(param, k, n, out);
     }
 }
 
@@ -307,23 +314,22 @@ __device__ __forceinline__ float block_scale(const double (&x)[4])
     return u >= 0x7f800000u ? __builtin_nanf("") : __uint_as_float(u) / 448.0f;
 }
 
-// One wave per block of 256 elements, four to a lane, four blocks in flight.  Moments, root and step in fp64.
+// One wave per block of 256 elements, four to a lane, two blocks in flight (one costs 6 % at 100 M parameters, four
+// 2 %).  Moments, root and step in fp64.
 template <typename P, typename G>
 __global__ __launch_bounds__(256) void adamw_coded(StepList list, StepArgs a)
 {
     constexpr bool COPY = sizeof(P) == 2;
     typedef std::conditional_t<COPY, float, P> S;
-    constexpr int U = STEP_CHUNK / (4 * BLOCK);
+    constexpr int U = CODED_CHUNK / (4 * BLOCK);
     const int i = find(list, blockIdx.x);
-    const Rates<double> r(a, list.decay[i]);
-    if (r.skip) return;
     P *param = (P *)list.param[i];
     const G *grad = (const G *)list.grad[i];
     S *held;
     if constexpr (COPY) held = a.master + list.first[i];
     else held = param;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long n = list.n[i], b0 = (long)(blockIdx.x - list.chunk0[i]) * STEP_CHUNK + wave * (U * BLOCK);
+    const long n = list.n[i], b0 = (long)(blockIdx.x - list.chunk0[i]) * CODED_CHUNK + wave * (U * BLOCK);
     const long blk0 = list.block[i] + b0 / BLOCK;
     const double rest1 = 1 - a.beta1, rest2 = 1 - a.beta2;
     Pack<G, 4> gk[U];
@@ -341,6 +347,8 @@ __global__ __launch_bounds__(256) void adamw_coded(StepList list, StepArgs a)
         ms[u] = a.m_scale[blk0 + u];
         vs[u] = a.v_scale[blk0 + u];
     }
+    const Rates<double> r(a, list.decay[i]);
+    if (r.skip) return;
 #pragma unroll
     for (int u = 0; u < U; u++) {
         if (b0 + u * BLOCK >= n) break;
@@ -376,9 +384,9 @@ __global__ __launch_bounds__(256) void adamw_decode(StepList list, const unsigne
                                                     const float *__restrict__ m_scale, const float *__restrict__ v_scale,
                                                     float *__restrict__ m_out, float *__restrict__ v_out)
 {
-    constexpr int U = STEP_CHUNK / (4 * 256);
+    constexpr int U = DECODE_CHUNK / (4 * 256);
     const int i = find(list, blockIdx.x);
-    const long n = list.n[i], k0 = (long)(blockIdx.x - list.chunk0[i]) * STEP_CHUNK + threadIdx.x * 4;
+    const long n = list.n[i], k0 = (long)(blockIdx.x - list.chunk0[i]) * DECODE_CHUNK + threadIdx.x * 4;
     const long at0 = (long)list.block[i] * BLOCK + k0;
     unsigned mc[U], vc[U];
     float ms[U], vs[U];
@@ -405,7 +413,8 @@ __global__ __launch_bounds__(256) void adamw_decode(StepList list, const unsigne
 }
 
 // ---------------------------------------------------------------------------- host
-// Hands tensors [0, count) that `take` accepts to `go`, LIST at a time, with their chunks counted.
+constexpr long WIDE_SMALL = 1 << 20;   // elements
+// Hands tensors [0, count) that `take` accepts to `go`, a list at a time, with their chunks counted.
 template <typename List, typename Take, typename Go>
 int in_lists(int count, long chunk, Take take, Go go)
 {
@@ -420,7 +429,7 @@ int in_lists(int count, long chunk, Take take, Go go)
             chunks = (n + chunk - 1) / chunk;
             if (chunks > 0x3fffffffL) return CCNN_E_RANGE;
         }
-        const bool full = list.count == LIST || (list.count > 0 && list.chunk0[list.count] + chunks > 0x7fffffffL);
+        const bool full = list.count == List::MOST || (list.count > 0 && list.chunk0[list.count] + chunks > 0x7fffffffL);
         if (list.count > 0 && (i == count || full)) {
             if (int e = go(list)) return e;
             list.count = 0;
@@ -463,14 +472,20 @@ int ccnn_grad_norm(const void *const *data, const long *n, const int *types, int
     if (!workspace || workspace_bytes < need) return CCNN_E_WORKSPACE;
     hipStream_t st = (hipStream_t)stream;
     double *partial = (double *)workspace;
-    int done = 0;
+    int done = 0, kinds = 0, only = 0;
+    long pieces = 0;
+    for (int type = CCNN_TYPE_F32; type <= CCNN_TYPE_F16; type++)
+        if (used[type]) kinds++, only = type;
+    for (int i = 0; i < count; i++) pieces += (n[i] + PIECE - 1) / PIECE;
+    const bool one = kinds == 1 && count <= NORM_TENSORS && pieces > 0 && pieces <= ONE_PIECES;
+    const long chunk = one ? PIECE : NORM_CHUNK;
     for (int type = CCNN_TYPE_F32; type <= CCNN_TYPE_F16; type++) {
         if (!used[type]) continue;
         const int e = in_lists<NormList>(
-            count, NORM_CHUNK,
+            count, chunk,
             [&](NormList &list, int i) -> long {
                 if (types[i] != type) return 0;
-                if (list.count < LIST) {
+                if (list.count < NormList::MOST) {
                     list.data[list.count] = data[i];
                     list.n[list.count] = n[i];
                 }
@@ -478,6 +493,15 @@ int ccnn_grad_norm(const void *const *data, const long *n, const int *types, int
             },
             [&](const NormList &list) -> int {
                 const int chunks = list.chunk0[list.count];
+                if (one) {
+                    launch("norm_one", only == CCNN_TYPE_F32   ? norm_one<float>
+                                       : only == CCNN_TYPE_F64 ? norm_one<double>
+                                       : only == CCNN_TYPE_BF16 ? norm_one<Bf16>
+                                                                : norm_one<F16>,
+                           dim3(1), dim3(TOTAL_THREADS), 0, st, list, max_norm, out);
+                    CCNN_LAUNCH_CHECK();
+                    return 0;
+                }
                 const dim3 grid((unsigned)chunks), block(256);
                 if (type == CCNN_TYPE_F32) launch("norm_partial", norm_partial<float>, grid, block, 0, st, list, partial + done);
                 else if (type == CCNN_TYPE_F64) launch("norm_partial", norm_partial<double>, grid, block, 0, st, list, partial + done);
@@ -489,6 +513,7 @@ int ccnn_grad_norm(const void *const *data, const long *n, const int *types, int
             });
         if (e) return e;
     }
+    if (one) return 0;
     launch("norm_total", norm_total, dim3(1), dim3(TOTAL_THREADS), 0, st, partial, done, max_norm, out);
     CCNN_LAUNCH_CHECK();
     return 0;
@@ -501,7 +526,8 @@ int ccnn_adamw_step(const ccnn_adamw_tensor_t *tensors, const void *const *grads
     if (count < 0 || (count > 0 && (!tensors || !grads || !grad_types)) || !clock) return CCNN_E_INVALID;
     if (moment_bits != 32 && moment_bits != 8) return CCNN_E_INVALID;
     if (!(beta1 >= 0 && beta1 < 1) || !(beta2 >= 0 && beta2 < 1) || !(eps >= 0)) return CCNN_E_INVALID;
-    bool wide = false, other = false, any = false;
+    bool wide = false, other = false;
+    long total = 0;
     for (int i = 0; i < count; i++) {
         const ccnn_adamw_tensor_t &t = tensors[i];
         const bool half = t.type == CCNN_TYPE_BF16 || t.type == CCNN_TYPE_F16;
@@ -510,33 +536,37 @@ int ccnn_adamw_step(const ccnn_adamw_tensor_t *tensors, const void *const *grads
         if (moment_bits == 8 && t.block > 0x7fffffffL) return CCNN_E_RANGE;
         if (half && t.n > 0 && !master) return CCNN_E_INVALID;
         (t.type == CCNN_TYPE_F64 ? wide : other) = true;
-        any |= t.n > 0;
+        total += t.n;
     }
     if (wide && (other || moment_bits == 8)) return CCNN_E_INVALID;
-    if (any && (!m || !v || (moment_bits == 8 && (!m_scale || !v_scale)))) return CCNN_E_INVALID;
+    if (total > 0 && (!m || !v || (moment_bits == 8 && (!m_scale || !v_scale)))) return CCNN_E_INVALID;
     hipStream_t st = (hipStream_t)stream;
     launch("adamw_clock", adamw_clock, dim3(1), dim3(1), 0, st, clock, lr, lr_device, beta1, beta2, clip);
     CCNN_LAUNCH_CHECK();
     const StepArgs args = {m, v, m_scale, v_scale, master, clock, beta1, beta2, eps};
     typedef void (*Kern)(StepList, StepArgs);
+    // One pack a thread until the parameters fill the device with them: a step of 47 k parameters is all latency
+    // (9.3 us in packs of four, see WIDE_SMALL); four in flight stream better beyond.
+    const bool small = total < WIDE_SMALL;
     const struct {
         int type, grad_type;
-        Kern wide, coded;
+        Kern one, four, coded;
     } kinds[] = {
-        {CCNN_TYPE_F32, CCNN_TYPE_F32, adamw_wide<float, float>, adamw_coded<float, float>},
-        {CCNN_TYPE_F64, CCNN_TYPE_F64, adamw_wide<double, double>, nullptr},
-        {CCNN_TYPE_BF16, CCNN_TYPE_BF16, adamw_wide<Bf16, Bf16>, adamw_coded<Bf16, Bf16>},
-        {CCNN_TYPE_BF16, CCNN_TYPE_F32, adamw_wide<Bf16, float>, adamw_coded<Bf16, float>},
-        {CCNN_TYPE_F16, CCNN_TYPE_F16, adamw_wide<F16, F16>, adamw_coded<F16, F16>},
-        {CCNN_TYPE_F16, CCNN_TYPE_F32, adamw_wide<F16, float>, adamw_coded<F16, float>},
+        {CCNN_TYPE_F32, CCNN_TYPE_F32, adamw_wide<float, float, 1>, adamw_wide<float, float, 4>, adamw_coded<float, float>},
+        {CCNN_TYPE_F64, CCNN_TYPE_F64, adamw_wide<double, double, 1>, adamw_wide<double, double, 4>, nullptr},
+        {CCNN_TYPE_BF16, CCNN_TYPE_BF16, adamw_wide<Bf16, Bf16, 1>, adamw_wide<Bf16, Bf16, 4>, adamw_coded<Bf16, Bf16>},
+        {CCNN_TYPE_BF16, CCNN_TYPE_F32, adamw_wide<Bf16, float, 1>, adamw_wide<Bf16, float, 4>, adamw_coded<Bf16, float>},
+        {CCNN_TYPE_F16, CCNN_TYPE_F16, adamw_wide<F16, F16, 1>, adamw_wide<F16, F16, 4>, adamw_coded<F16, F16>},
+        {CCNN_TYPE_F16, CCNN_TYPE_F32, adamw_wide<F16, float, 1>, adamw_wide<F16, float, 4>, adamw_coded<F16, float>},
     };
     for (const auto &kind : kinds) {
+        const Kern kern = moment_bits == 8 ? kind.coded : small ? kind.one : kind.four;
         const int e = in_lists<StepList>(
-            count, STEP_CHUNK,
+            count, moment_bits == 8 ? CODED_CHUNK : small ? 1024 : 4096,
             [&](StepList &list, int i) -> long {
                 const ccnn_adamw_tensor_t &t = tensors[i];
                 if (t.type != kind.type || grad_types[i] != kind.grad_type) return 0;
-                if (const int c = list.count; c < LIST) {
+                if (const int c = list.count; c < StepList::MOST) {
                     list.param[c] = t.param;
                     list.grad[c] = grads[i];
                     list.n[c] = t.n;
@@ -547,7 +577,7 @@ int ccnn_adamw_step(const ccnn_adamw_tensor_t *tensors, const void *const *grads
                 return t.n;
             },
             [&](const StepList &list) -> int {
-                launch(moment_bits == 8 ? "adamw_coded" : "adamw_wide", moment_bits == 8 ? kind.coded : kind.wide,
+                launch(moment_bits == 8 ? "adamw_coded" : "adamw_wide", kern,
                        dim3((unsigned)list.chunk0[list.count]), dim3(256), 0, st, list, args);
                 CCNN_LAUNCH_CHECK();
                 return 0;
@@ -567,9 +597,9 @@ int ccnn_adamw_moments(const ccnn_adamw_tensor_t *tensors, int count, const void
         if (tensors[i].block > 0x7fffffffL) return CCNN_E_RANGE;
     }
     return in_lists<StepList>(
-        count, STEP_CHUNK,
+        count, DECODE_CHUNK,
         [&](StepList &list, int i) -> long {
-            if (const int c = list.count; c < LIST) {
+            if (const int c = list.count; c < StepList::MOST) {
                 list.n[c] = tensors[i].n;
                 list.first[c] = tensors[i].first;
                 list.block[c] = (int)tensors[i].block;

@@ -117,6 +117,28 @@ __device__ __forceinline__ void store_pack(T *p, const Pack<T, N> &r)
     __builtin_memcpy(&w, &r, sizeof(r));
     __builtin_nontemporal_store(w, reinterpret_cast<V *>(p));
 }
+// N elements at p + k of a tensor of n, zeros behind its end.
+template <int N, typename T>
+__device__ __forceinline__ Pack<T, N> load_some(const T *p, long k, long n)
+{
+    if (k + N <= n) return load_pack<N>(p + k);
+    Pack<T, N> r = {};
+#pragma unroll
+    for (int e = 0; e < N; e++)
+        if (k + e < n) r.v[e] = p[k + e];
+    return r;
+}
+template <int N, typename T>
+__device__ __forceinline__ void store_some(T *p, long k, long n, const Pack<T, N> &r)
+{
+    if (k + N <= n) {
+        store_pack<N>(p + k, r);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < N; e++)
+        if (k + e < n) p[k + e] = r.v[e];
+}
 #endif
 
 }  // namespace ccnn

@@ -366,6 +366,25 @@ def _at(t):
     return t.data_ptr() if t is not None else None
 
 
+_T = torch.Tensor
+
+
+def _one_device(tensors, name, dtypes):
+    """The device that all the contiguous tensors are on."""
+    try:
+        if len(set(map(_T.get_device, tensors))) == 1 and all(map(_T.is_contiguous, tensors)) and tensors[0].is_cuda \
+                and all(t.dtype in dtypes for t in tensors):
+            return tensors[0].device
+    except (TypeError, RuntimeError):
+        pass
+    for i, t in enumerate(tensors):      # something is wrong: say what
+        _on_device(t, f"{name} {i}", dtypes)
+        _same_device(t, f"{name} {i}", tensors[0].device)
+        if not t.is_contiguous():
+            raise ValueError(f"{name} {i} must be contiguous")
+    raise TypeError(f"{name} list cannot be used")
+
+
 _raw_stream, _current = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
@@ -487,15 +506,9 @@ def grad_norm(grads, max_norm=float("inf")):
         raise ValueError("grad_norm needs at least one tensor")
     if not max_norm > 0:
         raise ValueError(f"max_norm must be positive, got {max_norm}")
-    dev = grads[0].device if isinstance(grads[0], torch.Tensor) else None
-    count = len(grads)
-    for i, g in enumerate(grads):
-        _on_device(g, f"gradient {i}", _TYPES)
-        if g.device != dev or not g.is_contiguous():
-            _same_device(g, f"gradient {i}", dev)
-            raise ValueError(f"gradient {i} must be contiguous")
-    at = (C.c_void_p * count)(*[g.data_ptr() for g in grads])
-    n = (C.c_long * count)(*[g.numel() for g in grads])
+    count, dev = len(grads), _one_device(grads, "gradient", _TYPES)
+    at = (C.c_void_p * count)(*map(_T.data_ptr, grads))
+    n = (C.c_long * count)(*map(_T.numel, grads))
     kinds = (C.c_int * count)(*[_TYPES[g.dtype] for g in grads])
     out = torch.empty(2, dtype=_F64, device=dev)
     nbytes = _l.load().ccnn_grad_norm_workspace_bytes(n, count)
@@ -559,7 +572,7 @@ class AdamW:
             raise ValueError("parameter tensors overlap")
         self.numel, self.blocks = first, block
         # what each gradient is held against, and the types' table for the usual case that they are the parameters'
-        self._expected = [(p.dtype, p.numel()) for p in self.params]
+        self._numels, self._dtypes = [p.numel() for p in self.params], [p.dtype for p in self.params]
         self._kinds = (C.c_int * n)(*[t.type for t in self._table])
         wide = _F64 if self.params[0].dtype == _F64 else _F32
         if state_bits == 32:
@@ -590,19 +603,17 @@ class AdamW:
         count = len(self.params)
         if len(grads) != count:
             raise ValueError(f"{len(grads)} gradients for {count} parameters")
-        for i, (g, (dtype, n)) in enumerate(zip(grads, self._expected)):
-            if not (isinstance(g, torch.Tensor) and g.is_cuda and g.dtype == dtype and g.device == dev and g.is_contiguous()
-                    and g.numel() == n):
+        if _one_device(grads, "gradient", _TYPES) != dev:
+            raise ValueError(f"gradients are on {grads[0].device}, the parameters on {dev}")
+        if list(map(_T.numel, grads)) != self._numels:
+            i = [g.numel() == n for g, n in zip(grads, self._numels)].index(False)
+            raise ValueError(f"gradient {i} has {grads[i].numel()} elements, its parameter {self._numels[i]}")
+        dtypes = [g.dtype for g in grads]
+        if dtypes != self._dtypes:
+            for i, (g, dtype) in enumerate(zip(grads, self._dtypes)):
                 _on_device(g, f"gradient {i}", (dtype, _F32) if dtype.itemsize == 2 else (dtype,))
-                _same_device(g, f"gradient {i}", dev)
-                if not g.is_contiguous():
-                    raise ValueError(f"gradient {i} must be contiguous")
-                if g.numel() != n:
-                    raise ValueError(f"gradient {i} has {g.numel()} elements, its parameter {n}")
-                kinds = None
-        if kinds is None:
-            kinds = (C.c_int * count)(*[_TYPES[g.dtype] for g in grads])
-        at = (C.c_void_p * count)(*[g.data_ptr() for g in grads])
+            kinds = (C.c_int * count)(*[_TYPES[d] for d in dtypes])
+        at = (C.c_void_p * count)(*map(_T.data_ptr, grads))
         if clip is not None:
             _req(clip, _F64, "clip", 2)
             _same_device(clip, "clip", self.device)

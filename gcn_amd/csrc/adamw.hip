@@ -11,15 +11,17 @@
 
 namespace ccnn {
 
-// tensors per launch: the argument block stays under 4 KB
-constexpr int NORM_TENSORS = 192, STEP_TENSORS = 64;
+// Tensors per launch: the argument block stays under 4 KB, and is short where a launch's latency counts (3 KB of
+// arguments cost the host 1.8 us more than a few words).
+constexpr int NORM_TENSORS = 192, STEP_TENSORS = 64, FEW_TENSORS = 16;
 constexpr int BLOCK = CCNN_MOMENT_BLOCK;
 
 // ---------------------------------------------------------------------------- gradient norm
 constexpr long NORM_CHUNK = 16384;
 
+template <int N>
 struct NormList {
-    static constexpr int MOST = NORM_TENSORS;
+    static constexpr int MOST = N;
     const void *data[MOST];
     long n[MOST];
     int chunk0[MOST + 1];   // first chunk of each tensor; [count] = all
@@ -53,7 +55,7 @@ __device__ __forceinline__ double block_sum(double v, double *lds)
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void norm_partial(NormList list, double *__restrict__ partial)
+__global__ __launch_bounds__(256) void norm_partial(NormList<NORM_TENSORS> list, double *__restrict__ partial)
 {
     constexpr int W = 16 / sizeof(T), U = 8;
     __shared__ double lds[4];
@@ -105,7 +107,7 @@ __global__ __launch_bounds__(TOTAL_THREADS) void norm_total(const double *__rest
 constexpr long PIECE = 2048, ONE_PIECES = 64;
 
 template <typename T>
-__global__ __launch_bounds__(TOTAL_THREADS) void norm_one(NormList list, double max_norm, double *__restrict__ out)
+__global__ __launch_bounds__(TOTAL_THREADS) void norm_one(NormList<FEW_TENSORS> list, double max_norm, double *__restrict__ out)
 {
     constexpr int W = 16 / sizeof(T), U = PIECE / (64 * W);
     __shared__ double lds[TOTAL_THREADS / 64];
@@ -130,8 +132,9 @@ __global__ __launch_bounds__(TOTAL_THREADS) void norm_one(NormList list, double 
 // ---------------------------------------------------------------------------- AdamW
 constexpr long CODED_CHUNK = 2048, DECODE_CHUNK = 4096;
 
+template <int N>
 struct StepList {
-    static constexpr int MOST = STEP_TENSORS;
+    static constexpr int MOST = N;
     void *param[MOST];
     const void *grad[MOST];
     long n[MOST], first[MOST];
@@ -185,7 +188,7 @@ __device__ __forceinline__ A stepped(A p, A m, A v_root, const Rates<A> &r)
 
 // U packs of four elements in flight per thread.
 template <typename P, typename G, int U>
-__global__ __launch_bounds__(256) void adamw_wide(StepList list, StepArgs a)
+__global__ __launch_bounds__(256) void adamw_wide(StepList<U == 1 ? FEW_TENSORS : STEP_TENSORS> list, StepArgs a)
 {
     typedef Wide<P> A;
     constexpr bool COPY = sizeof(P) == 2;   // the parameter is the rounding of its master copy
@@ -317,7 +320,7 @@ __device__ __forceinline__ float block_scale(const double (&x)[4])
 // One wave per block of 256 elements, four to a lane, two blocks in flight (one costs 6 % at 100 M parameters, four
 // 2 %).  Moments, root and step in fp64.
 template <typename P, typename G>
-__global__ __launch_bounds__(256) void adamw_coded(StepList list, StepArgs a)
+__global__ __launch_bounds__(256) void adamw_coded(StepList<STEP_TENSORS> list, StepArgs a)
 {
     constexpr bool COPY = sizeof(P) == 2;
     typedef std::conditional_t<COPY, float, P> S;
@@ -380,7 +383,7 @@ __global__ __launch_bounds__(256) void adamw_coded(StepList list, StepArgs a)
     }
 }
 
-__global__ __launch_bounds__(256) void adamw_decode(StepList list, const unsigned *__restrict__ m, const unsigned *__restrict__ v,
+__global__ __launch_bounds__(256) void adamw_decode(StepList<STEP_TENSORS> list, const unsigned *__restrict__ m, const unsigned *__restrict__ v,
                                                     const float *__restrict__ m_scale, const float *__restrict__ v_scale,
                                                     float *__restrict__ m_out, float *__restrict__ v_out)
 {
@@ -413,7 +416,9 @@ __global__ __launch_bounds__(256) void adamw_decode(StepList list, const unsigne
 }
 
 // ---------------------------------------------------------------------------- host
-constexpr long WIDE_SMALL = 1 << 20;   // elements
+// Below so many elements a step of few tensors takes one pack a thread and a short argument block: it is all latency
+// (47 k fp32 parameters: 5.3 us of the device instead of 9.3 in packs of four).
+constexpr long WIDE_SMALL = 1 << 20;
 // Hands tensors [0, count) that `take` accepts to `go`, a list at a time, with their chunks counted.
 template <typename List, typename Take, typename Go>
 int in_lists(int count, long chunk, Take take, Go go)
@@ -477,43 +482,46 @@ int ccnn_grad_norm(const void *const *data, const long *n, const int *types, int
     for (int type = CCNN_TYPE_F32; type <= CCNN_TYPE_F16; type++)
         if (used[type]) kinds++, only = type;
     for (int i = 0; i < count; i++) pieces += (n[i] + PIECE - 1) / PIECE;
-    const bool one = kinds == 1 && count <= NORM_TENSORS && pieces > 0 && pieces <= ONE_PIECES;
-    const long chunk = one ? PIECE : NORM_CHUNK;
+    auto take = [&](auto &list, int i, int type) -> long {
+        if (types[i] != type) return 0;
+        if (list.count < list.MOST) {
+            list.data[list.count] = data[i];
+            list.n[list.count] = n[i];
+        }
+        return n[i];
+    };
+    if (kinds == 1 && count <= FEW_TENSORS && pieces > 0 && pieces <= ONE_PIECES) {
+        typedef NormList<FEW_TENSORS> List;
+        return in_lists<List>(
+            count, PIECE, [&](List &list, int i) { return take(list, i, only); },
+            [&](const List &list) -> int {
+                launch("norm_one", only == CCNN_TYPE_F32    ? norm_one<float>
+                                   : only == CCNN_TYPE_F64  ? norm_one<double>
+                                   : only == CCNN_TYPE_BF16 ? norm_one<Bf16>
+                                                            : norm_one<F16>,
+                       dim3(1), dim3(TOTAL_THREADS), 0, st, list, max_norm, out);
+                CCNN_LAUNCH_CHECK();
+                return 0;
+            });
+    }
     for (int type = CCNN_TYPE_F32; type <= CCNN_TYPE_F16; type++) {
         if (!used[type]) continue;
-        const int e = in_lists<NormList>(
-            count, chunk,
-            [&](NormList &list, int i) -> long {
-                if (types[i] != type) return 0;
-                if (list.count < NormList::MOST) {
-                    list.data[list.count] = data[i];
-                    list.n[list.count] = n[i];
-                }
-                return n[i];
-            },
-            [&](const NormList &list) -> int {
+        typedef NormList<NORM_TENSORS> List;
+        const int e = in_lists<List>(
+            count, NORM_CHUNK, [&](List &list, int i) { return take(list, i, type); },
+            [&](const List &list) -> int {
                 const int chunks = list.chunk0[list.count];
-                if (one) {
-                    launch("norm_one", only == CCNN_TYPE_F32   ? norm_one<float>
-                                       : only == CCNN_TYPE_F64 ? norm_one<double>
-                                       : only == CCNN_TYPE_BF16 ? norm_one<Bf16>
-                                                                : norm_one<F16>,
-                           dim3(1), dim3(TOTAL_THREADS), 0, st, list, max_norm, out);
-                    CCNN_LAUNCH_CHECK();
-                    return 0;
-                }
-                const dim3 grid((unsigned)chunks), block(256);
-                if (type == CCNN_TYPE_F32) launch("norm_partial", norm_partial<float>, grid, block, 0, st, list, partial + done);
-                else if (type == CCNN_TYPE_F64) launch("norm_partial", norm_partial<double>, grid, block, 0, st, list, partial + done);
-                else if (type == CCNN_TYPE_BF16) launch("norm_partial", norm_partial<Bf16>, grid, block, 0, st, list, partial + done);
-                else launch("norm_partial", norm_partial<F16>, grid, block, 0, st, list, partial + done);
+                launch("norm_partial", type == CCNN_TYPE_F32    ? norm_partial<float>
+                                       : type == CCNN_TYPE_F64  ? norm_partial<double>
+                                       : type == CCNN_TYPE_BF16 ? norm_partial<Bf16>
+                                                                : norm_partial<F16>,
+                       dim3((unsigned)chunks), dim3(256), 0, st, list, partial + done);
                 CCNN_LAUNCH_CHECK();
                 done += chunks;
                 return 0;
             });
         if (e) return e;
     }
-    if (one) return 0;
     launch("norm_total", norm_total, dim3(1), dim3(TOTAL_THREADS), 0, st, partial, done, max_norm, out);
     CCNN_LAUNCH_CHECK();
     return 0;
@@ -544,13 +552,13 @@ int ccnn_adamw_step(const ccnn_adamw_tensor_t *tensors, const void *const *grads
     launch("adamw_clock", adamw_clock, dim3(1), dim3(1), 0, st, clock, lr, lr_device, beta1, beta2, clip);
     CCNN_LAUNCH_CHECK();
     const StepArgs args = {m, v, m_scale, v_scale, master, clock, beta1, beta2, eps};
-    typedef void (*Kern)(StepList, StepArgs);
-    // One pack a thread until the parameters fill the device with them: a step of 47 k parameters is all latency
-    // (9.3 us in packs of four, see WIDE_SMALL); four in flight stream better beyond.
-    const bool small = total < WIDE_SMALL;
+    typedef StepList<FEW_TENSORS> Few;
+    typedef StepList<STEP_TENSORS> Many;
     const struct {
         int type, grad_type;
-        Kern one, four, coded;
+        void (*one)(Few, StepArgs);
+        void (*four)(Many, StepArgs);
+        void (*coded)(Many, StepArgs);
     } kinds[] = {
         {CCNN_TYPE_F32, CCNN_TYPE_F32, adamw_wide<float, float, 1>, adamw_wide<float, float, 4>, adamw_coded<float, float>},
         {CCNN_TYPE_F64, CCNN_TYPE_F64, adamw_wide<double, double, 1>, adamw_wide<double, double, 4>, nullptr},
@@ -559,25 +567,31 @@ int ccnn_adamw_step(const ccnn_adamw_tensor_t *tensors, const void *const *grads
         {CCNN_TYPE_F16, CCNN_TYPE_F16, adamw_wide<F16, F16, 1>, adamw_wide<F16, F16, 4>, adamw_coded<F16, F16>},
         {CCNN_TYPE_F16, CCNN_TYPE_F32, adamw_wide<F16, float, 1>, adamw_wide<F16, float, 4>, adamw_coded<F16, float>},
     };
+    const bool small = moment_bits == 32 && total < WIDE_SMALL && count <= FEW_TENSORS;
     for (const auto &kind : kinds) {
-        const Kern kern = moment_bits == 8 ? kind.coded : small ? kind.one : kind.four;
-        const int e = in_lists<StepList>(
-            count, moment_bits == 8 ? CODED_CHUNK : small ? 1024 : 4096,
-            [&](StepList &list, int i) -> long {
-                const ccnn_adamw_tensor_t &t = tensors[i];
-                if (t.type != kind.type || grad_types[i] != kind.grad_type) return 0;
-                if (const int c = list.count; c < StepList::MOST) {
-                    list.param[c] = t.param;
-                    list.grad[c] = grads[i];
-                    list.n[c] = t.n;
-                    list.first[c] = t.first;
-                    list.block[c] = (int)t.block;
-                    list.decay[c] = t.decay;
-                }
-                return t.n;
-            },
-            [&](const StepList &list) -> int {
-                launch(moment_bits == 8 ? "adamw_coded" : "adamw_wide", kern,
+        auto take = [&](auto &list, int i) -> long {
+            const ccnn_adamw_tensor_t &t = tensors[i];
+            if (t.type != kind.type || grad_types[i] != kind.grad_type) return 0;
+            if (const int c = list.count; c < list.MOST) {
+                list.param[c] = t.param;
+                list.grad[c] = grads[i];
+                list.n[c] = t.n;
+                list.first[c] = t.first;
+                list.block[c] = (int)t.block;
+                list.decay[c] = t.decay;
+            }
+            return t.n;
+        };
+        int e;
+        if (small)
+            e = in_lists<Few>(count, 1024, take, [&](const Few &list) -> int {
+                launch("adamw_wide", kind.one, dim3((unsigned)list.chunk0[list.count]), dim3(256), 0, st, list, args);
+                CCNN_LAUNCH_CHECK();
+                return 0;
+            });
+        else
+            e = in_lists<Many>(count, moment_bits == 8 ? CODED_CHUNK : 4096, take, [&](const Many &list) -> int {
+                launch(moment_bits == 8 ? "adamw_coded" : "adamw_wide", moment_bits == 8 ? kind.coded : kind.four,
                        dim3((unsigned)list.chunk0[list.count]), dim3(256), 0, st, list, args);
                 CCNN_LAUNCH_CHECK();
                 return 0;
@@ -596,17 +610,18 @@ int ccnn_adamw_moments(const ccnn_adamw_tensor_t *tensors, int count, const void
         if (tensors[i].n > 0 && (!m || !v || !m_scale || !v_scale || !m_out || !v_out)) return CCNN_E_INVALID;
         if (tensors[i].block > 0x7fffffffL) return CCNN_E_RANGE;
     }
-    return in_lists<StepList>(
+    typedef StepList<STEP_TENSORS> List;
+    return in_lists<List>(
         count, DECODE_CHUNK,
-        [&](StepList &list, int i) -> long {
-            if (const int c = list.count; c < StepList::MOST) {
+        [&](List &list, int i) -> long {
+            if (const int c = list.count; c < list.MOST) {
                 list.n[c] = tensors[i].n;
                 list.first[c] = tensors[i].first;
                 list.block[c] = (int)tensors[i].block;
             }
             return tensors[i].n;
         },
-        [&](const StepList &list) -> int {
+        [&](const List &list) -> int {
             launch("adamw_decode", adamw_decode, dim3((unsigned)list.chunk0[list.count]), dim3(256), 0, (hipStream_t)stream,
                    list, (const unsigned *)m, (const unsigned *)v, m_scale, v_scale, m_out, v_out);
             CCNN_LAUNCH_CHECK();

@@ -307,10 +307,11 @@ struct FcTrainOut {
 };
 
 // NO: the class count when it is the reference's 13 (compile-time then), 0 for any other (no_rt).
+// want_logits: probs gets what the softmax is taken of instead.
 template <typename T, int MS, bool TRAIN, int NO>
 __global__ __launch_bounds__(256) void fc_head_fwd(const T *__restrict__ params, int off_w1, int off_b1,
                                                    int off_w2, int off_b2, int no_rt, const T *__restrict__ pool,
-                                                   int nrows, int pout, T *__restrict__ probs,
+                                                   int nrows, int pout, T *__restrict__ probs, int want_logits,
                                                    int *__restrict__ argmax, int *__restrict__ ctr,
                                                    FcTrainOut<T> tr)
 {
@@ -493,7 +494,8 @@ __global__ __launch_bounds__(256) void fc_head_fwd(const T *__restrict__ params,
     } else {
         for (int i = 0; i < H; i++) m0 = m0 + w2s[o0 + i * no] * zr[i];
     }
-    const T e0 = rexp(m0 + b2s[o0]), e1 = rexp(m1 + b2s[o1]);
+    const T x0 = m0 + b2s[o0], x1 = m1 + b2s[o1];
+    const T e0 = rexp(x0), e1 = rexp(x1);
     if (has0) es[s * 16 + o0] = e0;
     if (has1) es[s * 16 + o1] = e1;
     __syncthreads();
@@ -502,8 +504,8 @@ __global__ __launch_bounds__(256) void fc_head_fwd(const T *__restrict__ params,
     if (has0) ps[s * 16 + o0] = p0;
     if (has1) ps[s * 16 + o1] = p1;
     if (s < nb_done && probs) {
-        if (has0) probs[(long)(r0_done + s) * no + o0] = p0;
-        if (has1) probs[(long)(r0_done + s) * no + o1] = p1;
+        if (has0) probs[(long)(r0_done + s) * no + o0] = want_logits ? x0 : p0;
+        if (has1) probs[(long)(r0_done + s) * no + o1] = want_logits ? x1 : p1;
     }
     __syncthreads();
     if (argmax && jl == 0 && s < nb_done) {
@@ -662,7 +664,7 @@ template <typename T, bool FLIP>
 int forward_impl(const T *params, const T *cubes, long n, int z, T *probs, int *argmax, void *ws,
                  size_t ws_bytes, hipStream_t st, const int *idx9 = nullptr, long plane = 0,
                  const FcTrainOut<T> *tr = nullptr, long first = 0, T *pool_out = nullptr, unsigned char *px = nullptr,
-                 int *ctr_out = nullptr)
+                 int *ctr_out = nullptr, bool want_logits = false)
 {
     ccnn_dims_t d;
     if (make_dims(z, &d)) return CCNN_E_INVALID;
@@ -705,7 +707,7 @@ int forward_impl(const T *params, const T *cubes, long n, int z, T *probs, int *
         }
     }
     if (nwv == 0) return CCNN_E_RANGE;
-    typedef void (*FcKern)(const T *, int, int, int, int, int, const T *, int, int, T *, int *, int *, FcTrainOut<T>);
+    typedef void (*FcKern)(const T *, int, int, int, int, int, const T *, int, int, T *, int, int *, int *, FcTrainOut<T>);
     constexpr int C13 = CCNN_CLASSES;
     const bool c13 = d.n_classes == C13;
     const FcKern fc32 = train ? (c13 ? fc_head_fwd<T, 32, true, C13> : fc_head_fwd<T, 32, true, 0>)
@@ -740,7 +742,7 @@ int forward_impl(const T *params, const T *cubes, long n, int z, T *probs, int *
             launch(train ? "fc_head_fwd_train" : "fc_head_fwd", small ? fc16 : fc32, dim3(fg), dim3(256),
                    small ? FcHeadLds<T, 16>::bytes : FcHeadLds<T, 32>::bytes, st,
                    params, d.off_w1, d.off_b1, d.off_w2, d.off_b2, d.n_classes, w.pool, nr, d.pout,
-                   probs ? probs + s0 * d.n_classes : nullptr, argmax ? argmax + s0 : nullptr, w.ctr,
+                   probs ? probs + s0 * d.n_classes : nullptr, (int)want_logits, argmax ? argmax + s0 : nullptr, w.ctr,
                    tr ? *tr : FcTrainOut<T>{});
         }
         CCNN_LAUNCH_CHECK();
@@ -803,6 +805,22 @@ int ccnn_forward_f64(const double *params, const double *cubes, long n, int z, d
 {
     return forward_impl<double, false>(params, cubes, n, z, probs, argmax, workspace, workspace_bytes,
                                        (hipStream_t)stream);
+}
+
+int ccnn_forward_logits_f32(const float *params, const float *cubes, long n, int z, float *logits, int *argmax,
+                            void *workspace, size_t workspace_bytes, void *stream)
+{
+    if (!logits && n > 0) return CCNN_E_INVALID;
+    return forward_impl<float, true>(params, cubes, n, z, logits, argmax, workspace, workspace_bytes, (hipStream_t)stream,
+                                     nullptr, 0, nullptr, 0, nullptr, nullptr, nullptr, true);
+}
+
+int ccnn_forward_logits_f64(const double *params, const double *cubes, long n, int z, double *logits, int *argmax,
+                            void *workspace, size_t workspace_bytes, void *stream)
+{
+    if (!logits && n > 0) return CCNN_E_INVALID;
+    return forward_impl<double, false>(params, cubes, n, z, logits, argmax, workspace, workspace_bytes, (hipStream_t)stream,
+                                       nullptr, 0, nullptr, 0, nullptr, nullptr, nullptr, true);
 }
 
 int ccnn_forward_scene_f32(const float *params, const float *scene, const int *idx9, long n, int x, int y, int z,

@@ -55,6 +55,8 @@ _SIG = {
     "ccnn_forward_workspace_bytes": (C.c_size_t, [C.c_long, C.c_int, C.c_int]),
     "ccnn_forward_f32": (C.c_int, [_P, _P, C.c_long, C.c_int, _P, _P, _P, C.c_size_t, _P]),
     "ccnn_forward_f64": (C.c_int, [_P, _P, C.c_long, C.c_int, _P, _P, _P, C.c_size_t, _P]),
+    "ccnn_forward_logits_f32": (C.c_int, [_P, _P, C.c_long, C.c_int, _P, _P, _P, C.c_size_t, _P]),
+    "ccnn_forward_logits_f64": (C.c_int, [_P, _P, C.c_long, C.c_int, _P, _P, _P, C.c_size_t, _P]),
     "ccnn_count_correct": (C.c_int, [_P, _P, C.c_long, _P, _P]),
     "ccnn_sgd_workspace_bytes": (C.c_size_t, [C.c_int]),
     "ccnn_sgd_f64": (C.c_int, [_P, _P, _P, C.c_long, C.c_long, C.c_int, C.c_double, _P, _P, C.c_size_t, _P]),

@@ -153,6 +153,24 @@ def forward(params, cubes, z, want_probs=True, want_argmax=True, workspace=None)
     return probs, argmax
 
 
+def forward_logits(params, cubes, z, workspace=None):
+    """The test-loop forward up to its last layer: logits [n, classes], for log_probs."""
+    sfx, es = _sfx(params.dtype)
+    d = _l.dims(z)
+    _req(params, params.dtype, "params", d.nparams)
+    n = cubes.numel() // d.cube
+    _req(cubes, params.dtype, "cubes", n * d.cube)
+    logits = torch.empty((n, d.n_classes), dtype=params.dtype, device=params.device)
+    if n == 0:
+        return logits
+    lib = _l.load()
+    ws = (workspace or Workspace(params.device)).get(lib.ccnn_forward_workspace_bytes(n, z, es))
+    fn = getattr(lib, f"ccnn_forward_logits_{sfx}")
+    _l.check(fn(_ptr(params), _ptr(cubes), n, z, _ptr(logits), None, _ptr(ws), ws.numel(), _stream()),
+             f"ccnn_forward_logits_{sfx}")
+    return logits
+
+
 def forward_scene(params, scene, idx9, x, y, z, want_probs=True, want_argmax=True, workspace=None):
     """forward() on pixels of the scene: idx9 int32 [n, 9] neighbour lists; no cubes are stored."""
     sfx, es = _sfx(params.dtype)

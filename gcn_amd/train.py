@@ -7,6 +7,8 @@ functions over the C ABI.
                hyper_version_mGPU_MBGD.cu:957-1200 (one all-reduce per step
                instead of weight broadcast + gradient-slab gather)
     evaluate   the test loop + count_err (gcn_mbgd_fp64.cu:1182-1231)
+    score      the test pixels' log probabilities, entropies and runners-up
+    adamw      AdamW over the network's tensors, for fit_mbgd(optimizer=...)
 
 The loops keep the reference's bookkeeping: batch_num = T // B (the tail is
 dropped), epoch loss = sum of the per-sample losses / T (all T, although the tail
@@ -109,7 +111,8 @@ class MbgdStepper:
 
 
 def fit_mbgd(params, cubes, onehot, z, batch=100, lr=None, min_err=None, max_iter=300, fifo_init=None,
-             group=None, distributed=False, train_size=None, stepper=None, log=None, keep_tail=False):
+             group=None, distributed=False, train_size=None, stepper=None, log=None, keep_tail=False, optimizer=None,
+             max_norm=None):
     """Minibatch epochs; params updated in place (identically on every rank).
 
     Single process: cubes/onehot hold all T training samples.
@@ -120,8 +123,19 @@ def fit_mbgd(params, cubes, onehot, z, batch=100, lr=None, min_err=None, max_ite
     keep_tail (single process only): the last T % batch samples form a short final batch whose
     mean is taken over its own size (hyper_version_MBGD.cu:780, 794-796) instead of being
     dropped (gcn_mbgd_fp64.cu:895).
+    optimizer: an ops.AdamW over views of `params` (train.adamw makes one) that takes the steps instead of the
+    trainers' own rule, from the gradient summed over the batch (and the ranks); lr is then its own unless
+    given, and falls by the same schedule.  max_norm: the norm the batch's mean gradient is clipped to; a step
+    whose norm is not finite is left out.
     """
     f32 = params.dtype == torch.float32
+    if max_norm is not None and optimizer is None:
+        raise ValueError("max_norm needs an optimizer")
+    if optimizer is not None:
+        places = _places(optimizer, params)
+        lr = optimizer.lr if lr is None else lr
+        if isinstance(lr, torch.Tensor):
+            raise ValueError("the schedule needs lr as a number")
     lr = (0.04 if f32 else 0.5) if lr is None else lr
     min_err = (0.001 if f32 else 0.0001) if min_err is None else min_err
     fifo_init = (100.0 if f32 else 1.0) if fifo_init is None else fifo_init
@@ -136,7 +150,7 @@ def fit_mbgd(params, cubes, onehot, z, batch=100, lr=None, min_err=None, max_ite
         raise ValueError("this rank's slice is shorter than batch_num sub-batches")
     st = stepper or MbgdStepper(params, cubes, onehot, z)
     node = None
-    if distributed and stepper is None and params.is_cuda and comm.world > 1:
+    if distributed and stepper is None and optimizer is None and params.is_cuda and comm.world > 1:
         # gradient exchange + update in one kernel over xGMI; the group's own all_reduce (RCCL)
         # stays the fallback when the exchange cannot be set up or fails its self-test
         from .comm import NodeComm
@@ -157,7 +171,14 @@ def fit_mbgd(params, cubes, onehot, z, batch=100, lr=None, min_err=None, max_ite
     hist = History()
     for it in range(max_iter):
         for i0, (first, nb) in enumerate(steps):
-            if comm.world == 1 and stepper is None:
+            if optimizer is not None:
+                g = comm.all_reduce(st.grad(first, nb, loss_d[i0]))
+                grads = [g[a:b] for a, b in places]
+                clip = None
+                if max_norm is not None:
+                    clip = ops.grad_norm(grads, max_norm * (batch if nb == sub_b else nb))
+                optimizer.step(grads, lr=lr, clip=clip)
+            elif comm.world == 1 and stepper is None:
                 st.step_fused(first, nb, lr, loss_d[i0])
             elif node is not None and not node.shared_device:
                 ops.mbgd_step(params, cubes, onehot, first, nb, z, lr, loss_values=loss_d[i0], workspace=st.ws,
@@ -205,6 +226,39 @@ def fit_mbgd(params, cubes, onehot, z, batch=100, lr=None, min_err=None, max_ite
     if node is not None:
         node.close()
     return hist
+
+
+def _places(optimizer, params):
+    """Where in the flat vector each of the optimizer's tensors lies."""
+    places, size, base = [], params.element_size(), params.data_ptr()
+    for p in optimizer.params:
+        at, off = divmod(p.data_ptr() - base, size)
+        if p.dtype != params.dtype or off or at < 0 or at + p.numel() > params.numel():
+            raise ValueError("the optimizer's tensors must be views of params")
+        places.append((at, at + p.numel()))
+    return places
+
+
+def adamw(params, z, lr=1e-3, weight_decay=0.01, **options):
+    """ops.AdamW over the network's tensors in the flat vector `params`: decay on the weights, none on the
+    biases.  In fp32 the convolution's bias stays out, as that trainer never updates it
+    (gcn_mbgd_fp32.cu:1052-1059)."""
+    views = ops.param_views(params, z)
+    decays = [weight_decay, 0.0] * 3
+    if params.dtype == torch.float32:
+        del views[1], decays[1]
+    return ops.AdamW(views, lr=lr, weight_decay=decays, **options)
+
+
+def score(params, cubes, labels, z, top=3):
+    """ops.LogProbs of pixels against their labels (1..classes, int32; 0 = unlabelled, log probability 0):
+    how likely the model finds each label, how sure it is, and its `top` likeliest classes (counted
+    from 0)."""
+    n = labels.numel()
+    logits = ops.forward_logits(params, cubes, z)
+    if logits.shape[0] != n:
+        raise ValueError(f"{logits.shape[0]} pixels but {n} labels")
+    return ops.log_probs(logits, labels.reshape(-1) - 1, top=min(top, logits.shape[1]))
 
 
 def evaluate(params, cubes, test_labels, z):

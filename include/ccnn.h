@@ -127,6 +127,13 @@ int ccnn_forward_f32(const float *params, const float *cubes, long n, int z, flo
 int ccnn_forward_f64(const double *params, const double *cubes, long n, int z, double *probs,
                      int *argmax, void *workspace, size_t workspace_bytes, void *stream);
 
+/* ccnn_forward_* with the logits [n][13] the softmax is taken of in the place of the probabilities, for
+ * ccnn_log_probs (which keeps what exp would round away or overflow); argmax as above, optional. */
+int ccnn_forward_logits_f32(const float *params, const float *cubes, long n, int z, float *logits,
+                            int *argmax, void *workspace, size_t workspace_bytes, void *stream);
+int ccnn_forward_logits_f64(const double *params, const double *cubes, long n, int z, double *logits,
+                            int *argmax, void *workspace, size_t workspace_bytes, void *stream);
+
 /* ccnn_forward_* fed from the scene instead of pre-gathered cubes: sample i is the
  * neighbourhood idx9[i][0..9) and its cube element b*9+j is read as
  * scene[idx9[i][j] + b*x*y] inside the convolution kernel (preprocessing,

@@ -88,7 +88,7 @@ def weights(rows, kind, seed=1):
 
 
 SHAPES = [(1, 1), (1, 2), (3, 13), (257, 13), (5, 16), (7, 17), (130, 31), (4, 64), (3, 65), (9, 255), (2, 1000), (5, 1024),
-          (3, 1025), (2, 2049), (3, 4097), (1, 32003), (4, 50251), (1, 128000), (2, 131073), (70, 8191)]
+          (16385, 13), (16400, 41), (16390, 200), (20000, 5), (3, 1025), (2, 2049), (3, 4097), (1, 32003), (4, 50251), (1, 128000), (2, 131073), (70, 8191)]
 
 
 @pytest.mark.parametrize("kind", KINDS, ids=str)

@@ -186,9 +186,11 @@ __device__ __forceinline__ A stepped(A p, A m, A v_root, const Rates<A> &r)
     return p - (r.lr_decay * p + r.rate * m / (v_root * r.root + r.eps));
 }
 
-// U packs of four elements in flight per thread.
+// A wave to a chunk, U packs of four elements in flight per lane.
+constexpr int WIDE_THREADS = 64;
+
 template <typename P, typename G, int U>
-__global__ __launch_bounds__(256) void adamw_wide(StepList<U == 1 ? FEW_TENSORS : STEP_TENSORS> list, StepArgs a)
+__global__ __launch_bounds__(WIDE_THREADS) void adamw_wide(StepList<U == 1 ? FEW_TENSORS : STEP_TENSORS> list, StepArgs a)
 {
     typedef Wide<P> A;
     constexpr bool COPY = sizeof(P) == 2;   // the parameter is the rounding of its master copy
@@ -201,13 +203,13 @@ __global__ __launch_bounds__(256) void adamw_wide(StepList<U == 1 ? FEW_TENSORS 
     S *held;
     if constexpr (COPY) held = a.master + list.first[i];
     else held = param;
-    const long k0 = (long)(blockIdx.x - list.chunk0[i]) * (U * 256 * W) + threadIdx.x * W, n = list.n[i];
+    const long k0 = (long)(blockIdx.x - list.chunk0[i]) * (U * WIDE_THREADS * W) + threadIdx.x * W, n = list.n[i];
     Pack<A, W> mk[U], vk[U];
     Pack<S, W> pk[U];
     Pack<G, W> gk[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        const long k = k0 + u * 256 * W;
+        const long k = k0 + u * WIDE_THREADS * W;
         gk[u] = load_some<W>(grad, k, n);
         mk[u] = load_some<W>(m, k, n);
         vk[u] = load_some<W>(v, k, n);
@@ -218,7 +220,7 @@ __global__ __launch_bounds__(256) void adamw_wide(StepList<U == 1 ? FEW_TENSORS 
     const A b1 = (A)(1 - a.beta1), b2 = (A)(1 - a.beta2);
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        const long k = k0 + u * 256 * W;
+        const long k = k0 + u * WIDE_THREADS * W;
         Pack<P, W> out;
 #pragma unroll
         for (int e = 0; e < W; e++) {
@@ -584,15 +586,15 @@ int ccnn_adamw_step(const ccnn_adamw_tensor_t *tensors, const void *const *grads
         };
         int e;
         if (small)
-            e = in_lists<Few>(count, 1024, take, [&](const Few &list) -> int {
-                launch("adamw_wide", kind.one, dim3((unsigned)list.chunk0[list.count]), dim3(256), 0, st, list, args);
+            e = in_lists<Few>(count, WIDE_THREADS * 4, take, [&](const Few &list) -> int {
+                launch("adamw_wide", kind.one, dim3((unsigned)list.chunk0[list.count]), dim3(WIDE_THREADS), 0, st, list, args);
                 CCNN_LAUNCH_CHECK();
                 return 0;
             });
         else
-            e = in_lists<Many>(count, moment_bits == 8 ? CODED_CHUNK : 4096, take, [&](const Many &list) -> int {
+            e = in_lists<Many>(count, moment_bits == 8 ? CODED_CHUNK : WIDE_THREADS * 16, take, [&](const Many &list) -> int {
                 launch(moment_bits == 8 ? "adamw_coded" : "adamw_wide", moment_bits == 8 ? kind.coded : kind.four,
-                       dim3((unsigned)list.chunk0[list.count]), dim3(256), 0, st, list, args);
+                       dim3((unsigned)list.chunk0[list.count]), dim3(moment_bits == 8 ? 256 : WIDE_THREADS), 0, st, list, args);
                 CCNN_LAUNCH_CHECK();
                 return 0;
             });

@@ -251,40 +251,39 @@ __device__ __forceinline__ unsigned encode8(double y)
     return (unsigned)(u >> 49) - ((1023u - 7u) << 3);
 }
 
-__device__ __forceinline__ unsigned pack_codes(const double (&x)[4], float scale, bool floor)
+// Four codes of x / scale; positive: no sign, and what v says is above 0 keeps at least the smallest code.
+template <bool POSITIVE>
+__device__ __forceinline__ unsigned exact_codes(const double (&x)[4], const double (&v)[4], float scale)
 {
+    if (scale == 0) return 0;
     unsigned w = 0;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-        const double y = fabs(x[e]);
-        unsigned c = scale > 0 ? encode8(fmin(y / scale, 448.0)) : scale == 0 ? 0u : 0x7fu;
-        if (y != y) c = 0x7f;
-        if (floor && y > 0 && scale > 0 && c == 0) c = 1;
-        if (x[e] < 0) c |= 0x80;
+        const double y = fabs(x[e]) / scale;
+        unsigned c = y == y ? encode8(fmin(y, 448.0)) : 0x7fu;
+        if (POSITIVE && c == 0 && v[e] > 0) c = 1;
+        if (!POSITIVE && x[e] < 0) c |= 0x80;
         w |= c << (8 * e);
     }
     return w;
 }
 
-// The same, for all but a few in a hundred blocks: y in fp32 is within 2^-22 of itself, so where it gives the
-// same codes a little larger and a little smaller, no border lies between it and the exact quotient.
-// Scales outside the range where that holds, and blocks with an undecided element, go the way above.
-__device__ __forceinline__ unsigned quick_codes(const double (&x)[4], float scale, bool floor)
+// The same, for all but a few in a hundred blocks: y in fp32 is within 2^-21.5 of itself (three roundings and a
+// reciprocal), so where 2^-21 less and 2^-21 more give the same codes, no border lies between it and the
+// exact quotient.  Blocks with an undecided element or a root to be kept above 0, and scales outside the range
+// where that holds, go the way above.
+template <bool POSITIVE>
+__device__ __forceinline__ unsigned codes(const double (&x)[4], const double (&v)[4], const float (&x32)[4], float scale)
 {
-    const float inv = 1.0f / scale;
+    const float inv = __builtin_amdgcn_rcpf(scale), more = inv * (1.0f + 0x1p-21f), less = inv * (1.0f - 0x1p-21f);
     unsigned up = 0, down = 0;
-    float y[4];
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-        y[e] = (float)x[e] * inv;
-        if (floor) y[e] = x[e] > 0 ? fmaxf(y[e], 0x1p-9f) : y[e];
-    }
-    constexpr float MORE = 1.0f + 0x1p-21f, LESS = 1.0f - 0x1p-21f;
-    up = __builtin_amdgcn_cvt_pk_fp8_f32(y[0] * MORE, y[1] * MORE, up, false);
-    up = __builtin_amdgcn_cvt_pk_fp8_f32(y[2] * MORE, y[3] * MORE, up, true);
-    down = __builtin_amdgcn_cvt_pk_fp8_f32(y[0] * LESS, y[1] * LESS, down, false);
-    down = __builtin_amdgcn_cvt_pk_fp8_f32(y[2] * LESS, y[3] * LESS, down, true);
-    if (__any(up != down) || !(scale > 1e-30f && scale < 1e30f)) return pack_codes(x, scale, floor);
+    up = __builtin_amdgcn_cvt_pk_fp8_f32(x32[0] * more, x32[1] * more, up, false);
+    up = __builtin_amdgcn_cvt_pk_fp8_f32(x32[2] * more, x32[3] * more, up, true);
+    down = __builtin_amdgcn_cvt_pk_fp8_f32(x32[0] * less, x32[1] * less, down, false);
+    down = __builtin_amdgcn_cvt_pk_fp8_f32(x32[2] * less, x32[3] * less, down, true);
+    bool open = up != down;
+    if (POSITIVE) open |= ((down - 0x01010101u) & ~down & 0x80808080u) != 0;     // a byte of 0
+    if (!(scale > 1e-30f && scale < 1e30f) || __any(open)) return exact_codes<POSITIVE>(x, v, scale);
     return up;
 }
 
@@ -298,25 +297,25 @@ __device__ __forceinline__ double decay_to(double beta, double rest, double old,
     return a + b;
 }
 
-// sqrt to the last bit or two: the hardware's 2^-24 start and two corrections.
+// sqrt to the last bit or two: the hardware's 2^-24 start and two corrections.  0 gives 1e-150, which no fp32 and
+// no step can tell from it (but 1 / sqrt(0) * 0 could not be corrected).
 __device__ __forceinline__ double root64(double v)
 {
+    v += 1e-300;
     const double y = __builtin_amdgcn_rsq(v), h = 0.5 * y;
     double s = v * y;
     s = fma(fma(-s, s, v), h, s);
-    s = fma(fma(-s, s, v), h, s);
-    return v == 0 ? 0.0 : s;
+    return fma(fma(-s, s, v), h, s);
 }
 
-// (largest magnitude of the block in fp32) / 448, NaN if one of them is not finite; any NaN's bits are above
-// all others'.
-__device__ __forceinline__ float block_scale(const double (&x)[4])
+// h / 448, correctly rounded: of every fp32 from 1e-30 on the product with RN(1/448) is corrected to it by its
+// residual, below the quotient may be subnormal.
+__device__ __forceinline__ float scale_of(float h)
 {
-    unsigned u = 0;
-#pragma unroll
-    for (int e = 0; e < 4; e++) u = max(u, __float_as_uint((float)x[e]) & 0x7fffffffu);
-    u = lanes_max<64>(u);
-    return u >= 0x7f800000u ? __builtin_nanf("") : __uint_as_float(u) / 448.0f;
+    constexpr float INV = 1.0f / 448.0f;
+    if (h < 1e-30f) return h / 448.0f;
+    const float q = h * INV;
+    return fmaf(fmaf(-448.0f, q, h), INV, q);
 }
 
 // One wave per block of 256 elements, four to a lane, two blocks in flight (one costs 6 % at 100 M parameters, four
@@ -358,17 +357,20 @@ __global__ __launch_bounds__(256) void adamw_coded(StepList<STEP_TENSORS> list, 
     for (int u = 0; u < U; u++) {
         if (b0 + u * BLOCK >= n) break;
         const long k = b0 + u * BLOCK + lane * 4;
-        double m[4], root[4];
+        double m[4], v[4], root[4];
+        float m32[4], root32[4];
         Pack<P, 4> out;
-        const double old_m[4] = {__builtin_amdgcn_cvt_f32_fp8((int)mc[u], 0), __builtin_amdgcn_cvt_f32_fp8((int)mc[u], 1),
-                                 __builtin_amdgcn_cvt_f32_fp8((int)mc[u], 2), __builtin_amdgcn_cvt_f32_fp8((int)mc[u], 3)};
-        const double old_v[4] = {__builtin_amdgcn_cvt_f32_fp8((int)vc[u], 0), __builtin_amdgcn_cvt_f32_fp8((int)vc[u], 1),
-                                 __builtin_amdgcn_cvt_f32_fp8((int)vc[u], 2), __builtin_amdgcn_cvt_f32_fp8((int)vc[u], 3)};
+        const auto m01 = __builtin_amdgcn_cvt_pk_f32_fp8((int)mc[u], false), m23 = __builtin_amdgcn_cvt_pk_f32_fp8((int)mc[u], true);
+        const auto v01 = __builtin_amdgcn_cvt_pk_f32_fp8((int)vc[u], false), v23 = __builtin_amdgcn_cvt_pk_f32_fp8((int)vc[u], true);
+        const float old_m[4] = {m01[0], m01[1], m23[0], m23[1]}, old_v[4] = {v01[0], v01[1], v23[0], v23[1]};
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const double g = (double)widen(gk[u].v[e]) * r.scale, vo = old_v[e] * (double)vs[u];
-            m[e] = decay_to(a.beta1, rest1, old_m[e] * (double)ms[u], g);
-            root[e] = root64(decay_to(a.beta2, rest2, vo * vo, g * g));
+            const double g = (double)widen(gk[u].v[e]) * r.scale, vo = (double)old_v[e] * (double)vs[u];
+            m[e] = decay_to(a.beta1, rest1, (double)old_m[e] * (double)ms[u], g);
+            v[e] = decay_to(a.beta2, rest2, vo * vo, g * g);
+            root[e] = root64(v[e]);
+            m32[e] = (float)m[e];
+            root32[e] = (float)root[e];
             const double d = fma(root[e], r.root, r.eps);
             double x = __builtin_amdgcn_rcp(d);
             x = fma(fma(-d, x, 1.0), x, x);
@@ -378,9 +380,14 @@ __global__ __launch_bounds__(256) void adamw_coded(StepList<STEP_TENSORS> list, 
         }
         if constexpr (COPY) store_some<4>(held, k, n, pk[u]);
         store_some<4>(param, k, n, out);
-        const float sm = block_scale(m), sv = block_scale(root);
-        ((unsigned *)a.m)[(blk0 + u) * (BLOCK / 4) + lane] = quick_codes(m, sm, false);
-        ((unsigned *)a.v)[(blk0 + u) * (BLOCK / 4) + lane] = quick_codes(root, sv, true);
+        // the block's largest magnitudes; what is not finite is so in both moments, and its bits are above all others'
+        const unsigned high_m = lanes_max<64>(__float_as_uint(fmaxf(fmaxf(fabsf(m32[0]), fabsf(m32[1])), fmaxf(fabsf(m32[2]), fabsf(m32[3])))));
+        const unsigned high_v = lanes_max<64>(max(max(__float_as_uint(root32[0]), __float_as_uint(root32[1])), max(__float_as_uint(root32[2]), __float_as_uint(root32[3]))));
+        const bool lost = high_v >= 0x7f800000u || high_m >= 0x7f800000u;
+        const float sm = lost ? __builtin_nanf("") : scale_of(__uint_as_float(high_m));
+        const float sv = lost ? __builtin_nanf("") : scale_of(__uint_as_float(high_v));
+        ((unsigned *)a.m)[(blk0 + u) * (BLOCK / 4) + lane] = codes<false>(m, v, m32, sm);
+        ((unsigned *)a.v)[(blk0 + u) * (BLOCK / 4) + lane] = codes<true>(root, v, root32, sv);
         if (lane == 0) a.m_scale[blk0 + u] = sm, a.v_scale[blk0 + u] = sv;
     }
 }

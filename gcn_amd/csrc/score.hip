@@ -15,9 +15,10 @@ namespace ccnn {
 
 template <typename A>
 struct ScoreOut {
-    A *logp, *entropy, *top_logp, *stats;   // entropy and top_logp optional
+    A *logp, *entropy, *high, *log_sum;   // [rows] each: the rows of stats
+    A *top_logp;
     int *top_index;
-    int top;
+    int top, want_entropy;
 };
 
 struct Targets {
@@ -102,10 +103,10 @@ __device__ __forceinline__ void finish_row(const Sums<A> &a, long r, A given, lo
     const bool empty = a.m == ninf(A()) && a.s == A(0);
     const A l = empty ? ninf(A()) : logw(a.s), nan = nan_of(A());
     const bool bad = l != l;
-    o.stats[2 * r] = bad ? nan : a.m;
-    o.stats[2 * r + 1] = bad ? nan : l;
+    o.high[r] = bad ? nan : a.m;
+    o.log_sum[r] = bad ? nan : l;
     o.logp[r] = bad || y >= classes ? nan : y < 0 ? A(0) : empty ? ninf(A()) : (given - a.m) - l;
-    if (o.entropy) o.entropy[r] = bad ? nan : empty ? A(0) : l - a.t / a.s;
+    if (o.want_entropy) o.entropy[r] = bad ? nan : empty ? A(0) : l - a.t / a.s;
 }
 
 // ---------------------------------------------------------------------------- order of the alternatives
@@ -502,7 +503,7 @@ __global__ __launch_bounds__(256) void log_probs_join(const T *__restrict__ logi
 // ---------------------------------------------------------------------------- gradient
 template <typename A>
 struct GradIn {
-    const A *stats, *entropy, *d_logp, *d_entropy;
+    const A *entropy, *high, *log_sum, *d_logp, *d_entropy;
 };
 
 // What one row's elements have in common.
@@ -514,7 +515,7 @@ struct GradRow {
     __device__ GradRow(const GradIn<A> &in, const Targets &targets, long r, int classes)
     {
         y = targets.at(r);
-        m = in.stats[2 * r], l = in.stats[2 * r + 1];
+        m = in.high[r], l = in.log_sum[r];
         dl = in.d_logp && y >= 0 ? in.d_logp[r] : A(0);
         dh = in.d_entropy ? in.d_entropy[r] : A(0);
         h = in.d_entropy ? in.entropy[r] : A(0);
@@ -603,11 +604,12 @@ size_t slice_bytes(long rows, int classes, int top, int size)
 }
 
 template <typename T>
-int score_impl(const void *logits, long rows, int classes, long stride, Targets targets, int top, void *logp, void *entropy,
-               void *top_logp, int *top_index, void *stats, void *workspace, hipStream_t st)
+int score_impl(const void *logits, long rows, int classes, long stride, Targets targets, int top, int want_entropy,
+               void *stats, void *top_logp, int *top_index, void *workspace, hipStream_t st)
 {
     typedef Wide<T> A;
-    const ScoreOut<A> o = {(A *)logp, (A *)entropy, (A *)top_logp, (A *)stats, top_index, top};
+    A *s = (A *)stats;
+    const ScoreOut<A> o = {s, s + rows, s + 2 * rows, s + 3 * rows, (A *)top_logp, top_index, top, want_entropy};
     const T *x = (const T *)logits;
     if (classes <= SMALL_CLASSES) {
         typedef void (*Kern)(const T *, long, int, long, Targets, ScoreOut<A>);
@@ -636,10 +638,10 @@ int score_impl(const void *logits, long rows, int classes, long stride, Targets 
     // 65535 rows at most in a grid's second dimension
     for (long r0 = 0; r0 < rows; r0 += 65535) {
         const long nr = rows - r0 < 65535 ? rows - r0 : 65535;
-        ScoreOut<A> os = {o.logp + r0, o.entropy ? o.entropy + r0 : nullptr, top ? o.top_logp + r0 * top : nullptr,
-                          o.stats + 2 * r0, top ? o.top_index + r0 * top : nullptr, top};
+        const ScoreOut<A> os = {o.logp + r0, o.entropy + r0, o.high + r0, o.log_sum + r0, o.top_logp + r0 * top,
+                                o.top_index + r0 * top, top, want_entropy};
         const Targets ts = {(const char *)targets.p + r0 * targets.bytes, targets.bytes};
-        launch("log_probs_slice", entropy ? log_probs_slice<T, true> : log_probs_slice<T, false>,
+        launch("log_probs_slice", want_entropy ? log_probs_slice<T, true> : log_probs_slice<T, false>,
                dim3((unsigned)part.slices, (unsigned)nr), dim3(SLICE_THREADS), 0, st, x + r0 * stride, classes, stride, ts, os, part);
         CCNN_LAUNCH_CHECK();
     }
@@ -652,13 +654,14 @@ int score_impl(const void *logits, long rows, int classes, long stride, Targets 
 
 template <typename T>
 int score_grad_impl(const void *logits, long rows, int classes, long stride, Targets targets, const void *stats,
-                    const void *entropy, const void *d_logp, const void *d_entropy, void *d_logits, long d_stride,
+                    const void *d_logp, const void *d_entropy, void *d_logits, long d_stride,
                     hipStream_t st)
 {
     typedef Wide<T> A;
     const T *x = (const T *)logits;
     T *d = (T *)d_logits;
-    const GradIn<A> in = {(const A *)stats, (const A *)entropy, (const A *)d_logp, (const A *)d_entropy};
+    const A *s = (const A *)stats;
+    const GradIn<A> in = {s + rows, s + 2 * rows, s + 3 * rows, (const A *)d_logp, (const A *)d_entropy};
     if (classes <= SMALL_CLASSES) {
         const int lanes = classes <= 16 ? 16 : 64;
         const long per = 256 / lanes;
@@ -670,7 +673,7 @@ int score_grad_impl(const void *logits, long rows, int classes, long stride, Tar
     const long tile = 256 * GRAD_LOADS * (16 / sizeof(T));
     for (long r0 = 0; r0 < rows; r0 += 65535) {
         const long nr = rows - r0 < 65535 ? rows - r0 : 65535;
-        const GradIn<A> is = {in.stats + 2 * r0, in.entropy ? in.entropy + r0 : nullptr, in.d_logp ? in.d_logp + r0 : nullptr,
+        const GradIn<A> is = {in.entropy + r0, in.high + r0, in.log_sum + r0, in.d_logp ? in.d_logp + r0 : nullptr,
                               in.d_entropy ? in.d_entropy + r0 : nullptr};
         const Targets ts = {(const char *)targets.p + r0 * targets.bytes, targets.bytes};
         launch("log_probs_grad_wide", log_probs_grad_wide<T>, dim3((unsigned)((classes + tile - 1) / tile), (unsigned)nr),
@@ -701,39 +704,39 @@ size_t ccnn_log_probs_workspace_bytes(long rows, int classes, int top, int type)
 }
 
 int ccnn_log_probs(const void *logits, int type, long rows, int classes, long stride, const void *targets, int target_bytes,
-                   int top, void *logp, void *entropy, void *top_logp, int *top_index, void *stats, void *workspace,
+                   int top, int want_entropy, void *stats, void *top_logp, int *top_index, void *workspace,
                    size_t workspace_bytes, void *stream)
 {
     if (int e = score_args(logits, type, rows, classes, stride, targets, target_bytes)) return e;
     if (top < 0 || top > CCNN_MAX_TOP || top > classes) return CCNN_E_INVALID;
     if (rows == 0) return 0;
-    if (!logp || !stats || (top > 0 && (!top_logp || !top_index))) return CCNN_E_INVALID;
+    if (!stats || (top > 0 && (!top_logp || !top_index))) return CCNN_E_INVALID;
     const size_t need = ccnn_log_probs_workspace_bytes(rows, classes, top, type);
     if (workspace_bytes < need || (need && !workspace)) return CCNN_E_WORKSPACE;
     const Targets t = {targets, target_bytes};
     switch (type) {
-    case CCNN_TYPE_F32: return score_impl<float>(logits, rows, classes, stride, t, top, logp, entropy, top_logp, top_index, stats, workspace, (hipStream_t)stream);
-    case CCNN_TYPE_F64: return score_impl<double>(logits, rows, classes, stride, t, top, logp, entropy, top_logp, top_index, stats, workspace, (hipStream_t)stream);
-    case CCNN_TYPE_BF16: return score_impl<Bf16>(logits, rows, classes, stride, t, top, logp, entropy, top_logp, top_index, stats, workspace, (hipStream_t)stream);
-    default: return score_impl<F16>(logits, rows, classes, stride, t, top, logp, entropy, top_logp, top_index, stats, workspace, (hipStream_t)stream);
+    case CCNN_TYPE_F32: return score_impl<float>(logits, rows, classes, stride, t, top, want_entropy, stats, top_logp, top_index, workspace, (hipStream_t)stream);
+    case CCNN_TYPE_F64: return score_impl<double>(logits, rows, classes, stride, t, top, want_entropy, stats, top_logp, top_index, workspace, (hipStream_t)stream);
+    case CCNN_TYPE_BF16: return score_impl<Bf16>(logits, rows, classes, stride, t, top, want_entropy, stats, top_logp, top_index, workspace, (hipStream_t)stream);
+    default: return score_impl<F16>(logits, rows, classes, stride, t, top, want_entropy, stats, top_logp, top_index, workspace, (hipStream_t)stream);
     }
 }
 
 int ccnn_log_probs_grad(const void *logits, int type, long rows, int classes, long stride, const void *targets,
-                        int target_bytes, const void *stats, const void *entropy, const void *d_logp, const void *d_entropy,
+                        int target_bytes, const void *stats, const void *d_logp, const void *d_entropy,
                         void *d_logits, long d_stride, void *stream)
 {
     if (int e = score_args(logits, type, rows, classes, stride, targets, target_bytes)) return e;
     if (d_stride < classes) return CCNN_E_INVALID;
     if (rows == 0) return 0;
-    if (!stats || !d_logits || (!d_logp && !d_entropy) || (d_entropy && !entropy)) return CCNN_E_INVALID;
+    if (!stats || !d_logits || (!d_logp && !d_entropy)) return CCNN_E_INVALID;
     if (d_logits == logits && d_stride != stride) return CCNN_E_INVALID;
     const Targets t = {targets, target_bytes};
     switch (type) {
-    case CCNN_TYPE_F32: return score_grad_impl<float>(logits, rows, classes, stride, t, stats, entropy, d_logp, d_entropy, d_logits, d_stride, (hipStream_t)stream);
-    case CCNN_TYPE_F64: return score_grad_impl<double>(logits, rows, classes, stride, t, stats, entropy, d_logp, d_entropy, d_logits, d_stride, (hipStream_t)stream);
-    case CCNN_TYPE_BF16: return score_grad_impl<Bf16>(logits, rows, classes, stride, t, stats, entropy, d_logp, d_entropy, d_logits, d_stride, (hipStream_t)stream);
-    default: return score_grad_impl<F16>(logits, rows, classes, stride, t, stats, entropy, d_logp, d_entropy, d_logits, d_stride, (hipStream_t)stream);
+    case CCNN_TYPE_F32: return score_grad_impl<float>(logits, rows, classes, stride, t, stats, d_logp, d_entropy, d_logits, d_stride, (hipStream_t)stream);
+    case CCNN_TYPE_F64: return score_grad_impl<double>(logits, rows, classes, stride, t, stats, d_logp, d_entropy, d_logits, d_stride, (hipStream_t)stream);
+    case CCNN_TYPE_BF16: return score_grad_impl<Bf16>(logits, rows, classes, stride, t, stats, d_logp, d_entropy, d_logits, d_stride, (hipStream_t)stream);
+    default: return score_grad_impl<F16>(logits, rows, classes, stride, t, stats, d_logp, d_entropy, d_logits, d_stride, (hipStream_t)stream);
     }
 }
 

@@ -71,10 +71,9 @@ _SIG = {
     "ccnn_update_f32": (C.c_int, [_P, _P, C.c_float, C.c_int, C.c_int, _P]),
     "ccnn_update_adagrad_f64": (C.c_int, [_P, _P, _P, C.c_double, C.c_long, C.c_long, _P]),
     "ccnn_log_probs_workspace_bytes": (C.c_size_t, [C.c_long, C.c_int, C.c_int, C.c_int]),
-    "ccnn_log_probs": (C.c_int, [_P, C.c_int, C.c_long, C.c_int, C.c_long, _P, C.c_int, C.c_int, _P, _P, _P, _P, _P, _P,
+    "ccnn_log_probs": (C.c_int, [_P, C.c_int, C.c_long, C.c_int, C.c_long, _P, C.c_int, C.c_int, C.c_int, _P, _P, _P, _P,
                                  C.c_size_t, _P]),
-    "ccnn_log_probs_grad": (C.c_int, [_P, C.c_int, C.c_long, C.c_int, C.c_long, _P, C.c_int, _P, _P, _P, _P, _P, C.c_long,
-                                      _P]),
+    "ccnn_log_probs_grad": (C.c_int, [_P, C.c_int, C.c_long, C.c_int, C.c_long, _P, C.c_int, _P, _P, _P, _P, C.c_long, _P]),
     "ccnn_grad_norm_workspace_bytes": (C.c_size_t, [_P, C.c_int]),
     "ccnn_grad_norm": (C.c_int, [_P, _P, _P, C.c_int, C.c_double, _P, _P, C.c_size_t, _P]),
     "ccnn_adamw_step": (C.c_int, [_P, _P, _P, C.c_int, C.c_int, _P, _P, _P, _P, _P, _P, C.c_double, _P, C.c_double, C.c_double,

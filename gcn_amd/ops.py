@@ -368,11 +368,11 @@ _TYPES = {_F32: _l.TYPE_F32, _F64: _l.TYPE_F64, torch.bfloat16: _l.TYPE_BF16, to
 
 
 def _on_device(t, name, dtypes):
-    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+    if isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes:
+        return t
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError(f"{name} must be a CUDA tensor")
-    if t.dtype not in dtypes:
-        raise TypeError(f"{name} has dtype {t.dtype}, expected one of {', '.join(str(d) for d in dtypes)}")
-    return t
+    raise TypeError(f"{name} has dtype {t.dtype}, expected one of {', '.join(str(d) for d in dtypes)}")
 
 
 def _same_device(t, name, device):
@@ -420,12 +420,12 @@ def _enqueue(index, name, *args):
 
 
 class LogProbs(NamedTuple):
-    """What log_probs returns; fp64 for fp64 logits, else fp32."""
+    """What log_probs returns; fp64 for fp64 logits, else fp32.  logp and entropy are rows of stats."""
     logp: torch.Tensor                   # [rows] log probability of the target
     entropy: Optional[torch.Tensor]      # [rows] in nats
     top_logp: Optional[torch.Tensor]     # [rows, top] in falling order
     top_index: Optional[torch.Tensor]    # [rows, top] int32
-    stats: torch.Tensor                  # [rows, 2] largest logit, log sum exp(x - largest)
+    stats: torch.Tensor                  # [4, rows] logp, entropy, largest logit, log sum exp(x - largest)
 
 
 def _rows(t, name):
@@ -457,7 +457,7 @@ def log_probs(logits, targets, top=0, want_entropy=True):
     of their indices.  -> LogProbs.  A negative target gives 0, one of `classes` or more NaN.  -inf
     logits are classes that are not allowed; a row of nothing else has log probabilities of -inf and
     entropy 0, a row with a NaN or +inf has NaN everywhere and top_index -1."""
-    _on_device(logits, "logits", tuple(_TYPES))
+    _on_device(logits, "logits", _TYPES)
     rows, classes, stride = _rows(logits, "logits")
     dev = logits.device
     target_bytes = _target_bytes(targets, rows, dev)
@@ -465,24 +465,23 @@ def log_probs(logits, targets, top=0, want_entropy=True):
     if top < 0 or top > min(_l.MAX_TOP, classes):
         raise ValueError(f"top must be between 0 and {min(_l.MAX_TOP, classes)}, got {top}")
     wide, kind = _F64 if logits.dtype == _F64 else _F32, _TYPES[logits.dtype]
-    stats = torch.empty((rows, 2), dtype=wide, device=dev)
-    logp = torch.empty(rows, dtype=wide, device=dev)
-    entropy = torch.empty(rows, dtype=wide, device=dev) if want_entropy else None
+    stats = torch.empty((4, rows), dtype=wide, device=dev)
+    logp, entropy, _, _ = stats.unbind(0)
     top_logp = torch.empty((rows, top), dtype=wide, device=dev) if top else None
     top_index = torch.empty((rows, top), dtype=torch.int32, device=dev) if top else None
     if rows:
         nbytes = _l.load().ccnn_log_probs_workspace_bytes(rows, classes, top, kind)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         _enqueue(dev.index, "ccnn_log_probs", logits.data_ptr(), kind, rows, classes, stride, targets.data_ptr(), target_bytes,
-                 top, logp.data_ptr(), _at(entropy), _at(top_logp), _at(top_index), stats.data_ptr(), _at(ws), nbytes)
-    return LogProbs(logp, entropy, top_logp, top_index, stats)
+                 top, bool(want_entropy), stats.data_ptr(), _at(top_logp), _at(top_index), _at(ws), nbytes)
+    return LogProbs(logp, entropy if want_entropy else None, top_logp, top_index, stats)
 
 
 def log_probs_grad(logits, targets, scored, d_logp=None, d_entropy=None, out=None):
     """Gradient of sum(d_logp * logp) + sum(d_entropy * entropy) to the logits, from what log_probs
     returned for them.  d_logp / d_entropy: [rows] of the type of scored.logp, one of them at least.
     out: [rows, classes] of the logits' type (rows may be strided), the logits themselves allowed."""
-    _on_device(logits, "logits", tuple(_TYPES))
+    _on_device(logits, "logits", _TYPES)
     rows, classes, stride = _rows(logits, "logits")
     dev, wide = logits.device, _F64 if logits.dtype == _F64 else _F32
     target_bytes = _target_bytes(targets, rows, dev)
@@ -490,9 +489,8 @@ def log_probs_grad(logits, targets, scored, d_logp=None, d_entropy=None, out=Non
         raise ValueError("neither d_logp nor d_entropy given")
     if d_entropy is not None and scored.entropy is None:
         raise ValueError("d_entropy needs a log_probs call with want_entropy")
-    for t, name, n in ((scored.stats, "stats", 2 * rows), (d_logp, "d_logp", rows), (d_entropy, "d_entropy", rows),
-                       (scored.entropy, "entropy", rows)):
-        if t is not None:
+    for t, name, n in ((scored.stats, "stats", 4 * rows), (d_logp, "d_logp", rows), (d_entropy, "d_entropy", rows)):
+        if t is not None and not (isinstance(t, _T) and t.dtype == wide and t.device == dev and t.is_contiguous() and t.numel() == n):
             _req(t, wide, name, n)
             _same_device(t, name, dev)
     given, out_stride = out is not None, classes
@@ -511,7 +509,7 @@ def log_probs_grad(logits, targets, scored, d_logp=None, d_entropy=None, out=Non
                 and b < a + ((rows - 1) * stride + classes) * size:
             raise ValueError("out overlaps the logits without being them")
         _enqueue(dev.index, "ccnn_log_probs_grad", a, _TYPES[logits.dtype], rows, classes, stride, targets.data_ptr(),
-                 target_bytes, scored.stats.data_ptr(), _at(scored.entropy), _at(d_logp), _at(d_entropy), b, out_stride)
+                 target_bytes, scored.stats.data_ptr(), _at(d_logp), _at(d_entropy), b, out_stride)
     return out
 
 
@@ -571,7 +569,7 @@ class AdamW:
         first = block = 0
         spans = []
         for i, p in enumerate(self.params):
-            _on_device(p, f"parameter {i}", tuple(_TYPES))
+            _on_device(p, f"parameter {i}", _TYPES)
             _same_device(p, f"parameter {i}", self.device)
             if not p.is_contiguous():
                 raise ValueError(f"parameter {i} must be contiguous")

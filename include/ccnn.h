@@ -394,32 +394,31 @@ int ccnn_mbgd_step_dp_f64(ccnn_comm_t *comm, double *params, const double *cubes
  * alignment of an element).  All results are fp64 for fp64 logits and fp32 for the other types.
  *   targets   int32 or int64 (target_bytes 4 or 8), the class of each row counted from 0; negative =
  *             none given (logp 0); classes or more = an error the device reports as logp NaN
- *   logp      [rows] log softmax at the target
- *   entropy   [rows], optional: -sum p log p in nats
+ *   stats     [4][rows]: log softmax at the target; with want_entropy the entropy -sum p log p in nats;
+ *             the largest logit m; log sum exp(x - m)
  *   top_logp, top_index  [rows][top], top <= CCNN_MAX_TOP and <= classes: the most likely classes in
  *             falling order, equal logits in the order of their indices
- *   stats     [rows][2]: largest logit m and log sum exp(x - m), for ccnn_log_probs_grad
- * -inf is a class that is not allowed.  A row of nothing else has logp -inf, entropy 0, stats -inf and
- * top_logp -inf; a row with a NaN or +inf has NaN everywhere and top_index -1.
+ * -inf is a class that is not allowed.  A row of nothing else has entropy 0 and log probabilities,
+ * m and log sum of -inf; a row with a NaN or +inf has NaN everywhere and top_index -1.
  * workspace: ccnn_log_probs_workspace_bytes() bytes (a function of its arguments only; 0 = none
  * needed); it need not be initialised, and calls that share one must be ordered by one stream. */
 #define CCNN_MAX_TOP 64
 #define CCNN_MAX_LOGITS (1 << 30)
 size_t ccnn_log_probs_workspace_bytes(long rows, int classes, int top, int type);
 int ccnn_log_probs(const void *logits, int type, long rows, int classes, long stride,
-                   const void *targets, int target_bytes, int top, void *logp, void *entropy,
-                   void *top_logp, int *top_index, void *stats, void *workspace,
-                   size_t workspace_bytes, void *stream);
+                   const void *targets, int target_bytes, int top, int want_entropy, void *stats,
+                   void *top_logp, int *top_index, void *workspace, size_t workspace_bytes,
+                   void *stream);
 
-/* Gradient of sum(d_logp * logp) + sum(d_entropy * entropy) to the logits, from the stats (and, with
- * d_entropy, the entropy) that ccnn_log_probs left: d_logits rows x classes of the logits' type, row
+/* Gradient of sum(d_logp * logp) + sum(d_entropy * entropy) to the logits, from the stats that
+ * ccnn_log_probs left (with d_entropy: with want_entropy): d_logits rows x classes of the logits' type, row
  * stride d_stride.  d_logp or d_entropy may be NULL (no such term), not both.  A negative target has no
  * logp term; rows with nothing allowed get 0; rows with a target of `classes` or more, NaN.  d_logits
  * may be the logits themselves (same stride); it must not overlap them otherwise. */
 int ccnn_log_probs_grad(const void *logits, int type, long rows, int classes, long stride,
                         const void *targets, int target_bytes, const void *stats,
-                        const void *entropy, const void *d_logp, const void *d_entropy,
-                        void *d_logits, long d_stride, void *stream);
+                        const void *d_logp, const void *d_entropy, void *d_logits, long d_stride,
+                        void *stream);
 
 /* Norm of many gradient tensors taken as one vector, and the factor that limits it.
  * data, n, types: HOST arrays of `count` pointers, element counts (0 allowed) and CCNN_TYPE_*.

@@ -113,21 +113,21 @@ def test_scoring_and_optimiser_calls_refuse_bad_arguments():
     import ctypes as C
     lib, ok, nul = L.load(), C.c_void_p(64), C.c_void_p()
 
-    def score(x=ok, kind=1, rows=2, classes=5, stride=5, y=ok, yb=4, top=2, logp=ok, tl=ok, ti=ok, stats=ok):
-        return lib.ccnn_log_probs(x, kind, rows, classes, stride, y, yb, top, logp, nul, tl, ti, stats, nul, 0, nul)
+    def score(x=ok, kind=1, rows=2, classes=5, stride=5, y=ok, yb=4, top=2, tl=ok, ti=ok, stats=ok):
+        return lib.ccnn_log_probs(x, kind, rows, classes, stride, y, yb, top, 1, stats, tl, ti, nul, 0, nul)
 
     assert score(rows=0) == 0
     for bad in (dict(x=nul), dict(kind=0), dict(kind=5), dict(rows=-1), dict(classes=0), dict(stride=4), dict(y=nul),
-                dict(yb=2), dict(top=-1), dict(top=6), dict(logp=nul), dict(tl=nul), dict(ti=nul), dict(stats=nul)):
+                dict(yb=2), dict(top=-1), dict(top=6), dict(tl=nul), dict(ti=nul), dict(stats=nul)):
         assert score(**bad) == -1, bad
     assert score(rows=1 << 31) == -3 and score(classes=(1 << 30) + 1, stride=1 << 40) == -3
     assert score(classes=100, stride=100, top=65) == -1
 
-    def grad(x=ok, kind=1, classes=5, stride=5, stats=ok, h=ok, dl=ok, dh=ok, out=C.c_void_p(4096), ostride=5, rows=2):
-        return lib.ccnn_log_probs_grad(x, kind, rows, classes, stride, ok, 4, stats, h, dl, dh, out, ostride, nul)
+    def grad(x=ok, kind=1, classes=5, stride=5, stats=ok, dl=ok, dh=ok, out=C.c_void_p(4096), ostride=5, rows=2):
+        return lib.ccnn_log_probs_grad(x, kind, rows, classes, stride, ok, 4, stats, dl, dh, out, ostride, nul)
 
     assert grad(rows=0) == 0
-    for bad in (dict(x=nul), dict(kind=9), dict(stats=nul), dict(h=nul), dict(dl=nul, dh=nul), dict(out=nul), dict(ostride=4),
+    for bad in (dict(x=nul), dict(kind=9), dict(stats=nul), dict(dl=nul, dh=nul), dict(out=nul), dict(ostride=4),
                 dict(out=ok, ostride=6)):
         assert grad(**bad) == -1, bad
 

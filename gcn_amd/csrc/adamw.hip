@@ -147,26 +147,41 @@ struct StepList {
 struct StepArgs {
     void *m, *v;
     float *m_scale, *v_scale, *master;
-    const double *clock;
-    double beta1, beta2, eps;
+    double *clock;
+    double beta1, beta2, eps, lr;
+    const double *lr_device, *clip;
 };
 
-// clock: t, beta1^t, beta2^t | lr, lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t), gradient factor (NaN: no step)
-__global__ void adamw_clock(double *clock, double lr, const double *lr_device, double beta1, double beta2, const double *clip)
-{
-    const double scale = clip ? clip[1] : 1.0;
-    clock[6] = scale;
-    if (!(fabs(scale) < __builtin_huge_val())) {
-        clock[6] = __builtin_nan("");
-        return;
+// What a step takes from the clock, for all its elements alike.
+struct Tick {
+    double t, beta1_t, beta2_t, lr, rate, root, scale;   // steps, powers; lr, lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t), gradient factor
+    bool skip;
+    __device__ explicit Tick(const StepArgs &a)
+    {
+        scale = a.clip ? a.clip[1] : 1.0;
+        lr = a.lr_device ? *a.lr_device : a.lr;
+        t = a.clock[0] + 1;
+        beta1_t = a.clock[1] * a.beta1;
+        beta2_t = a.clock[2] * a.beta2;
+        rate = lr / (1 - beta1_t);
+        root = 1 / sqrt(1 - beta2_t);
+        skip = !(fabs(scale) < __builtin_huge_val());
     }
-    const double rate = lr_device ? *lr_device : lr;
-    clock[0] += 1;
-    clock[1] *= beta1;
-    clock[2] *= beta2;
-    clock[3] = rate;
-    clock[4] = rate / (1 - clock[1]);
-    clock[5] = 1 / sqrt(1 - clock[2]);
+    __device__ void keep(double *clock) const
+    {
+        clock[0] = t, clock[1] = beta1_t, clock[2] = beta2_t;
+    }
+};
+
+// clock: t, beta1^t, beta2^t | lr, lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t), gradient factor (NaN: no step) | arrivals
+__global__ void adamw_clock(StepArgs a)
+{
+    const Tick tick(a);
+    if (!tick.skip) tick.keep(a.clock);
+    a.clock[3] = tick.lr;
+    a.clock[4] = tick.rate;
+    a.clock[5] = tick.root;
+    a.clock[6] = tick.skip ? __builtin_nan("") : tick.scale;
 }
 
 template <typename A>
@@ -178,7 +193,26 @@ struct Rates {
           skip(!(a.clock[6] == a.clock[6]))
     {
     }
+    __device__ Rates(const StepArgs &a, const Tick &tick, double decay)
+        : scale((A)tick.scale), lr_decay((A)(tick.lr * decay)), rate((A)tick.rate), root((A)tick.root), eps((A)a.eps),
+          skip(tick.skip)
+    {
+    }
 };
+
+// A launch that is the whole step moves the clock itself: every workgroup has read it when it arrives here, the last
+// to arrive writes it and leaves the count at 0.
+__device__ __forceinline__ void arrive(const StepArgs &a, const Tick &tick)
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");     // the reads above are done
+    if (threadIdx.x == 0) {
+        unsigned *arrivals = reinterpret_cast<unsigned *>(a.clock + CCNN_ADAMW_CLOCK - 1);
+        if (atomicAdd(arrivals, 1u) == gridDim.x - 1) {
+            tick.keep(a.clock);
+            *arrivals = 0;
+        }
+    }
+}
 
 template <typename A>
 __device__ __forceinline__ A stepped(A p, A m, A v_root, const Rates<A> &r)
@@ -215,7 +249,14 @@ __global__ __launch_bounds__(WIDE_THREADS) void adamw_wide(StepList<U == 1 ? FEW
         vk[u] = load_some<W>(v, k, n);
         pk[u] = load_some<W>(held, k, n);
     }
-    const Rates<A> r(a, list.decay[i]);
+    std::conditional_t<U == 1, Tick, int> tick = [&] {
+        if constexpr (U == 1) return Tick(a);
+        else return 0;
+    }();
+    const Rates<A> r = [&] {
+        if constexpr (U == 1) return Rates<A>(a, tick, list.decay[i]);
+        else return Rates<A>(a, list.decay[i]);
+    }();
     if (r.skip) return;
     const A b1 = (A)(1 - a.beta1), b2 = (A)(1 - a.beta2);
 #pragma unroll
@@ -235,6 +276,7 @@ __global__ __launch_bounds__(WIDE_THREADS) void adamw_wide(StepList<U == 1 ? FEW
         if constexpr (COPY) store_some<W>(held, k, n, pk[u]);
         store_some<W>(param, k, n, out);
     }
+    if constexpr (U == 1) arrive(a, tick);
 }
 
 // e4m3: values 2^-9 apart below 2^-6, then eight to each power of two up to 448.
@@ -425,8 +467,9 @@ __global__ __launch_bounds__(256) void adamw_decode(StepList<STEP_TENSORS> list,
 }
 
 // ---------------------------------------------------------------------------- host
-// Below so many elements a step of few tensors takes one pack a thread and a short argument block: it is all latency
-// (47 k fp32 parameters: 5.3 us of the device instead of 9.3 in packs of four).
+// Below so many elements a step of few tensors of one type is one launch, with one pack a thread, a short argument block
+// and the clock moved by its last workgroup: it is all latency (47 k fp32 parameters: 5.3 us of the device instead
+// of 9.3 in packs of four, and another launch costs the host 3).
 constexpr long WIDE_SMALL = 1 << 20;
 // Hands tensors [0, count) that `take` accepts to `go`, a list at a time, with their chunks counted.
 template <typename List, typename Take, typename Go>
@@ -558,9 +601,7 @@ int ccnn_adamw_step(const ccnn_adamw_tensor_t *tensors, const void *const *grads
     if (wide && (other || moment_bits == 8)) return CCNN_E_INVALID;
     if (total > 0 && (!m || !v || (moment_bits == 8 && (!m_scale || !v_scale)))) return CCNN_E_INVALID;
     hipStream_t st = (hipStream_t)stream;
-    launch("adamw_clock", adamw_clock, dim3(1), dim3(1), 0, st, clock, lr, lr_device, beta1, beta2, clip);
-    CCNN_LAUNCH_CHECK();
-    const StepArgs args = {m, v, m_scale, v_scale, master, clock, beta1, beta2, eps};
+    const StepArgs args = {m, v, m_scale, v_scale, master, clock, beta1, beta2, eps, lr, lr_device, clip};
     typedef StepList<FEW_TENSORS> Few;
     typedef StepList<STEP_TENSORS> Many;
     const struct {
@@ -576,7 +617,13 @@ int ccnn_adamw_step(const ccnn_adamw_tensor_t *tensors, const void *const *grads
         {CCNN_TYPE_F16, CCNN_TYPE_F16, adamw_wide<F16, F16, 1>, adamw_wide<F16, F16, 4>, adamw_coded<F16, F16>},
         {CCNN_TYPE_F16, CCNN_TYPE_F32, adamw_wide<F16, float, 1>, adamw_wide<F16, float, 4>, adamw_coded<F16, float>},
     };
-    const bool small = moment_bits == 32 && total < WIDE_SMALL && count <= FEW_TENSORS;
+    bool alike = true;
+    for (int i = 1; i < count; i++) alike &= tensors[i].type == tensors[0].type && grad_types[i] == grad_types[0];
+    const bool small = moment_bits == 32 && total > 0 && total < WIDE_SMALL && count <= FEW_TENSORS && alike;
+    if (!small) {
+        launch("adamw_clock", adamw_clock, dim3(1), dim3(1), 0, st, args);
+        CCNN_LAUNCH_CHECK();
+    }
     for (const auto &kind : kinds) {
         auto take = [&](auto &list, int i) -> long {
             const ccnn_adamw_tensor_t &t = tensors[i];

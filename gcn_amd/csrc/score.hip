@@ -19,6 +19,10 @@ struct ScoreOut {
     A *top_logp;
     int *top_index;
     int top, want_entropy;
+    ScoreOut from(long r) const
+    {
+        return {logp + r, entropy + r, high + r, log_sum + r, top_logp + r * top, top_index + r * top, top, want_entropy};
+    }
 };
 
 struct Targets {
@@ -28,6 +32,7 @@ struct Targets {
     {
         return bytes == 8 ? (long)((const long long *)p)[r] : (long)((const int *)p)[r];
     }
+    Targets from(long r) const { return {(const char *)p + r * bytes, bytes}; }
 };
 
 // Running softmax sums of part of a row: maximum m, s = sum e^(x-m), t = sum e^(x-m)(x-m).
@@ -504,6 +509,10 @@ __global__ __launch_bounds__(256) void log_probs_join(const T *__restrict__ logi
 template <typename A>
 struct GradIn {
     const A *entropy, *high, *log_sum, *d_logp, *d_entropy;
+    GradIn from(long r) const
+    {
+        return {entropy + r, high + r, log_sum + r, d_logp ? d_logp + r : nullptr, d_entropy ? d_entropy + r : nullptr};
+    }
 };
 
 // What one row's elements have in common.
@@ -578,6 +587,7 @@ __global__ __launch_bounds__(256) void log_probs_grad_wide(const T *logits, int 
 
 // ---------------------------------------------------------------------------- host
 constexpr int SMALL_CLASSES = 1024;
+constexpr long ROWS_AT_ONCE = 1 << 24;   // of few classes: 64 threads each stay below the 2^32 of a launch
 
 // Slices of a row: one up to UNSPLIT classes, where a workgroup ends with the row before a second launch could join
 // slices (one row of 50000 bf16 with 20 alternatives: 10.3 us whole, 12.0 in slices; of 128000: 17.0 and 12.7;
@@ -628,9 +638,12 @@ int score_impl(const void *logits, long rows, int classes, long stride, Targets 
                           : classes <= 256 ? (many ? log_probs_small<T, 16, 16> : log_probs_small<T, 64, 4>)
                                            : log_probs_small<T, 64, 16>;
         const long per = 256 / group;
-        launch("log_probs_small", kern, dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, st, x, rows, classes, stride,
-               targets, o);
-        CCNN_LAUNCH_CHECK();
+        for (long r0 = 0; r0 < rows; r0 += ROWS_AT_ONCE) {
+            const long nr = rows - r0 < ROWS_AT_ONCE ? rows - r0 : ROWS_AT_ONCE;
+            launch("log_probs_small", kern, dim3((unsigned)((nr + per - 1) / per)), dim3(256), 0, st, x + r0 * stride, nr,
+                   classes, stride, targets.from(r0), o.from(r0));
+            CCNN_LAUNCH_CHECK();
+        }
         return 0;
     }
     SliceOut<A> part = {};
@@ -643,11 +656,9 @@ int score_impl(const void *logits, long rows, int classes, long stride, Targets 
     // 65535 rows at most in a grid's second dimension
     for (long r0 = 0; r0 < rows; r0 += 65535) {
         const long nr = rows - r0 < 65535 ? rows - r0 : 65535;
-        const ScoreOut<A> os = {o.logp + r0, o.entropy + r0, o.high + r0, o.log_sum + r0, o.top_logp + r0 * top,
-                                o.top_index + r0 * top, top, want_entropy};
-        const Targets ts = {(const char *)targets.p + r0 * targets.bytes, targets.bytes};
         launch("log_probs_slice", want_entropy ? log_probs_slice<T, true> : log_probs_slice<T, false>,
-               dim3((unsigned)part.slices, (unsigned)nr), dim3(SLICE_THREADS), 0, st, x + r0 * stride, classes, stride, ts, os, part);
+               dim3((unsigned)part.slices, (unsigned)nr), dim3(SLICE_THREADS), 0, st, x + r0 * stride, classes, stride,
+               targets.from(r0), o.from(r0), part);
         CCNN_LAUNCH_CHECK();
     }
     if (part.slices > 1) {
@@ -670,19 +681,19 @@ int score_grad_impl(const void *logits, long rows, int classes, long stride, Tar
     if (classes <= SMALL_CLASSES) {
         const int lanes = classes <= 16 ? 16 : 64;
         const long per = 256 / lanes;
-        launch("log_probs_grad_small", log_probs_grad_small<T>, dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, st, x,
-               rows, classes, stride, targets, in, d, d_stride, lanes);
-        CCNN_LAUNCH_CHECK();
+        for (long r0 = 0; r0 < rows; r0 += ROWS_AT_ONCE) {
+            const long nr = rows - r0 < ROWS_AT_ONCE ? rows - r0 : ROWS_AT_ONCE;
+            launch("log_probs_grad_small", log_probs_grad_small<T>, dim3((unsigned)((nr + per - 1) / per)), dim3(256), 0, st,
+                   x + r0 * stride, nr, classes, stride, targets.from(r0), in.from(r0), d + r0 * d_stride, d_stride, lanes);
+            CCNN_LAUNCH_CHECK();
+        }
         return 0;
     }
     const long tile = 256 * GRAD_LOADS * (16 / sizeof(T));
     for (long r0 = 0; r0 < rows; r0 += 65535) {
         const long nr = rows - r0 < 65535 ? rows - r0 : 65535;
-        const GradIn<A> is = {in.entropy + r0, in.high + r0, in.log_sum + r0, in.d_logp ? in.d_logp + r0 : nullptr,
-                              in.d_entropy ? in.d_entropy + r0 : nullptr};
-        const Targets ts = {(const char *)targets.p + r0 * targets.bytes, targets.bytes};
         launch("log_probs_grad_wide", log_probs_grad_wide<T>, dim3((unsigned)((classes + tile - 1) / tile), (unsigned)nr),
-               dim3(256), 0, st, x + r0 * stride, classes, stride, ts, is, d + r0 * d_stride, d_stride);
+               dim3(256), 0, st, x + r0 * stride, classes, stride, targets.from(r0), in.from(r0), d + r0 * d_stride, d_stride);
         CCNN_LAUNCH_CHECK();
     }
     return 0;

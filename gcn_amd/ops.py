@@ -403,13 +403,16 @@ def _one_device(tensors, name, dtypes):
     raise TypeError(f"{name} list cannot be used")
 
 
+_CALLS = {}
 _raw_stream, _current = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
 def _enqueue(index, name, *args):
     """Calls a library function with device `index` current and that device's current stream as its last
     argument.  Addresses go as plain numbers: the host side of a small call is most of it."""
-    fn = getattr(_l.load(), name)
+    fn = _CALLS.get(name)
+    if fn is None:
+        fn = _CALLS[name] = getattr(_l.load(), name)
     if index == _current():
         rc = fn(*args, _raw_stream(index))
     else:
@@ -443,18 +446,22 @@ def _rows(t, name):
 
 
 def _target_bytes(targets, rows, device):
-    _on_device(targets, "targets", (torch.int32, torch.int64))
-    _same_device(targets, "targets", device)
-    if targets.dim() != 1 or targets.shape[0] != rows or (rows > 1 and targets.stride(0) != 1):
+    if not (isinstance(targets, _T) and targets.dtype in _TARGET_BYTES and targets.device == device and targets.shape == (rows,)
+            and targets.is_contiguous()):
+        _on_device(targets, "targets", _TARGET_BYTES)
+        _same_device(targets, "targets", device)
         raise ValueError(f"targets must be contiguous [{rows}], got {list(targets.shape)}")
-    return 4 if targets.dtype == torch.int32 else 8
+    return _TARGET_BYTES[targets.dtype]
+
+
+_TARGET_BYTES = {torch.int32: 4, torch.int64: 8}
 
 
 def log_probs(logits, targets, top=0, want_entropy=True):
     """Scores each row of logits [rows, classes] (fp32, fp64, bf16 or fp16; rows may be strided) at its
     target, int32 or int64 [rows], counted from 0: log probability of the target, entropy of the row,
     the `top` (at most 64) most likely classes with their log probabilities, equal logits in the order
-    of their indices.  -> LogProbs.  A negative target gives 0, one of `classes` or more NaN.  -inf
+    of their indices.  -> LogProbs; no autograd history, see log_probs_grad.  A negative target gives 0, one of `classes` or more NaN.  -inf
     logits are classes that are not allowed; a row of nothing else has log probabilities of -inf and
     entropy 0, a row with a NaN or +inf has NaN everywhere and top_index -1."""
     _on_device(logits, "logits", _TYPES)
@@ -462,16 +469,20 @@ def log_probs(logits, targets, top=0, want_entropy=True):
     dev = logits.device
     target_bytes = _target_bytes(targets, rows, dev)
     top = int(top)
-    if top < 0 or top > min(_l.MAX_TOP, classes):
+    if top and not 0 < top <= min(_l.MAX_TOP, classes):
         raise ValueError(f"top must be between 0 and {min(_l.MAX_TOP, classes)}, got {top}")
-    wide, kind = _F64 if logits.dtype == _F64 else _F32, _TYPES[logits.dtype]
+    kind = _TYPES[logits.dtype]
+    wide = _F64 if kind == _l.TYPE_F64 else _F32
     stats = torch.empty((4, rows), dtype=wide, device=dev)
     logp, entropy, _, _ = stats.unbind(0)
-    top_logp = torch.empty((rows, top), dtype=wide, device=dev) if top else None
-    top_index = torch.empty((rows, top), dtype=torch.int32, device=dev) if top else None
+    top_logp = top_index = ws = None
+    if top:
+        top_logp = torch.empty((rows, top), dtype=wide, device=dev)
+        top_index = torch.empty((rows, top), dtype=torch.int32, device=dev)
     if rows:
         nbytes = _l.load().ccnn_log_probs_workspace_bytes(rows, classes, top, kind)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        if nbytes:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         _enqueue(dev.index, "ccnn_log_probs", logits.data_ptr(), kind, rows, classes, stride, targets.data_ptr(), target_bytes,
                  top, bool(want_entropy), stats.data_ptr(), _at(top_logp), _at(top_index), _at(ws), nbytes)
     return LogProbs(logp, entropy if want_entropy else None, top_logp, top_index, stats)
@@ -589,6 +600,7 @@ class AdamW:
         self.numel, self.blocks = first, block
         # what each gradient is held against, and the types' table for the usual case that they are the parameters'
         self._numels, self._dtypes = [p.numel() for p in self.params], [p.dtype for p in self.params]
+        self._places = [p.data_ptr() for p in self.params]
         self._kinds = (C.c_int * n)(*[t.type for t in self._table])
         wide = _F64 if self.params[0].dtype == _F64 else _F32
         if state_bits == 32:
@@ -619,6 +631,8 @@ class AdamW:
         count = len(self.params)
         if len(grads) != count:
             raise ValueError(f"{len(grads)} gradients for {count} parameters")
+        if list(map(_T.data_ptr, self.params)) != self._places:
+            raise ValueError("a parameter's memory is not what it was when the optimiser was made")
         if _one_device(grads, "gradient", _TYPES) != dev:
             raise ValueError(f"gradients are on {grads[0].device}, the parameters on {dev}")
         if list(map(_T.numel, grads)) != self._numels:

@@ -446,7 +446,7 @@ int ccnn_grad_norm(const void *const *data, const long *n, const int *types, int
  * least the smallest code, so a denominator never becomes 0 by rounding.  A block's bytes behind the tensor's end are left 0.  A gradient that is not finite makes
  * its whole block NaN (with 32 bits: its element).
  * clock [CCNN_ADAMW_CLOCK] device doubles: clock[0] = t, steps taken so far, clock[1] = beta1^t,
- * clock[2] = beta2^t (initially 0, 1, 1); the call advances them on the device, so a captured step counts
+ * clock[2] = beta2^t (initially 0, 1, 1, and the rest 0); the call advances them on the device, so a captured step counts
  * on when it is replayed.  lr_device, if not NULL, is read instead of lr.  clip, if not NULL, is
  * ccnn_grad_norm's out: when clip[1] is not finite nothing is changed, t included. */
 #define CCNN_MOMENT_BLOCK 256

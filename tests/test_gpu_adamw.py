@@ -350,3 +350,8 @@ def test_refused():
         with pytest.raises(err):
             call()
     assert opt.step_count == 0 and not p.any()
+    moved = torch.zeros(10, device="cuda")
+    other = ops.AdamW([moved])
+    moved.data = torch.zeros(10, device="cuda")           # the memory the optimiser knew is gone
+    with pytest.raises(ValueError):
+        other.step([g])

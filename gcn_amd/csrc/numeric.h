@@ -96,6 +96,7 @@ struct Pack {
     T v[N];
 };
 template <int BYTES> struct Words;
+template <> struct Words<4> { typedef unsigned type __attribute__((aligned(2))); };
 template <> struct Words<8> { typedef unsigned type __attribute__((ext_vector_type(2), aligned(2))); };
 template <> struct Words<16> { typedef unsigned type __attribute__((ext_vector_type(4), aligned(2))); };
 template <> struct Words<32> { typedef unsigned type __attribute__((ext_vector_type(8), aligned(2))); };

@@ -152,26 +152,29 @@ __device__ __forceinline__ void put_top(const ScoreOut<A> &o, long r, int place,
 }
 
 // ---------------------------------------------------------------------------- up to 1024 classes
-// G lanes to a row, E elements to a lane, all of them in registers.  The sums are one pass over the
-// registers.  Alternatives, with a wave to a row: value by value, the largest left, all elements that equal it
-// placed in the order of their indices (element e of lane i is class e G + i) and struck out.  With several rows
-// to a wave: one by one, the lane whose best was taken looking for its next - what one row needs all rows of the
-// wave wait for, and equal values of one row would be looked for in all (20000 x 1000 bf16, 20 alternatives:
-// 54 us the first way, 101 the second; 207400 x 13 fp32, 3 alternatives: 11.7 and 8.7).
+// G lanes to a row, E elements to a lane, all of them in registers, loaded W at once: element e of lane i is class
+// (e / W) G W + i W + e % W.  The sums are one pass over the registers.  Alternatives, with a wave to a row: value
+// by value, the largest left, all elements that equal it placed in the order of their classes and struck out.
+// With several rows to a wave: one by one, the lane whose best was taken looking for its next - what one row needs
+// all rows of the wave wait for, and equal values of one row would be looked for in all (20000 x 1000 bf16, 20
+// alternatives: 54 us the first way, 101 the second; 207400 x 13 fp32, 3 alternatives: 11.7 and 8.7).
 template <typename T, int G, int E>
 __global__ __launch_bounds__(256) void log_probs_small(const T *__restrict__ logits, long rows, int classes, long stride,
                                                        Targets targets, ScoreOut<Wide<T>> o)
 {
     typedef Wide<T> A;
+    constexpr int FULL = 16 / sizeof(T), W = E < FULL ? E : FULL;
     const int lane = threadIdx.x % G;
     const long r = (long)blockIdx.x * (256 / G) + threadIdx.x / G;
     if (r >= rows) return;               // whole groups leave: the others' exchanges stay among themselves
     const T *row = logits + r * stride;
+    auto place_of = [&](int e) { return e / W * (G * W) + lane * W + e % W; };
     A x[E];
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-        const int j = e * G + lane;
-        x[e] = j < classes ? (A)widen(row[j]) : ninf(A());
+    for (int c = 0; c < E; c += W) {
+        const Pack<T, W> p = load_some<W>(row, place_of(c), classes);
+#pragma unroll
+        for (int e = 0; e < W; e++) x[c + e] = place_of(c + e) < classes ? (A)widen(p.v[e]) : ninf(A());
     }
     const long y = targets.at(r);
     const A given = lane == 0 && y >= 0 && y < classes ? (A)widen(row[y]) : A(0);
@@ -199,21 +202,28 @@ __global__ __launch_bounds__(256) void log_probs_small(const T *__restrict__ log
         const A gone = nan_of(A());             // not equal to, and passed over by the maximum of, anything
 #pragma unroll
         for (int e = 0; e < E; e++)
-            if (e * G + lane >= classes) x[e] = gone;
+            if (place_of(e) >= classes) x[e] = gone;
         for (int k = 0; k < o.top;) {
             const A high = over_lanes<G>(max_of(x), [](A a, A b) { return max_of(a, b); });
 #pragma unroll
-            for (int e = 0; e < E; e++) {
-                const bool here = x[e] == high;
-                const unsigned long long all = __ballot(here);
-                if (all) {
-                    const int place = k + __popcll(all & ((1ull << lane) - 1));
-                    if (here) {
-                        if (place < o.top) put_top(o, r, place, high, e * G + lane, m, l);
-                        x[e] = gone;
-                    }
-                    k += __popcll(all);
+            for (int c = 0; c < E; c += W) {
+                unsigned long long all[W], any = 0;
+#pragma unroll
+                for (int e = 0; e < W; e++) any |= all[e] = __ballot(x[c + e] == high);
+                if (!any) continue;
+                int place = k;
+#pragma unroll
+                for (int e = 0; e < W; e++) {
+                    place += __popcll(all[e] & ((1ull << lane) - 1));     // in the lanes before
+                    k += __popcll(all[e]);
                 }
+#pragma unroll
+                for (int e = 0; e < W; e++)
+                    if (x[c + e] == high) {
+                        if (place < o.top) put_top(o, r, place, high, place_of(c + e), m, l);
+                        place++;
+                        x[c + e] = gone;
+                    }
             }
         }
     } else {
@@ -223,15 +233,15 @@ __global__ __launch_bounds__(256) void log_probs_small(const T *__restrict__ log
             int at = -1;
 #pragma unroll
             for (int e = 0; e < E; e++)
-                if (!(taken >> e & 1) && e * G + lane < classes && (at < 0 || x[e] > v)) v = x[e], at = e;
-            return at < 0 ? Key<A>(0) : key_of(v, at * G + lane);
+                if (!(taken >> e & 1) && place_of(e) < classes && (at < 0 || x[e] > v)) v = x[e], at = e;
+            return at < 0 ? Key<A>(0) : key_of(v, place_of(at));
         };
         Key<A> best = next();
         for (int k = 0; k < o.top; k++) {
             const Key<A> high = lanes_max<G>(best);
             if (lane == 0) put_top(o, r, k, key_value(high), (int)key_index(high), m, l);
             if (best == high && k + 1 < o.top) {
-                taken |= 1u << (key_index(high) / G);
+                taken |= 1u << (key_index(high) / (G * W) * W + key_index(high) % W);
                 best = next();
             }
         }
@@ -243,7 +253,7 @@ __global__ __launch_bounds__(256) void log_probs_small(const T *__restrict__ log
 // largest element with the load it came in.  The k-th largest of 64 groups' largest is a bar that the
 // top k elements all reach and few others do; only the threads that hold such an element look at their part
 // again, what reaches the bar is collected in LDS and put in order by counting.
-constexpr int SLICE_THREADS = 512;
+constexpr int SLICE_THREADS = 512;   // or 64: see wave_rows
 constexpr int CANDIDATES = 1024;
 
 template <typename A>
@@ -254,13 +264,14 @@ struct SliceOut {
     long length;      // elements of a slice (the last may be shorter), a multiple of the load width
 };
 
-template <typename A>
+template <typename A, int NT>
 struct SliceLds {
-    Key<A> key[SLICE_THREADS];
-    Key<A> found[CANDIDATES];
-    A m[SLICE_THREADS / 64], s[SLICE_THREADS / 64], t[SLICE_THREADS / 64];
+    static constexpr int MOST = NT * 2;    // candidates
+    Key<A> key[NT];
+    Key<A> found[MOST];
+    A m[NT / 64], s[NT / 64], t[NT / 64];
     Key<A> bar;
-    int owners[SLICE_THREADS];
+    int owners[NT];
     int n_owners, n_found;
 };
 
@@ -315,15 +326,15 @@ __device__ __forceinline__ void in_rounds(Get get, int n, int top, K *lds, Put p
     }
 }
 
-template <typename T, bool ENTROPY>
-__global__ __launch_bounds__(SLICE_THREADS) void log_probs_slice(const T *__restrict__ logits, int classes, long stride,
-                                                                 Targets targets, ScoreOut<Wide<T>> o, SliceOut<Wide<T>> part)
+template <typename T, bool ENTROPY, int NT>
+__global__ __launch_bounds__(NT) void log_probs_slice(const T *__restrict__ logits, int classes, long stride, Targets targets,
+                                                      ScoreOut<Wide<T>> o, SliceOut<Wide<T>> part)
 {
     typedef Wide<T> A;
-    constexpr int W = 16 / sizeof(T), NT = SLICE_THREADS, U = 4;
-    __shared__ SliceLds<A> lds;
-    const long r = blockIdx.y;
-    const int slice = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    constexpr int W = 16 / sizeof(T), U = 4, MOST = SliceLds<A, NT>::MOST;
+    __shared__ SliceLds<A, NT> lds;
+    const long r = blockIdx.x / part.slices;
+    const int slice = blockIdx.x % part.slices, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const long begin = slice * part.length;
     const int n = (int)min((long)classes - begin, part.length);
     const T *row = logits + r * stride + begin;
@@ -440,12 +451,12 @@ __global__ __launch_bounds__(SLICE_THREADS) void log_probs_slice(const T *__rest
             const A x = widen(p.v[e]);
             if (e < count && key_of(x, at) >= bar) {
                 const int place = atomicAdd(&lds.n_found, 1);
-                if (place < CANDIDATES) lds.found[place] = key_of(x, (unsigned)(begin + (long)at * W + e));
+                if (place < MOST) lds.found[place] = key_of(x, (unsigned)(begin + (long)at * W + e));
             }
         }
     }
     __syncthreads();
-    if (lds.n_found <= CANDIDATES) {
+    if (lds.n_found <= MOST) {
         in_order(lds.found, lds.n_found, o.top, put);
         if (part.sums)     // a last slice shorter than the list: nothing behind its elements
             for (int place = lds.n_found + tid; place < o.top; place += NT) put(place, Key<A>(0));
@@ -540,17 +551,22 @@ struct GradRow {
     }
 };
 
+// A thread to each 16 bytes of a row, rows one after the other.
 template <typename T>
-__global__ __launch_bounds__(256) void log_probs_grad_small(const T *logits, long rows, int classes, long stride,
+__global__ __launch_bounds__(256) void log_probs_grad_packs(const T *logits, unsigned rows, int classes, long stride,
                                                             Targets targets, GradIn<Wide<T>> in, T *d_logits, long d_stride,
-                                                            int lanes)
+                                                            unsigned packs)
 {
     typedef Wide<T> A;
-    const long r = ((long)blockIdx.x * 256 + threadIdx.x) / lanes;
+    constexpr int W = 16 / sizeof(T);
+    const unsigned q = blockIdx.x * 256 + threadIdx.x, r = q / packs;
+    const int j = (int)(q - r * packs) * W;
     if (r >= rows) return;
+    Pack<T, W> p = load_some<W>(logits + r * stride, j, classes);
     const GradRow<A> row(in, targets, r, classes);
-    for (int j = threadIdx.x % lanes; j < classes; j += lanes)
-        narrow(row.at((A)widen(logits[r * stride + j]), j), d_logits[r * d_stride + j]);
+#pragma unroll
+    for (int e = 0; e < W; e++) narrow(row.at((A)widen(p.v[e]), j + e), p.v[e]);
+    store_some<W>(d_logits + r * d_stride, j, classes, p);
 }
 
 constexpr int GRAD_LOADS = 2;   // 1 and 4 are a few per cent slower over 1 GB of logits
@@ -587,7 +603,14 @@ __global__ __launch_bounds__(256) void log_probs_grad_wide(const T *logits, int 
 
 // ---------------------------------------------------------------------------- host
 constexpr int SMALL_CLASSES = 1024;
-constexpr long ROWS_AT_ONCE = 1 << 24;   // of few classes: 64 threads each stay below the 2^32 of a launch
+constexpr int PACKED_CLASSES = 1024;    // gradient: 16 bytes a thread up to here, tiles of a row beyond (65536 x 2048 bf16:
+                                        // 126 and 90 us; 200000 x 200: 43 us, a wave to a row took 96)
+constexpr long ROWS_AT_ONCE = 1 << 24, SLICED_AT_ONCE = 1 << 22;   // 64 or 512 threads each stay below a launch's 2^32
+
+// A wave to a row, in place of a workgroup, for short rows if there are enough of them: 100000 x 1025 bf16 takes 68 us
+// instead of 303, 16384 x 16384 93 instead of 116, 1024 x 4096 5.1 instead of 6.1; 3001 x 32003 fp32 with 5
+// alternatives would take 100 instead of 73.
+inline bool wave_rows(long rows, int classes) { return rows >= 512 && classes <= 16384; }
 
 // Slices of a row: one up to UNSPLIT classes, where a workgroup ends with the row before a second launch could join
 // slices (one row of 50000 bf16 with 20 alternatives: 10.3 us whole, 12.0 in slices; of 128000: 17.0 and 12.7;
@@ -653,11 +676,13 @@ int score_impl(const void *logits, long rows, int classes, long stride, Targets 
         part.sums = c.take<Sums<A>>(rows * part.slices);
         part.keys = c.take<Key<A>>(rows * part.slices * (size_t)top);
     }
-    // 65535 rows at most in a grid's second dimension
-    for (long r0 = 0; r0 < rows; r0 += 65535) {
-        const long nr = rows - r0 < 65535 ? rows - r0 : 65535;
-        launch("log_probs_slice", want_entropy ? log_probs_slice<T, true> : log_probs_slice<T, false>,
-               dim3((unsigned)part.slices, (unsigned)nr), dim3(SLICE_THREADS), 0, st, x + r0 * stride, classes, stride,
+    const bool waves = wave_rows(rows, classes);
+    const auto kern = waves ? (want_entropy ? log_probs_slice<T, true, 64> : log_probs_slice<T, false, 64>)
+                            : (want_entropy ? log_probs_slice<T, true, SLICE_THREADS> : log_probs_slice<T, false, SLICE_THREADS>);
+    const int threads = waves ? 64 : SLICE_THREADS;
+    for (long r0 = 0; r0 < rows; r0 += SLICED_AT_ONCE) {
+        const long nr = rows - r0 < SLICED_AT_ONCE ? rows - r0 : SLICED_AT_ONCE;
+        launch("log_probs_slice", kern, dim3((unsigned)(nr * part.slices)), dim3(threads), 0, st, x + r0 * stride, classes, stride,
                targets.from(r0), o.from(r0), part);
         CCNN_LAUNCH_CHECK();
     }
@@ -678,13 +703,14 @@ int score_grad_impl(const void *logits, long rows, int classes, long stride, Tar
     T *d = (T *)d_logits;
     const A *s = (const A *)stats;
     const GradIn<A> in = {s + rows, s + 2 * rows, s + 3 * rows, (const A *)d_logp, (const A *)d_entropy};
-    if (classes <= SMALL_CLASSES) {
-        const int lanes = classes <= 16 ? 16 : 64;
-        const long per = 256 / lanes;
-        for (long r0 = 0; r0 < rows; r0 += ROWS_AT_ONCE) {
-            const long nr = rows - r0 < ROWS_AT_ONCE ? rows - r0 : ROWS_AT_ONCE;
-            launch("log_probs_grad_small", log_probs_grad_small<T>, dim3((unsigned)((nr + per - 1) / per)), dim3(256), 0, st,
-                   x + r0 * stride, nr, classes, stride, targets.from(r0), in.from(r0), d + r0 * d_stride, d_stride, lanes);
+    if (classes <= PACKED_CLASSES) {
+        const unsigned packs = (unsigned)((classes * sizeof(T) + 15) / 16);
+        const long most = (1L << 31) / packs;             // rows of a launch: their packs are counted in 32 bits
+        for (long r0 = 0; r0 < rows; r0 += most) {
+            const long nr = rows - r0 < most ? rows - r0 : most;
+            launch("log_probs_grad_packs", log_probs_grad_packs<T>, dim3((unsigned)((nr * packs + 255) / 256)), dim3(256), 0, st,
+                   x + r0 * stride, (unsigned)nr, classes, stride, targets.from(r0), in.from(r0), d + r0 * d_stride, d_stride,
+                   packs);
             CCNN_LAUNCH_CHECK();
         }
         return 0;

@@ -539,8 +539,8 @@ def grad_norm(grads, max_norm=float("inf")):
     kinds = (C.c_int * count)(*[_TYPES[g.dtype] for g in grads])
     out = torch.empty(2, dtype=_F64, device=dev)
     nbytes = _l.load().ccnn_grad_norm_workspace_bytes(n, count)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _enqueue(dev.index, "ccnn_grad_norm", at, n, kinds, count, float(max_norm), out.data_ptr(), ws.data_ptr(), nbytes)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _enqueue(dev.index, "ccnn_grad_norm", at, n, kinds, count, float(max_norm), out.data_ptr(), _at(ws), nbytes)
     return out
 
 

@@ -88,7 +88,7 @@ def weights(rows, kind, seed=1):
 
 
 SHAPES = [(1, 1), (1, 2), (3, 13), (257, 13), (5, 16), (7, 17), (130, 31), (4, 64), (3, 65), (9, 255), (2, 1000), (5, 1024),
-          (16385, 13), (16400, 41), (16390, 200), (20000, 5), (3, 1025), (2, 2049), (3, 4097), (1, 32003), (4, 50251), (3, 65536), (2, 65537), (1, 128000), (2, 131073), (70, 8191), (600, 70001)]
+          (16385, 13), (16400, 41), (16390, 200), (20000, 5), (3, 1025), (2, 2049), (3, 4097), (1, 32003), (4, 50251), (520, 1025), (513, 1037), (600, 8190), (3, 65536), (2, 65537), (1, 128000), (2, 131073), (70, 8191), (600, 70001)]
 
 
 @pytest.mark.parametrize("kind", KINDS, ids=str)
@@ -125,9 +125,7 @@ def test_strided_rows_in_and_out(rows, classes, pad, kind):
     check_scores(odd, y, 7)
 
 
-@pytest.mark.parametrize("kind", KINDS, ids=str)
-@pytest.mark.parametrize("classes", [1, 5, 13, 300, 9001, 70000, 200000])
-def test_masked_and_odd_values(classes, kind):
+def odd_rows(classes, kind):
     low = torch.finfo(kind).min
     rows = 12
     x, y = problem(rows, classes, kind, seed=4)
@@ -150,11 +148,29 @@ def test_masked_and_odd_values(classes, kind):
     y[2] = classes - 1
     y[3] = 0
     y[11] = -100                                  # no target
+    return x, y
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=str)
+@pytest.mark.parametrize("classes", [1, 5, 13, 300, 9001, 70000, 200000])
+def test_masked_and_odd_values(classes, kind):
+    x, y = odd_rows(classes, kind)
     r, want = check_scores(x, y, min(classes, 20))
-    dl, dh = weights(rows, kind)
+    dl, dh = weights(len(y), kind)
     check_grad(x, y, r, want, dl, dh)
     check_grad(x, y, r, want, dl, None)
     check_grad(x, y, r, want, None, dh)
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=str)
+@pytest.mark.parametrize("classes,times", [(13, 1400), (50, 1400), (200, 1400), (1500, 45), (9001, 43)])
+def test_masked_and_odd_values_in_many_rows(classes, times, kind):
+    """The row counts from which other shapes of the kernels take over."""
+    x, y = odd_rows(classes, kind)
+    x, y = x.repeat(times, 1), y.repeat(times)
+    r, want = check_scores(x, y, min(classes, 20))
+    dl, dh = weights(len(y), kind)
+    check_grad(x, y, r, want, dl, dh)
 
 
 @pytest.mark.parametrize("kind", KINDS, ids=str)
@@ -181,11 +197,8 @@ def test_large_common_offset(offset, kind):
     check_grad(x, y, r, want, dl, dh)
 
 
-@pytest.mark.parametrize("kind", KINDS, ids=str)
-@pytest.mark.parametrize("classes", [16, 50, 200, 500, 4096, 20000, 128000])
-def test_ties_and_clustered_alternatives(classes, kind):
-    """Alternatives that sit together, far apart, all equal, or on one stride that a single lane would own."""
-    rows, top = 10, min(64, classes)
+def clustered_rows(classes, top):
+    rows = 10
     x = torch.zeros(rows, classes, dtype=torch.float64)
     ar = torch.arange(classes, dtype=torch.float64)
     x[0] = ar / classes * 4
@@ -195,8 +208,24 @@ def test_ties_and_clustered_alternatives(classes, kind):
     for i, step in enumerate((8, 64, 512, 2048, 4096)):
         x[4 + i, ::step] = 2.0 + torch.arange(len(x[0, ::step]), dtype=torch.float64) / 1e3
     x[9] = (torch.arange(classes) * 2654435761 % 17).double() / 16
-    y = torch.arange(rows, dtype=torch.int64)
+    return x, torch.arange(rows, dtype=torch.int64)
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=str)
+@pytest.mark.parametrize("classes", [16, 50, 200, 500, 4096, 20000, 128000])
+def test_ties_and_clustered_alternatives(classes, kind):
+    """Alternatives that sit together, far apart, all equal, or on one stride that a single lane would own."""
+    top = min(64, classes)
+    x, y = clustered_rows(classes, top)
     check_scores(x.to(kind).cuda(), y.cuda(), top)
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=str)
+@pytest.mark.parametrize("classes,times", [(16, 1640), (50, 1640), (200, 1640), (1025, 52), (4096, 52), (16384, 52)])
+def test_ties_and_clustered_alternatives_in_many_rows(classes, times, kind):
+    top = min(64, classes)
+    x, y = clustered_rows(classes, top)
+    check_scores(x.to(kind).cuda().repeat(times, 1), y.cuda().repeat(times), top)
 
 
 def test_target_out_of_range_is_seen():

@@ -18,9 +18,10 @@ constexpr int BLOCK = CCNN_MOMENT_BLOCK;
 
 // ---------------------------------------------------------------------------- gradient norm
 // Squares are summed in fp64 (no square of an fp32 gradient overflows it, and 2e8 of them lose nothing), in an order
-// that the chunks alone fix.  Bound by the memory: 202 M bf16 gradients in 72 us, 5.6 TB/s, and 4 us for the sum of the
-// 12359 partial sums.  Chunks of 64 K are no faster, workgroups of 512 slower.
-constexpr long NORM_CHUNK = 16384;
+// that the sizes alone fix.  A wave to a chunk: short ones while they are needed to fill the device, long ones beyond
+// (202 M bf16 gradients: 69 us, 5.9 TB/s; 78 with workgroups of 256 to 16 K, 73 with a wave to 16 K).
+inline long norm_chunk(long total) { return total < (1L << 25) ? 4096 : 32768; }
+constexpr int NORM_THREADS = 64;
 
 template <int N>
 struct NormList {
@@ -58,31 +59,31 @@ __device__ __forceinline__ double block_sum(double v, double *lds)
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void norm_partial(NormList<NORM_TENSORS> list, double *__restrict__ partial)
+__global__ __launch_bounds__(NORM_THREADS) void norm_partial(NormList<NORM_TENSORS> list, int chunk, double *__restrict__ partial)
 {
-    constexpr int W = 16 / sizeof(T), U = 8;
-    __shared__ double lds[4];
+    constexpr int W = 16 / sizeof(T), U = 8, STRIDE = NORM_THREADS * W;
     const int i = find(list, blockIdx.x);
-    const T *p = (const T *)list.data[i] + (long)(blockIdx.x - list.chunk0[i]) * NORM_CHUNK;
-    const int n = (int)min(list.n[i] - (long)(blockIdx.x - list.chunk0[i]) * NORM_CHUNK, NORM_CHUNK);
+    const long at = (long)(blockIdx.x - list.chunk0[i]) * chunk;
+    const T *p = (const T *)list.data[i] + at;
+    const int n = (int)min(list.n[i] - at, (long)chunk);
     double s = 0;
-    for (int k = threadIdx.x * W; k < n; k += U * 256 * W) {
+    for (int k = threadIdx.x * W; k < n; k += U * STRIDE) {
         Pack<T, W> x[U];
 #pragma unroll
         for (int u = 0; u < U; u++)
-            if (k + u * 256 * W + W <= n) x[u] = load_pack<W>(p + k + u * 256 * W);
+            if (k + u * STRIDE + W <= n) x[u] = load_pack<W>(p + k + u * STRIDE);
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int at = k + u * 256 * W;
-            if (at + W <= n) {
+            const int j0 = k + u * STRIDE;
+            if (j0 + W <= n) {
 #pragma unroll
                 for (int e = 0; e < W; e++) s += (double)widen(x[u].v[e]) * (double)widen(x[u].v[e]);
             } else {
-                for (int j = at; j < n; j++) s += (double)widen(p[j]) * (double)widen(p[j]);
+                for (int j = j0; j < n; j++) s += (double)widen(p[j]) * (double)widen(p[j]);
             }
         }
     }
-    s = block_sum<256>(s, lds);
+    s = lanes_sum<64>(s);
     if (threadIdx.x == 0) partial[blockIdx.x] = s;
 }
 
@@ -521,6 +522,14 @@ int in_lists(int count, long chunk, Take take, Go go)
     return 0;
 }
 
+inline long sum_of(const long *n, int count)
+{
+    long total = 0;
+    for (int i = 0; i < count; i++)
+        if (n[i] > 0) total += n[i];
+    return total;
+}
+
 inline bool norm_in_one(const long *n, int count)
 {
     if (count > FEW_TENSORS) return false;
@@ -539,9 +548,10 @@ extern "C" {
 size_t ccnn_grad_norm_workspace_bytes(const long *n, int count)
 {
     if (!n || count < 0 || norm_in_one(n, count)) return 0;
+    const long chunk = norm_chunk(sum_of(n, count));
     size_t chunks = 1;
     for (int i = 0; i < count; i++)
-        if (n[i] > 0) chunks += (size_t)((n[i] + NORM_CHUNK - 1) / NORM_CHUNK);
+        if (n[i] > 0) chunks += (size_t)(n[i] / chunk + (n[i] % chunk != 0));
     return chunks * sizeof(double);
 }
 
@@ -574,6 +584,7 @@ int ccnn_grad_norm(const void *const *data, const long *n, const int *types, int
         return 0;
     }
     double *partial = (double *)workspace;
+    const long chunk = norm_chunk(sum_of(n, count));
     int done = 0;
     auto take = [&](auto &list, int i, int type) -> long {
         if (types[i] != type) return 0;
@@ -587,14 +598,14 @@ int ccnn_grad_norm(const void *const *data, const long *n, const int *types, int
         if (!used[type]) continue;
         typedef NormList<NORM_TENSORS> List;
         const int e = in_lists<List>(
-            count, NORM_CHUNK, [&](List &list, int i) { return take(list, i, type); },
+            count, chunk, [&](List &list, int i) { return take(list, i, type); },
             [&](const List &list) -> int {
                 const int chunks = list.chunk0[list.count];
                 launch("norm_partial", type == CCNN_TYPE_F32    ? norm_partial<float>
                                        : type == CCNN_TYPE_F64  ? norm_partial<double>
                                        : type == CCNN_TYPE_BF16 ? norm_partial<Bf16>
                                                                 : norm_partial<F16>,
-                       dim3((unsigned)chunks), dim3(256), 0, st, list, partial + done);
+                       dim3((unsigned)chunks), dim3(NORM_THREADS), 0, st, list, (int)chunk, partial + done);
                 CCNN_LAUNCH_CHECK();
                 done += chunks;
                 return 0;

@@ -254,7 +254,8 @@ __global__ __launch_bounds__(256) void log_probs_small(const T *__restrict__ log
 // top k elements all reach and few others do; only the threads that hold such an element look at their part
 // again, what reaches the bar is collected in LDS and put in order by counting.
 // Without entropy and alternatives the memory bounds it: 4096 x 128000 bf16 in 167 us, 6.3 TB/s.  With both it is the
-// vector units (10.5 operations an element and an exponential that counts for four): 2048 x 128000 bf16 in 101 us.
+// vector units (10.5 operations an element and an exponential that counts for four): 2048 x 128000 bf16 in 101 us;
+// x L - c in one multiply-add in place of (x - m) L changes nothing there and costs short rows 8 %.
 // One row of 128000 takes 7.4 us in slices and 5.5 to join them, most of it the four waits of the selection.
 constexpr int SLICE_THREADS = 512;   // or 64: see wave_rows
 constexpr int CANDIDATES = 1024;      // of the joining workgroup

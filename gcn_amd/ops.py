@@ -611,7 +611,9 @@ class AdamW:
             self.m_scale, self.v_scale = (torch.zeros(block, dtype=_F32, device=self.device) for _ in range(2))
         self.master = None
         if any(p.element_size() == 2 for p in self.params):
-            self.master = torch.cat([p.detach().reshape(-1).float() for p in self.params])
+            flat = [p.detach().reshape(-1) for p in self.params]
+            same = len(set(self._dtypes)) == 1
+            self.master = torch.cat(flat).float() if same else torch.cat([p.float() for p in flat])
         self._clock = torch.zeros(_l.ADAMW_CLOCK, dtype=_F64, device=self.device)
         self._set_step(0)
 

@@ -489,10 +489,11 @@ __global__ __launch_bounds__(256) void adamw_decode(StepList<STEP_TENSORS> list,
 }
 
 // ---------------------------------------------------------------------------- host
-// Below so many elements a step of few tensors of one type is one launch, with one pack a thread, a short argument block
-// and the clock moved by its last workgroup: it is all latency (47 k fp32 parameters: 5.3 us of the device instead
-// of 9.3 in packs of four, and another launch costs the host 3).
-constexpr long WIDE_SMALL = 1 << 20;
+// Below so many elements a step of few tensors of one type is one launch, with one pack a lane, a short argument block
+// and the clock moved by the last workgroup to arrive: 47 k fp32 parameters take 5.5 us of the device instead of 7.1
+// in two launches, and 7 us of the host instead of 9.7.  Each arrival costs some 10 ns, one after the other: 100 k
+// take 8 us either way, 1 M would take 48 instead of 9.
+constexpr long WIDE_SMALL = 3 << 15;
 // Hands tensors [0, count) that `take` accepts to `go`, a list at a time, with their chunks counted.
 template <typename List, typename Take, typename Go>
 int in_lists(int count, long chunk, Take take, Go go)

@@ -174,6 +174,20 @@ def test_more_tensors_than_one_launch_lists(bits):
     assert n[0].item() == pytest.approx(float(torch.cat([g.cpu().double() for g in grads]).norm()), rel=1e-13)
 
 
+@pytest.mark.parametrize("kind", [F32, F64, BF16], ids=str)
+@pytest.mark.parametrize("sizes", [[98303], [98304], [3 << 15, 5], [50000, 47000, 1304], [1500001]])
+def test_sizes_around_the_one_launch_step(kind, sizes):
+    """Below 98304 elements the step's one launch moves its own clock, from there on a launch before it does."""
+    params, lr, u = tensors(sizes, kind, 6, 0.5), 1e-2, ref.half_step(F64 if kind == F64 else F32)
+    want, opt = ref.AdamW(params, lr), ops.AdamW(params, lr=lr)
+    for k in range(3):
+        grads = tensors(sizes, kind, 400 + k, 1e-3)
+        opt.step(grads)
+        want.step(grads)
+        assert opt.step_count == k + 1
+    check(opt, want, params, 3, u, lr)
+
+
 def test_types_mixed_in_one_list():
     kinds = [F32, BF16, F16, BF16, F32, F16]
     params = [tensors([777 + i], k, i, 0.5)[0] for i, k in enumerate(kinds)]

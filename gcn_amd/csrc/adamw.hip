@@ -286,7 +286,8 @@ __global__ __launch_bounds__(WIDE_THREADS) void adamw_wide(StepList<U == 1 ? FEW
         for (int e = 0; e < W; e++) {
             const A g = (A)widen(gk[u].v[e]) * r.scale;
             mk[u].v[e] += b1 * (g - mk[u].v[e]);
-            vk[u].v[e] += b2 * (g * g - vk[u].v[e]);
+            const A old_v = vk[u].v[e];
+            vk[u].v[e] += b2 * (g * g - (old_v == -ninf(A()) ? A(0) : old_v));   // what is beyond the type stays infinite
             pk[u].v[e] = stepped((A)pk[u].v[e], mk[u].v[e], (A)sqrt(vk[u].v[e]), r);
             narrow(pk[u].v[e], out.v[e]);
         }

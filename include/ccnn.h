@@ -444,7 +444,8 @@ int ccnn_grad_norm(const void *const *data, const long *n, const int *types, int
  * moments are computed in fp64 from the old codes, as beta x + (1 - beta) y with each operation rounded by
  * itself, and then rounded once, to the nearest code (ties to the even one); a sqrt(v) above 0 keeps at
  * least the smallest code, so a denominator never becomes 0 by rounding.  A block's bytes behind the tensor's end are left 0.  A gradient that is not finite makes
- * its whole block NaN (with 32 bits: its element).
+ * its whole block NaN (with 32 bits: its element).  With 32 bits a g^2 that does not fit the type makes v infinite for
+ * good, and the element is then moved by its decay alone.
  * clock [CCNN_ADAMW_CLOCK] device doubles: clock[0] = t, steps taken so far, clock[1] = beta1^t,
  * clock[2] = beta2^t (initially 0, 1, 1, and the rest 0); the call advances them on the device, so a captured step counts
  * on when it is replayed.  lr_device, if not NULL, is read instead of lr.  clip, if not NULL, is

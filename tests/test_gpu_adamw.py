@@ -128,6 +128,20 @@ def test_magnitudes_at_the_edges(bits):
     assert (p.cpu().double() - want.p[0]).abs().max() < 3 * 0.1 * 1e-5 + 1e-10
 
 
+@pytest.mark.parametrize("n", [1000, 200001])
+def test_a_square_beyond_fp32_stops_its_element(n):
+    """A finite gradient whose square does not fit fp32 makes v infinite, and the element no longer moves; the others do."""
+    p = torch.zeros(n, device="cuda")
+    g = torch.full((n,), 0.1, device="cuda")
+    g[n - 7] = 1e20
+    opt = ops.AdamW([p], weight_decay=0.0)
+    for _ in range(3):
+        opt.step([g])
+        g[n - 7] = 0.1
+    assert torch.isfinite(p).all() and p[n - 7] == 0 and (p[: n - 7] < 0).all() and (p[n - 6:] < 0).all()
+    assert opt.moments()[1][n - 7] == math.inf
+
+
 def test_a_root_above_zero_never_becomes_zero():
     g = torch.full((256,), 1e-7, device="cuda")
     g[0] = 1.0

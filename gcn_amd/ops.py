@@ -618,7 +618,15 @@ class AdamW:
         self._set_step(0)
 
     def _set_step(self, t):
-        self._clock.copy_(torch.tensor([t, self.betas[0] ** t, self.betas[1] ** t] + [0.0] * (_l.ADAMW_CLOCK - 3), dtype=_F64))
+        powers = []
+        for beta in self.betas:         # multiplied step by step as the device does, so that a loaded optimiser goes on alike
+            x = 1.0
+            for _ in range(t):
+                x, before = x * beta, x
+                if x == before:         # 0, or where it stops changing
+                    break
+            powers.append(x)
+        self._clock.copy_(torch.tensor([t, *powers] + [0.0] * (_l.ADAMW_CLOCK - 3), dtype=_F64))
 
     @property
     def step_count(self):

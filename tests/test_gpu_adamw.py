@@ -142,6 +142,29 @@ def test_a_square_beyond_fp32_stops_its_element(n):
     assert opt.moments()[1][n - 7] == math.inf
 
 
+@pytest.mark.parametrize("kind,bits", [(F32, 32), (F64, 32), (BF16, 8)], ids=str)
+def test_a_loaded_optimiser_continues_bit_for_bit(kind, bits):
+    params = tensors([700, 300], kind, 21, 0.5)
+    opt = ops.AdamW(params, lr=1e-2, betas=(0.87, 0.983), state_bits=bits)
+    for k in range(57):
+        opt.step(tensors([700, 300], kind, 500 + k, 1e-2))
+    other = [p.clone() for p in params]
+    new = ops.AdamW(other, lr=1e-2, betas=(0.87, 0.983), state_bits=bits)
+    new.load_state_dict(opt.state_dict())
+    assert torch.equal(new._clock[:3], opt._clock[:3])
+    g = tensors([700, 300], kind, 600, 1e-2)
+    opt.step(g)
+    new.step(g)
+    assert all(torch.equal(a, b) for a, b in zip(params, other))
+    assert all(torch.equal(a, b) for a, b in zip(opt.moments(), new.moments()))
+
+
+def test_powers_of_long_runs():
+    opt = ops.AdamW([torch.zeros(1, device="cuda")], betas=(0.0, 0.9))
+    opt._set_step(10 ** 9)                       # 0.9^t has stopped changing long before
+    assert opt._clock[0] == 10 ** 9 and opt._clock[1] == 0 and 0 <= opt._clock[2] < 1e-300
+
+
 def test_a_root_above_zero_never_becomes_zero():
     g = torch.full((256,), 1e-7, device="cuda")
     g[0] = 1.0

@@ -625,7 +625,7 @@ int ccnn_adamw_step(const ccnn_adamw_tensor_t *tensors, const void *const *grads
 {
     if (count < 0 || (count > 0 && (!tensors || !grads || !grad_types)) || !clock) return CCNN_E_INVALID;
     if (moment_bits != 32 && moment_bits != 8) return CCNN_E_INVALID;
-    if (!(beta1 >= 0 && beta1 < 1) || !(beta2 >= 0 && beta2 < 1) || !(eps >= 0)) return CCNN_E_INVALID;
+    if (!(beta1 >= 0 && beta1 < 1) || !(beta2 >= 0 && beta2 < 1) || !(eps > 0)) return CCNN_E_INVALID;
     bool wide = false, other = false;
     long total = 0;
     for (int i = 0; i < count; i++) {
@@ -639,6 +639,7 @@ int ccnn_adamw_step(const ccnn_adamw_tensor_t *tensors, const void *const *grads
         total += t.n;
     }
     if (wide && (other || moment_bits == 8)) return CCNN_E_INVALID;
+    if (other && !((float)eps > 0)) return CCNN_E_INVALID;     // without a gradient yet the quotient would be 0 / 0
     if (total > 0 && (!m || !v || (moment_bits == 8 && (!m_scale || !v_scale)))) return CCNN_E_INVALID;
     hipStream_t st = (hipStream_t)stream;
     const StepArgs args = {m, v, m_scale, v_scale, master, clock, beta1, beta2, eps, lr, lr_device, clip};

@@ -571,8 +571,8 @@ class AdamW:
         decays = [float(weight_decay)] * n if not hasattr(weight_decay, "__len__") else [float(w) for w in weight_decay]
         if len(decays) != n:
             raise ValueError(f"{len(decays)} weight_decay factors for {n} tensors")
-        if not all(0 <= b < 1 for b in betas) or len(betas) != 2 or not eps >= 0:
-            raise ValueError(f"betas must be two numbers in [0, 1) and eps not negative, got {betas}, {eps}")
+        if not all(0 <= b < 1 for b in betas) or len(betas) != 2:
+            raise ValueError(f"betas must be two numbers in [0, 1), got {betas}")
         self.device = self.params[0].device if isinstance(self.params[0], torch.Tensor) else None
         self.betas, self.eps, self.state_bits = (float(betas[0]), float(betas[1])), float(eps), state_bits
         self.lr = lr
@@ -588,6 +588,8 @@ class AdamW:
                 raise TypeError("fp64 parameters do not mix with others in one optimiser")
             if p.dtype == _F64 and state_bits == 8:
                 raise TypeError("moments in 8 bits are not for fp64 parameters")
+            if not (eps if p.dtype == _F64 else C.c_float(eps).value) > 0:
+                raise ValueError(f"eps must be positive, in fp32 too where the parameters are not fp64, got {eps}")
             kind = _TYPES[p.dtype]
             self._table[i] = (p.data_ptr(), p.numel(), first, block, decays[i], kind)
             if p.numel():

@@ -433,6 +433,7 @@ int ccnn_grad_norm(const void *const *data, const long *n, const int *types, int
 /* One AdamW step (decoupled weight decay) over `count` parameter tensors:
  *   g *= clip[1];  m += (1 - beta1)(g - m);  v += (1 - beta2)(g^2 - v)
  *   p -= lr (decay p + m / (1 - beta1^t) / (sqrt(v / (1 - beta2^t)) + eps))
+ * eps > 0, as fp32 too where the parameters are not F64.
  * tensors, grads, grad_types: HOST arrays of `count` entries.  `type` of a parameter is F32, F64, BF16 or
  * F16; its gradient's the same, or F32 for BF16 and F16.  F64 does not mix with the others in one call.
  * `first` is the tensor's place (in elements) in the flat arrays `master` (fp32, needed for BF16 and F16 parameters: the step is taken

@@ -159,6 +159,7 @@ def test_scoring_and_optimiser_calls_refuse_bad_arguments():
     assert step((64, 10, 0, 0, 0.1, 2), bits=8) == -1                      # 8-bit moments of doubles
     assert step(fine, (64, 10, 0, 0, 0.1, 2)) == -1                        # doubles among others
     assert step((64, 10, 0, 0, 0.1, 3), kinds=[4]) == -1
+    assert step(fine, eps=0.0) == -1 and step(fine, eps=1e-46) == -1 and step((64, 10, 0, 0, 0.1, 2), eps=0.0) == -1
     for bad in ((0, 10, 0, 0, 0.1, 1), (64, -1, 0, 0, 0.1, 1), (64, 10, -1, 0, 0.1, 1), (64, 10, 0, -1, 0.1, 1),
                 (64, 10, 0, 0, 0.1, 0)):
         assert step(bad) == -1, bad

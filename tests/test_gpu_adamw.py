@@ -165,6 +165,37 @@ def test_powers_of_long_runs():
     assert opt._clock[0] == 10 ** 9 and opt._clock[1] == 0 and 0 <= opt._clock[2] < 1e-300
 
 
+@pytest.mark.parametrize("kind,bits", [(F32, 32), (BF16, 32), (BF16, 8), (F64, 32)], ids=str)
+def test_the_smallest_eps(kind, bits):
+    """A parameter that never has a gradient stays where it is, down to the smallest eps that is taken."""
+    smallest = 5e-324 if kind == F64 else 1e-45
+    p = torch.ones(500, dtype=kind, device="cuda")
+    opt = ops.AdamW([p], eps=smallest, weight_decay=0.0, state_bits=bits)
+    opt.step([torch.zeros_like(p)])
+    assert (p == 1).all()
+    for eps in (0.0, smallest / 4, math.nan):
+        with pytest.raises(ValueError):
+            ops.AdamW([p], eps=eps, state_bits=bits)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_elements_beyond_32_bits(bits):
+    """A tensor of more than 2^31 elements: the same gradient at a few places far apart and nowhere else."""
+    n = (1 << 31) + 5003
+    p = torch.zeros(n, dtype=BF16, device="cuda")
+    g = torch.zeros(n, dtype=BF16, device="cuda")
+    at = torch.tensor([0, 1 << 30, (1 << 31) - 1, 1 << 31, n - 257, n - 1], device="cuda")
+    g[at] = 0.5
+    norm = ops.grad_norm([g], math.inf)
+    assert norm.tolist() == [pytest.approx(0.5 * math.sqrt(6), rel=1e-15), 1.0]
+    opt = ops.AdamW([p], lr=0.25, weight_decay=0.0, state_bits=bits)
+    opt.step([g])
+    assert (p[at] == -0.25).all() and torch.count_nonzero(p) == 6
+    m, v = opt.moments()
+    assert (m[at] - 0.05).abs().max() < 0.05 * 2.0 ** -4 and torch.count_nonzero(m) == 6
+    assert (v[at] - 0.00025).abs().max() < 0.00025 * 2.0 ** -2 and torch.count_nonzero(v) == 6
+
+
 def test_a_root_above_zero_never_becomes_zero():
     g = torch.full((256,), 1e-7, device="cuda")
     g[0] = 1.0

@@ -228,6 +228,46 @@ def test_ties_and_clustered_alternatives_in_many_rows(classes, times, kind):
     check_scores(x.to(kind).cuda().repeat(times, 1), y.cuda().repeat(times), top)
 
 
+SIGNALLING = {torch.float32: (torch.int32, 0x7f800001), torch.float64: (torch.int64, 0x7ff0000000000001),
+              torch.bfloat16: (torch.int16, 0x7f81), torch.float16: (torch.int16, 0x7c01)}
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=str)
+@pytest.mark.parametrize("rows,classes", [(3, 13), (3, 700), (3, 5000), (600, 5000), (2, 200000)])
+def test_rows_of_signalling_nans(rows, classes, kind):
+    """Arithmetic turns these NaNs into others, so a largest value of theirs need not be found again; the results of
+    the calls before lie in the memory that is written."""
+    x, y = problem(rows, classes, kind, seed=9)
+    bits, code = SIGNALLING[kind]
+    x = x.contiguous()
+    x.view(bits)[0] = code
+    x.view(bits)[1, ::3] = code
+    top = min(classes, 40)
+    for _ in range(3):
+        torch.full((rows, top), 5, dtype=torch.int32, device="cuda")
+        torch.full((rows, top), 5, dtype=wide(kind), device="cuda")
+        r = ops.log_probs(x, y, top=top)
+        for k in (0, 1):
+            assert torch.isnan(r.logp[k]) and torch.isnan(r.entropy[k]) and torch.isnan(r.top_logp[k]).all()
+            assert (r.top_index[k] == -1).all()
+    x[:2] = 0.5
+    check_scores(x, y, top)
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=str)
+@pytest.mark.parametrize("rows,classes", [(64, 2), (40, 13), (40, 200), (40, 1000), (40, 5000), (600, 5000), (40, 100000)])
+def test_no_log_probability_above_zero_and_no_entropy_below(rows, classes, kind):
+    """One class with all of the weight, or nearly all of it."""
+    g = torch.Generator().manual_seed(rows + classes)
+    x = torch.full((rows, classes), -1e4, dtype=torch.float64)
+    x[1::2] = -20.0 * torch.rand(len(x[1::2]), 1, generator=g, dtype=torch.float64)
+    at = torch.randint(0, classes, (rows,), generator=g)
+    x[torch.arange(rows), at] = 17.0 * torch.rand(rows, generator=g, dtype=torch.float64)
+    x, y = x.to(kind).cuda(), at.int().cuda()
+    r, _ = check_scores(x, y, min(classes, 5))
+    assert (r.logp <= 0).all() and (r.top_logp <= 0).all() and (r.stats[3] >= 0).all() and (r.entropy >= 0).all()
+
+
 def test_target_out_of_range_is_seen():
     x, _ = problem(4, 13, torch.float32)
     y = torch.tensor([12, 13, 2 ** 31 - 1, -1], dtype=torch.int32).cuda()

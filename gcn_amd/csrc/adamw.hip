@@ -167,12 +167,14 @@ struct StepArgs {
     double *clock;
     double beta1, beta2, eps, lr;
     const double *lr_device, *clip;
+    bool alone;   // the launch is the whole step, and moves the clock
 };
 
 // What a step takes from the clock, for all its elements alike.
 struct Tick {
     double t, beta1_t, beta2_t, lr, rate, root, scale;   // steps, powers; lr, lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t), gradient factor
     bool skip;
+    __device__ Tick() {}
     __device__ explicit Tick(const StepArgs &a)
     {
         scale = a.clip ? a.clip[1] : 1.0;
@@ -190,7 +192,8 @@ struct Tick {
     }
 };
 
-// clock: t, beta1^t, beta2^t | lr, lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t), gradient factor (NaN: no step) | arrivals
+// clock: t, beta1^t, beta2^t | lr, lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t), gradient factor (NaN: no step) | arrivals,
+// of all and of each group
 __global__ void adamw_clock(StepArgs a)
 {
     const Tick tick(a);
@@ -217,17 +220,32 @@ struct Rates {
     }
 };
 
-// A launch that is the whole step moves the clock itself: every workgroup has read it when it arrives here, the last
-// to arrive writes it and leaves the count at 0.
+// A launch that is the whole step moves the clock itself: every wave has read it when its workgroup arrives here, the
+// last to arrive writes it and leaves the counts at 0.  One count takes an arrival some 7 ns after the one before, so
+// beyond a few workgroups they arrive in groups, each counting in a cache line of its own, and then the groups do
+// (1 M fp32 parameters in 3907 workgroups: 48 us with one count, 6.9 with 32 groups, 8.3 with 16; 400 k: 4.9 us with 32,
+// 5.7 with 128).
+constexpr unsigned ARRIVE_AT_ONCE = 64, ARRIVE_GROUPS = 32, ARRIVE_LINE = 16;
+static_assert(CCNN_ADAMW_CLOCK == ARRIVE_LINE * (ARRIVE_GROUPS + 1), "a line of the clock, and one for each group");
+
+template <int THREADS>
 __device__ __forceinline__ void arrive(const StepArgs &a, const Tick &tick)
 {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");     // the reads above are done
-    if (threadIdx.x == 0) {
-        unsigned *arrivals = reinterpret_cast<unsigned *>(a.clock + CCNN_ADAMW_CLOCK - 1);
-        if (atomicAdd(arrivals, 1u) == gridDim.x - 1) {
-            tick.keep(a.clock);
-            *arrivals = 0;
-        }
+    if (THREADS > 64) __syncthreads();
+    else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");     // the reads above are done
+    if (threadIdx.x != 0) return;
+    unsigned *all = reinterpret_cast<unsigned *>(a.clock + 7);
+    unsigned parts = gridDim.x;
+    if (parts > ARRIVE_AT_ONCE) {
+        const unsigned group = blockIdx.x % ARRIVE_GROUPS, members = (gridDim.x - group + ARRIVE_GROUPS - 1) / ARRIVE_GROUPS;
+        unsigned *mine = reinterpret_cast<unsigned *>(a.clock + ARRIVE_LINE * (1 + group));
+        if (atomicAdd(mine, 1u) != members - 1) return;
+        *mine = 0;
+        parts = ARRIVE_GROUPS;
+    }
+    if (atomicAdd(all, 1u) == parts - 1) {
+        tick.keep(a.clock);
+        *all = 0;
     }
 }
 
@@ -268,14 +286,9 @@ __global__ __launch_bounds__(WIDE_THREADS) void adamw_wide(StepList<U == 1 ? FEW
         vk[u] = load_some<W>(v, k, n);
         pk[u] = load_some<W>(held, k, n);
     }
-    std::conditional_t<U == 1, Tick, int> tick = [&] {
-        if constexpr (U == 1) return Tick(a);
-        else return 0;
-    }();
-    const Rates<A> r = [&] {
-        if constexpr (U == 1) return Rates<A>(a, tick, list.decay[i]);
-        else return Rates<A>(a, list.decay[i]);
-    }();
+    const bool alone = U == 1 || a.alone;
+    const Tick tick = alone ? Tick(a) : Tick();
+    const Rates<A> r = alone ? Rates<A>(a, tick, list.decay[i]) : Rates<A>(a, list.decay[i]);
     if (r.skip) return;
     const A b1 = (A)(1 - a.beta1), b2 = (A)(1 - a.beta2);
 #pragma unroll
@@ -296,7 +309,7 @@ __global__ __launch_bounds__(WIDE_THREADS) void adamw_wide(StepList<U == 1 ? FEW
         if constexpr (COPY) store_some<W>(held, k, n, pk[u]);
         store_some<W>(param, k, n, out);
     }
-    if constexpr (U == 1) arrive(a, tick);
+    if (alone) arrive<WIDE_THREADS>(a, tick);
 }
 
 // e4m3: values 2^-9 apart below 2^-6, then eight to each power of two up to 448.
@@ -384,7 +397,7 @@ __device__ __forceinline__ float scale_of(float h)
 // 2 %).  Moments, root and step in fp64, so that codes, scales and steps are those of the definition whatever the
 // order of operations.  101 M bf16 parameters with fp32 master copy (16 bytes each) in 299 us, 5.4 TB/s; the vector
 // units are busy for some 60 % of it (342 operations a block and lane in an earlier form were 75 % and 4 % slower).
-template <typename P, typename G>
+template <typename P, typename G, bool ALONE>
 __global__ __launch_bounds__(256) void adamw_coded(StepList<STEP_TENSORS> list, StepArgs a)
 {
     constexpr bool COPY = sizeof(P) == 2;
@@ -415,7 +428,8 @@ __global__ __launch_bounds__(256) void adamw_coded(StepList<STEP_TENSORS> list, 
         ms[u] = a.m_scale[blk0 + u];
         vs[u] = a.v_scale[blk0 + u];
     }
-    const Rates<double> r(a, list.decay[i]);
+    const Tick tick = ALONE ? Tick(a) : Tick();
+    const Rates<double> r = ALONE ? Rates<double>(a, tick, list.decay[i]) : Rates<double>(a, list.decay[i]);
     if (r.skip) return;
 #pragma unroll
     for (int u = 0; u < U; u++) {
@@ -454,6 +468,7 @@ __global__ __launch_bounds__(256) void adamw_coded(StepList<STEP_TENSORS> list, 
         ((unsigned *)a.v)[(blk0 + u) * (BLOCK / 4) + lane] = codes<true>(root, v, root32, sv);
         if (lane == 0) a.m_scale[blk0 + u] = sm, a.v_scale[blk0 + u] = sv;
     }
+    if (ALONE) arrive<256>(a, tick);
 }
 
 // 8-bit moments read out: 101 M of each in 142 us, 7.1 TB/s, four fifths of it written.
@@ -490,11 +505,12 @@ __global__ __launch_bounds__(256) void adamw_decode(StepList<STEP_TENSORS> list,
 }
 
 // ---------------------------------------------------------------------------- host
-// Below so many elements a step of few tensors of one type is one launch, with one pack a lane, a short argument block
-// and the clock moved by the last workgroup to arrive: 47 k fp32 parameters take 5.5 us of the device instead of 7.1
-// in two launches, and 7 us of the host instead of 9.7.  Each arrival costs some 10 ns, one after the other: 100 k
-// take 8 us either way, 1 M would take 48 instead of 9.
-constexpr long WIDE_SMALL = 3 << 15;
+// A step of one pair of types is one launch that moves the clock itself.  Of few tensors and up to WIDE_SMALL elements it has
+// one pack a lane and a short argument block: fp32, 47 k in 4.9 us of the device and 1 M in 6.9 (four packs 6.2 and 8.3,
+// the clock in a launch of its own 7.2 and 8.9), 4 M in 21.2 (four packs 20.2).  With 8-bit moments working out the
+// step's rates in every wave pays up to ALONE_CODED: 1 M in 7.2 us instead of 8.0, 4 M 16.4 and 16.0, 100 M 304 and 291.
+constexpr long WIDE_SMALL = 1 << 20, ALONE_CODED = 3 << 20;
+
 // Hands tensors [0, count) that `take` accepts to `go`, a list at a time, with their chunks counted.
 template <typename List, typename Take, typename Go>
 int in_lists(int count, long chunk, Take take, Go go)
@@ -642,26 +658,27 @@ int ccnn_adamw_step(const ccnn_adamw_tensor_t *tensors, const void *const *grads
     if (other && !((float)eps > 0)) return CCNN_E_INVALID;     // without a gradient yet the quotient would be 0 / 0
     if (total > 0 && (!m || !v || (moment_bits == 8 && (!m_scale || !v_scale)))) return CCNN_E_INVALID;
     hipStream_t st = (hipStream_t)stream;
-    const StepArgs args = {m, v, m_scale, v_scale, master, clock, beta1, beta2, eps, lr, lr_device, clip};
+    StepArgs args = {m, v, m_scale, v_scale, master, clock, beta1, beta2, eps, lr, lr_device, clip, false};
     typedef StepList<FEW_TENSORS> Few;
     typedef StepList<STEP_TENSORS> Many;
     const struct {
         int type, grad_type;
         void (*one)(Few, StepArgs);
         void (*four)(Many, StepArgs);
-        void (*coded)(Many, StepArgs);
+        void (*coded)(Many, StepArgs), (*coded_alone)(Many, StepArgs);
     } kinds[] = {
-        {CCNN_TYPE_F32, CCNN_TYPE_F32, adamw_wide<float, float, 1>, adamw_wide<float, float, 4>, adamw_coded<float, float>},
-        {CCNN_TYPE_F64, CCNN_TYPE_F64, adamw_wide<double, double, 1>, adamw_wide<double, double, 4>, nullptr},
-        {CCNN_TYPE_BF16, CCNN_TYPE_BF16, adamw_wide<Bf16, Bf16, 1>, adamw_wide<Bf16, Bf16, 4>, adamw_coded<Bf16, Bf16>},
-        {CCNN_TYPE_BF16, CCNN_TYPE_F32, adamw_wide<Bf16, float, 1>, adamw_wide<Bf16, float, 4>, adamw_coded<Bf16, float>},
-        {CCNN_TYPE_F16, CCNN_TYPE_F16, adamw_wide<F16, F16, 1>, adamw_wide<F16, F16, 4>, adamw_coded<F16, F16>},
-        {CCNN_TYPE_F16, CCNN_TYPE_F32, adamw_wide<F16, float, 1>, adamw_wide<F16, float, 4>, adamw_coded<F16, float>},
+        {CCNN_TYPE_F32, CCNN_TYPE_F32, adamw_wide<float, float, 1>, adamw_wide<float, float, 4>, adamw_coded<float, float, false>, adamw_coded<float, float, true>},
+        {CCNN_TYPE_F64, CCNN_TYPE_F64, adamw_wide<double, double, 1>, adamw_wide<double, double, 4>, nullptr, nullptr},
+        {CCNN_TYPE_BF16, CCNN_TYPE_BF16, adamw_wide<Bf16, Bf16, 1>, adamw_wide<Bf16, Bf16, 4>, adamw_coded<Bf16, Bf16, false>, adamw_coded<Bf16, Bf16, true>},
+        {CCNN_TYPE_BF16, CCNN_TYPE_F32, adamw_wide<Bf16, float, 1>, adamw_wide<Bf16, float, 4>, adamw_coded<Bf16, float, false>, adamw_coded<Bf16, float, true>},
+        {CCNN_TYPE_F16, CCNN_TYPE_F16, adamw_wide<F16, F16, 1>, adamw_wide<F16, F16, 4>, adamw_coded<F16, F16, false>, adamw_coded<F16, F16, true>},
+        {CCNN_TYPE_F16, CCNN_TYPE_F32, adamw_wide<F16, float, 1>, adamw_wide<F16, float, 4>, adamw_coded<F16, float, false>, adamw_coded<F16, float, true>},
     };
     bool alike = true;
     for (int i = 1; i < count; i++) alike &= tensors[i].type == tensors[0].type && grad_types[i] == grad_types[0];
-    const bool small = moment_bits == 32 && total > 0 && total < WIDE_SMALL && count <= FEW_TENSORS && alike;
-    if (!small) {
+    args.alone = alike && total > 0 && count <= STEP_TENSORS && (moment_bits == 32 || total < ALONE_CODED);
+    const bool small = args.alone && moment_bits == 32 && total < WIDE_SMALL && count <= FEW_TENSORS;
+    if (!args.alone) {
         launch("adamw_clock", adamw_clock, dim3(1), dim3(1), 0, st, args);
         CCNN_LAUNCH_CHECK();
     }
@@ -688,7 +705,7 @@ int ccnn_adamw_step(const ccnn_adamw_tensor_t *tensors, const void *const *grads
             });
         else
             e = in_lists<Many>(count, moment_bits == 8 ? CODED_CHUNK : WIDE_THREADS * 16, take, [&](const Many &list) -> int {
-                launch(moment_bits == 8 ? "adamw_coded" : "adamw_wide", moment_bits == 8 ? kind.coded : kind.four,
+                launch(moment_bits == 8 ? "adamw_coded" : "adamw_wide", moment_bits == 32 ? kind.four : args.alone ? kind.coded_alone : kind.coded,
                        dim3((unsigned)list.chunk0[list.count]), dim3(moment_bits == 8 ? 256 : WIDE_THREADS), 0, st, list, args);
                 CCNN_LAUNCH_CHECK();
                 return 0;

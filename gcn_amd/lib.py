@@ -36,7 +36,7 @@ class AdamwTensor(C.Structure):
 
 
 TYPE_F32, TYPE_F64, TYPE_BF16, TYPE_F16 = 1, 2, 3, 4     # CCNN_TYPE_*
-MAX_TOP, MOMENT_BLOCK, ADAMW_CLOCK = 64, 256, 8
+MAX_TOP, MOMENT_BLOCK, ADAMW_CLOCK = 64, 256, 528
 
 _P = C.c_void_p
 _SIG = {

@@ -448,11 +448,11 @@ int ccnn_grad_norm(const void *const *data, const long *n, const int *types, int
  * its whole block NaN (with 32 bits: its element).  With 32 bits a g^2 that does not fit the type makes v infinite for
  * good, and the element is then moved by its decay alone.
  * clock [CCNN_ADAMW_CLOCK] device doubles: clock[0] = t, steps taken so far, clock[1] = beta1^t,
- * clock[2] = beta2^t (initially 0, 1, 1, and the rest 0); the call advances them on the device, so a captured step counts
+ * clock[2] = beta2^t (initially 0, 1, 1, and the rest 0; the rest is the call's own); the call advances them on the device, so a captured step counts
  * on when it is replayed.  lr_device, if not NULL, is read instead of lr.  clip, if not NULL, is
  * ccnn_grad_norm's out: when clip[1] is not finite nothing is changed, t included. */
 #define CCNN_MOMENT_BLOCK 256
-#define CCNN_ADAMW_CLOCK 8
+#define CCNN_ADAMW_CLOCK 528
 typedef struct ccnn_adamw_tensor {
     void *param;
     long n;

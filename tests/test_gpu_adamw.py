@@ -245,7 +245,7 @@ def test_more_tensors_than_one_launch_lists(bits):
 @pytest.mark.parametrize("kind", [F32, F64, BF16], ids=str)
 @pytest.mark.parametrize("sizes", [[98303], [98304], [3 << 15, 5], [50000, 47000, 1304], [1500001]])
 def test_sizes_around_the_one_launch_step(kind, sizes):
-    """Below 98304 elements the step's one launch moves its own clock, from there on a launch before it does."""
+    """Steps of middling sizes, whichever launch moves their clock."""
     params, lr, u = tensors(sizes, kind, 6, 0.5), 1e-2, ref.half_step(F64 if kind == F64 else F32)
     want, opt = ref.AdamW(params, lr), ops.AdamW(params, lr=lr)
     for k in range(3):
@@ -254,6 +254,31 @@ def test_sizes_around_the_one_launch_step(kind, sizes):
         want.step(grads)
         assert opt.step_count == k + 1
     check(opt, want, params, 3, u, lr)
+
+
+@pytest.mark.parametrize("bits,sizes", [(32, [1]), (32, [64 * 256]), (32, [64 * 256 + 1]), (32, [33 * 256] * 16), (32, [1 << 20]),
+                                        (32, [(1 << 20) - 1]), (32, [9000] * 64), (32, [9000] * 65), (32, [0, 5000, 0]),
+                                        (8, [64 * 2048]), (8, [64 * 2048 + 1]), (8, [(3 << 20) - 1]), (8, [3 << 20]), (8, [777] * 64),
+                                        (8, [777] * 65)], ids=str)
+def test_the_clock_moves_once_a_step(bits, sizes):
+    """Whatever launch moves it: alone, in groups that meet, in front of several; also where other work runs beside it."""
+    params = tensors(sizes, F32, 30, 0.5)
+    many = tensors([5000] * 40, F32, 31, 0.5)
+    opt, other = ops.AdamW(params, state_bits=bits), ops.AdamW(many)
+    grads, g2 = tensors(sizes, F32, 32, 1e-2), tensors([5000] * 40, F32, 33, 1e-2)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    x1 = x2 = 1.0
+    for k in range(20):
+        opt.step(grads)
+        with torch.cuda.stream(side):
+            other.step(g2)
+        x1, x2 = x1 * 0.9, x2 * 0.999
+        if k % 7 == 3:
+            assert opt._clock[:3].tolist() == [k + 1, x1, x2]
+    torch.cuda.synchronize()
+    for o in (opt, other):
+        assert o._clock[:3].tolist() == [20, x1, x2] and not o._clock[7:].any()
 
 
 def test_types_mixed_in_one_list():

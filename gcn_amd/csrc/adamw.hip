@@ -147,7 +147,8 @@ __global__ __launch_bounds__(TOTAL_THREADS) void norm_one(FewList list, double m
 }
 
 // ---------------------------------------------------------------------------- AdamW
-constexpr long CODED_CHUNK = 2048, DECODE_CHUNK = 4096;
+constexpr long DECODE_CHUNK = 4096;
+constexpr int coded_chunk(bool alone) { return (alone ? 4 : 8) * BLOCK; }
 
 template <int N>
 struct StepList {
@@ -394,7 +395,7 @@ __device__ __forceinline__ float scale_of(float h)
 }
 
 // One wave per block of 256 elements, four to a lane, two blocks in flight (one costs 6 % at 100 M parameters, four
-// 2 %).  Moments, root and step in fp64, so that codes, scales and steps are those of the definition whatever the
+// 2 %; a small step has one, 100 k bf16 parameters in 5.3 us instead of 6.1).  Moments, root and step in fp64, so that codes, scales and steps are those of the definition whatever the
 // order of operations.  101 M bf16 parameters with fp32 master copy (16 bytes each) in 299 us, 5.4 TB/s; the vector
 // units are busy for some 60 % of it (342 operations a block and lane in an earlier form were 75 % and 4 % slower).
 template <typename P, typename G, bool ALONE>
@@ -402,7 +403,7 @@ __global__ __launch_bounds__(256) void adamw_coded(StepList<STEP_TENSORS> list, 
 {
     constexpr bool COPY = sizeof(P) == 2;
     typedef std::conditional_t<COPY, float, P> S;
-    constexpr int U = CODED_CHUNK / (4 * BLOCK);
+    constexpr int U = ALONE ? 1 : 2, CHUNK = coded_chunk(ALONE);
     const int i = find(list, blockIdx.x);
     P *param = (P *)list.param[i];
     const G *grad = (const G *)list.grad[i];
@@ -410,7 +411,7 @@ __global__ __launch_bounds__(256) void adamw_coded(StepList<STEP_TENSORS> list, 
     if constexpr (COPY) held = a.master + list.first[i];
     else held = param;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long n = list.n[i], b0 = (long)(blockIdx.x - list.chunk0[i]) * CODED_CHUNK + wave * (U * BLOCK);
+    const long n = list.n[i], b0 = (long)(blockIdx.x - list.chunk0[i]) * CHUNK + wave * (U * BLOCK);
     const long blk0 = list.block[i] + b0 / BLOCK;
     const double rest1 = 1 - a.beta1, rest2 = 1 - a.beta2;
     Pack<G, 4> gk[U];
@@ -508,8 +509,9 @@ __global__ __launch_bounds__(256) void adamw_decode(StepList<STEP_TENSORS> list,
 // A step of one pair of types is one launch that moves the clock itself.  Of few tensors and up to WIDE_SMALL elements it has
 // one pack a lane and a short argument block: fp32, 47 k in 4.9 us of the device and 1 M in 6.9 (four packs 6.2 and 8.3,
 // the clock in a launch of its own 7.2 and 8.9), 4 M in 21.2 (four packs 20.2).  With 8-bit moments working out the
-// step's rates in every wave pays up to ALONE_CODED: 1 M in 7.2 us instead of 8.0, 4 M 16.4 and 16.0, 100 M 304 and 291.
-constexpr long WIDE_SMALL = 1 << 20, ALONE_CODED = 3 << 20;
+// step's rates in every wave pays up to ALONE_CODED: bf16, 1 M in 7.2 us instead of 8.8, 4.3 M in 18.7 either way, 8 M
+// in 30 instead of 28.5.
+constexpr long WIDE_SMALL = 1 << 20, ALONE_CODED = 5 << 20;
 
 // Hands tensors [0, count) that `take` accepts to `go`, a list at a time, with their chunks counted.
 template <typename List, typename Take, typename Go>
@@ -704,7 +706,7 @@ int ccnn_adamw_step(const ccnn_adamw_tensor_t *tensors, const void *const *grads
                 return 0;
             });
         else
-            e = in_lists<Many>(count, moment_bits == 8 ? CODED_CHUNK : WIDE_THREADS * 16, take, [&](const Many &list) -> int {
+            e = in_lists<Many>(count, moment_bits == 8 ? coded_chunk(args.alone) : WIDE_THREADS * 16, take, [&](const Many &list) -> int {
                 launch(moment_bits == 8 ? "adamw_coded" : "adamw_wide", moment_bits == 32 ? kind.four : args.alone ? kind.coded_alone : kind.coded,
                        dim3((unsigned)list.chunk0[list.count]), dim3(moment_bits == 8 ? 256 : WIDE_THREADS), 0, st, list, args);
                 CCNN_LAUNCH_CHECK();

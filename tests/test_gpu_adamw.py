@@ -258,7 +258,7 @@ def test_sizes_around_the_one_launch_step(kind, sizes):
 
 @pytest.mark.parametrize("bits,sizes", [(32, [1]), (32, [64 * 256]), (32, [64 * 256 + 1]), (32, [33 * 256] * 16), (32, [1 << 20]),
                                         (32, [(1 << 20) - 1]), (32, [9000] * 64), (32, [9000] * 65), (32, [0, 5000, 0]),
-                                        (8, [64 * 2048]), (8, [64 * 2048 + 1]), (8, [(3 << 20) - 1]), (8, [3 << 20]), (8, [777] * 64),
+                                        (8, [64 * 2048]), (8, [64 * 2048 + 1]), (8, [64 * 1024]), (8, [64 * 1024 + 1]), (8, [(5 << 20) - 1]), (8, [5 << 20]), (8, [777] * 64),
                                         (8, [777] * 65)], ids=str)
 def test_the_clock_moves_once_a_step(bits, sizes):
     """Whatever launch moves it: alone, in groups that meet, in front of several; also where other work runs beside it."""

@@ -1,10 +1,12 @@
 """ctypes binding of libccnn_hip.so.  There is no CPU fallback: if the shared
 library is missing the import of any compute entry point fails loudly."""
 import ctypes as C
+import importlib.util
 import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("CCNN_LIB_PATH") or os.path.join(_HERE, "lib", "libccnn_hip.so")
+CALLS_PATH = os.path.join(_HERE, "lib", "ccnn_torch_calls.so")
 
 FILTERS, COV_LEN, STRIDE, POOL_LEN, HIDDEN, CLASSES, PER_LAYER, FILTER_SIZE = 20, 19, 2, 2, 100, 13, 9, 171
 
@@ -142,6 +144,27 @@ def load():
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+_calls = None
+# what the module beside the library calls, in the order of its bind()
+_CALLED = ("ccnn_log_probs_workspace_bytes", "ccnn_log_probs", "ccnn_log_probs_grad", "ccnn_grad_norm_workspace_bytes",
+           "ccnn_grad_norm", "ccnn_adamw_step")
+
+
+def calls():
+    """The module with the host side of the scoring and optimiser calls (torch_calls.cpp), bound to the library."""
+    global _calls
+    if _calls is None:
+        lib = load()
+        if not os.path.exists(CALLS_PATH):
+            raise ImportError(f"{CALLS_PATH} not found: build it with `python -c 'import __graft_entry__ as g; g.build()'`.")
+        spec = importlib.util.spec_from_file_location("ccnn_torch_calls", CALLS_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.bind(*[C.cast(getattr(lib, name), C.c_void_p).value for name in _CALLED])
+        _calls = module
+    return _calls
 
 
 def error_string(code):

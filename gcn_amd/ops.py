@@ -380,46 +380,36 @@ def _same_device(t, name, device):
         raise ValueError(f"{name} is on {t.device}, expected {device}")
 
 
-def _at(t):
-    return t.data_ptr() if t is not None else None
-
-
 _T = torch.Tensor
 
 
-def _one_device(tensors, name, dtypes):
-    """The device that all the contiguous tensors are on."""
-    try:
-        if len(set(map(_T.get_device, tensors))) == 1 and all(map(_T.is_contiguous, tensors)) and tensors[0].is_cuda \
-                and all(t.dtype in dtypes for t in tensors):
-            return tensors[0].device
-    except (TypeError, RuntimeError):
-        pass
-    for i, t in enumerate(tensors):      # something is wrong: say what
+def _refuse_list(tensors, name, dtypes):
+    """Says what is wrong with a list that has to be contiguous tensors on one device."""
+    for i, t in enumerate(tensors):
         _on_device(t, f"{name} {i}", dtypes)
         _same_device(t, f"{name} {i}", tensors[0].device)
         if not t.is_contiguous():
             raise ValueError(f"{name} {i} must be contiguous")
-    raise TypeError(f"{name} list cannot be used")
 
 
-_CALLS = {}
 _raw_stream, _current = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
-def _enqueue(index, name, *args):
-    """Calls a library function with device `index` current and that device's current stream as its last
-    argument.  Addresses go as plain numbers: the host side of a small call is most of it."""
-    fn = _CALLS.get(name)
-    if fn is None:
-        fn = _CALLS[name] = getattr(_l.load(), name)
+def _called(name, like, *args):
+    """What the module beside the library gives for `name`, with like's device current and that device's current
+    stream.  None: an argument is not what it has to be."""
+    index = like.get_device() if isinstance(like, _T) else -1
+    if index < 0:
+        return None
+    call = getattr(_l.calls(), name)
     if index == _current():
-        rc = fn(*args, _raw_stream(index))
+        got = call(_raw_stream(index), index, *args)
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, _raw_stream(index))
-    if rc:
-        _l.check(rc, name)
+            got = call(_raw_stream(index), index, *args)
+    if type(got) is int:
+        _l.check(got, f"ccnn_{name}")
+    return got
 
 
 class LogProbs(NamedTuple):
@@ -432,29 +422,53 @@ class LogProbs(NamedTuple):
 
 
 def _rows(t, name):
-    """(rows, columns, elements from row to row) of a matrix whose rows are contiguous and do not overlap."""
-    shape, stride = t.shape, t.stride()
-    if len(shape) != 2 or shape[1] < 1:
-        raise ValueError(f"{name} must be [rows, classes] with at least one class, got {list(shape)}")
-    rows, classes = shape
-    if classes > 1 and stride[1] != 1:
+    """(rows, columns) of a matrix whose rows are contiguous and do not overlap."""
+    if t.dim() != 2 or t.shape[1] < 1:
+        raise ValueError(f"{name} must be [rows, classes] with at least one class, got {list(t.shape)}")
+    rows, classes = t.shape
+    if classes > 1 and t.stride(1) != 1:
         raise ValueError(f"{name} must be contiguous along its classes")
-    step = stride[0] if rows > 1 else classes
-    if step < classes:
+    if rows > 1 and t.stride(0) < classes:
         raise ValueError(f"rows of {name} overlap")
-    return rows, classes, step
+    return rows, classes
 
 
-def _target_bytes(targets, rows, device):
-    if not (isinstance(targets, _T) and targets.dtype in _TARGET_BYTES and targets.device == device and targets.shape == (rows,)
-            and targets.is_contiguous()):
-        _on_device(targets, "targets", _TARGET_BYTES)
-        _same_device(targets, "targets", device)
+def _refuse_scored(logits, targets):
+    _on_device(logits, "logits", _TYPES)
+    rows, classes = _rows(logits, "logits")
+    _on_device(targets, "targets", (torch.int32, torch.int64))
+    _same_device(targets, "targets", logits.device)
+    if targets.shape != (rows,) or not targets.is_contiguous():
         raise ValueError(f"targets must be contiguous [{rows}], got {list(targets.shape)}")
-    return _TARGET_BYTES[targets.dtype]
+    return rows, classes
 
 
-_TARGET_BYTES = {torch.int32: 4, torch.int64: 8}
+def _refuse_log_probs(logits, targets, top):
+    _, classes = _refuse_scored(logits, targets)
+    if not 0 <= top <= min(_l.MAX_TOP, classes):
+        raise ValueError(f"top must be between 0 and {min(_l.MAX_TOP, classes)}, got {top}")
+    raise ValueError("logits cannot be used")
+
+
+def _refuse_log_probs_grad(logits, targets, scored, d_logp, d_entropy, out):
+    rows, _ = _refuse_scored(logits, targets)
+    dev, wide = logits.device, _F64 if logits.dtype == _F64 else _F32
+    if d_logp is None and d_entropy is None:
+        raise ValueError("neither d_logp nor d_entropy given")
+    if d_entropy is not None and scored.entropy is None:
+        raise ValueError("d_entropy needs a log_probs call with want_entropy")
+    for t, name, n in ((scored.stats, "stats", 4 * rows), (d_logp, "d_logp", rows), (d_entropy, "d_entropy", rows)):
+        if t is not None:
+            _req(t, wide, name, n)
+            _same_device(t, name, dev)
+    if out is not None:
+        _on_device(out, "out", (logits.dtype,))
+        _same_device(out, "out", dev)
+        if out.shape != logits.shape:
+            raise ValueError(f"out is {list(out.shape)}, the logits are {list(logits.shape)}")
+        _rows(out, "out")
+        raise ValueError("out overlaps the logits without being them")
+    raise ValueError("logits cannot be used")
 
 
 def log_probs(logits, targets, top=0, want_entropy=True):
@@ -464,64 +478,21 @@ def log_probs(logits, targets, top=0, want_entropy=True):
     of their indices.  -> LogProbs; no autograd history, see log_probs_grad.  A negative target gives 0, one of `classes` or more NaN.  -inf
     logits are classes that are not allowed; a row of nothing else has log probabilities of -inf and
     entropy 0, a row with a NaN or +inf has NaN everywhere and top_index -1."""
-    _on_device(logits, "logits", _TYPES)
-    rows, classes, stride = _rows(logits, "logits")
-    dev = logits.device
-    target_bytes = _target_bytes(targets, rows, dev)
     top = int(top)
-    if top and not 0 < top <= min(_l.MAX_TOP, classes):
-        raise ValueError(f"top must be between 0 and {min(_l.MAX_TOP, classes)}, got {top}")
-    kind = _TYPES[logits.dtype]
-    wide = _F64 if kind == _l.TYPE_F64 else _F32
-    stats = torch.empty((4, rows), dtype=wide, device=dev)
-    logp, entropy, _, _ = stats.unbind(0)
-    top_logp = top_index = ws = None
-    if top:
-        top_logp = torch.empty((rows, top), dtype=wide, device=dev)
-        top_index = torch.empty((rows, top), dtype=torch.int32, device=dev)
-    if rows:
-        nbytes = _l.load().ccnn_log_probs_workspace_bytes(rows, classes, top, kind)
-        if nbytes:
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        _enqueue(dev.index, "ccnn_log_probs", logits.data_ptr(), kind, rows, classes, stride, targets.data_ptr(), target_bytes,
-                 top, bool(want_entropy), stats.data_ptr(), _at(top_logp), _at(top_index), _at(ws), nbytes)
-    return LogProbs(logp, entropy if want_entropy else None, top_logp, top_index, stats)
+    got = _called("log_probs", logits, logits, targets, top, bool(want_entropy))
+    if got is None:
+        _refuse_log_probs(logits, targets, top)
+    return LogProbs(*got)
 
 
 def log_probs_grad(logits, targets, scored, d_logp=None, d_entropy=None, out=None):
     """Gradient of sum(d_logp * logp) + sum(d_entropy * entropy) to the logits, from what log_probs
     returned for them.  d_logp / d_entropy: [rows] of the type of scored.logp, one of them at least.
     out: [rows, classes] of the logits' type (rows may be strided), the logits themselves allowed."""
-    _on_device(logits, "logits", _TYPES)
-    rows, classes, stride = _rows(logits, "logits")
-    dev, wide = logits.device, _F64 if logits.dtype == _F64 else _F32
-    target_bytes = _target_bytes(targets, rows, dev)
-    if d_logp is None and d_entropy is None:
-        raise ValueError("neither d_logp nor d_entropy given")
-    if d_entropy is not None and scored.entropy is None:
-        raise ValueError("d_entropy needs a log_probs call with want_entropy")
-    for t, name, n in ((scored.stats, "stats", 4 * rows), (d_logp, "d_logp", rows), (d_entropy, "d_entropy", rows)):
-        if t is not None and not (isinstance(t, _T) and t.dtype == wide and t.device == dev and t.is_contiguous() and t.numel() == n):
-            _req(t, wide, name, n)
-            _same_device(t, name, dev)
-    given, out_stride = out is not None, classes
-    if given:
-        _on_device(out, "out", (logits.dtype,))
-        _same_device(out, "out", dev)
-        if out.shape != logits.shape:
-            raise ValueError(f"out is {list(out.shape)}, the logits are {list(logits.shape)}")
-        _, _, out_stride = _rows(out, "out")
-    else:
-        out = torch.empty((rows, classes), dtype=logits.dtype, device=dev)
-    if rows:
-        size = logits.element_size()
-        a, b = logits.data_ptr(), out.data_ptr()
-        if given and (a, stride) != (b, out_stride) and a < b + ((rows - 1) * out_stride + classes) * size \
-                and b < a + ((rows - 1) * stride + classes) * size:
-            raise ValueError("out overlaps the logits without being them")
-        _enqueue(dev.index, "ccnn_log_probs_grad", a, _TYPES[logits.dtype], rows, classes, stride, targets.data_ptr(),
-                 target_bytes, scored.stats.data_ptr(), _at(d_logp), _at(d_entropy), b, out_stride)
-    return out
+    got = _called("log_probs_grad", logits, logits, targets, scored.stats, scored.entropy, d_logp, d_entropy, out)
+    if got is None:
+        _refuse_log_probs_grad(logits, targets, scored, d_logp, d_entropy, out)
+    return got
 
 
 def grad_norm(grads, max_norm=float("inf")):
@@ -531,17 +502,14 @@ def grad_norm(grads, max_norm=float("inf")):
     grads = list(grads)
     if not grads:
         raise ValueError("grad_norm needs at least one tensor")
-    if not max_norm > 0:
-        raise ValueError(f"max_norm must be positive, got {max_norm}")
-    count, dev = len(grads), _one_device(grads, "gradient", _TYPES)
-    at = (C.c_void_p * count)(*map(_T.data_ptr, grads))
-    n = (C.c_long * count)(*map(_T.numel, grads))
-    kinds = (C.c_int * count)(*[_TYPES[g.dtype] for g in grads])
-    out = torch.empty(2, dtype=_F64, device=dev)
-    nbytes = _l.load().ccnn_grad_norm_workspace_bytes(n, count)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _enqueue(dev.index, "ccnn_grad_norm", at, n, kinds, count, float(max_norm), out.data_ptr(), _at(ws), nbytes)
-    return out
+    max_norm = float(max_norm)
+    got = _called("grad_norm", grads[0], grads, max_norm)
+    if got is None:
+        if not max_norm > 0:
+            raise ValueError(f"max_norm must be positive, got {max_norm}")
+        _refuse_list(grads, "gradient", _TYPES)
+        raise ValueError("the gradients cannot be used")
+    return got
 
 
 class AdamW:
@@ -600,10 +568,7 @@ class AdamW:
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise ValueError("parameter tensors overlap")
         self.numel, self.blocks = first, block
-        # what each gradient is held against, and the types' table for the usual case that they are the parameters'
-        self._numels, self._dtypes = [p.numel() for p in self.params], [p.dtype for p in self.params]
-        self._places = [p.data_ptr() for p in self.params]
-        self._kinds = (C.c_int * n)(*[t.type for t in self._table])
+        self._table_at = C.addressof(self._table)
         wide = _F64 if self.params[0].dtype == _F64 else _F32
         if state_bits == 32:
             self.m, self.v = (torch.zeros(first, dtype=wide, device=self.device) for _ in range(2))
@@ -614,7 +579,7 @@ class AdamW:
         self.master = None
         if any(p.element_size() == 2 for p in self.params):
             flat = [p.detach().reshape(-1) for p in self.params]
-            same = len(set(self._dtypes)) == 1
+            same = len({p.dtype for p in self.params}) == 1
             self.master = torch.cat(flat).float() if same else torch.cat([p.float() for p in flat])
         self._clock = torch.zeros(_l.ADAMW_CLOCK, dtype=_F64, device=self.device)
         self._set_step(0)
@@ -639,35 +604,28 @@ class AdamW:
         """One step from `grads`, one contiguous tensor per parameter with its size, of its type (or fp32
         for bf16 / fp16).  lr: instead of self.lr.  clip: grad_norm's result; its factor scales every
         gradient, and a factor that is not finite leaves everything as it is, the step count too."""
-        grads, kinds, dev = list(grads), self._kinds, self.device
-        count = len(self.params)
-        if len(grads) != count:
-            raise ValueError(f"{len(grads)} gradients for {count} parameters")
-        if list(map(_T.data_ptr, self.params)) != self._places:
+        grads, lr = list(grads), self.lr if lr is None else lr
+        got = _called("adamw_step", self.params[0], self.params, grads, self._table_at, self.state_bits, self.m, self.v,
+                      self.m_scale, self.v_scale, self.master, self._clock, lr, self.betas[0], self.betas[1], self.eps, clip)
+        if got is None:
+            self._refuse_step(grads, lr, clip)
+
+    def _refuse_step(self, grads, lr, clip):
+        if len(grads) != len(self.params):
+            raise ValueError(f"{len(grads)} gradients for {len(self.params)} parameters")
+        if any(p.data_ptr() != (t.param or 0) for p, t in zip(self.params, self._table)):
             raise ValueError("a parameter's memory is not what it was when the optimiser was made")
-        if _one_device(grads, "gradient", _TYPES) != dev:
-            raise ValueError(f"gradients are on {grads[0].device}, the parameters on {dev}")
-        if list(map(_T.numel, grads)) != self._numels:
-            i = [g.numel() == n for g, n in zip(grads, self._numels)].index(False)
-            raise ValueError(f"gradient {i} has {grads[i].numel()} elements, its parameter {self._numels[i]}")
-        dtypes = [g.dtype for g in grads]
-        if dtypes != self._dtypes:
-            for i, (g, dtype) in enumerate(zip(grads, self._dtypes)):
-                _on_device(g, f"gradient {i}", (dtype, _F32) if dtype.itemsize == 2 else (dtype,))
-            kinds = (C.c_int * count)(*[_TYPES[d] for d in dtypes])
-        at = (C.c_void_p * count)(*map(_T.data_ptr, grads))
-        if clip is not None:
-            _req(clip, _F64, "clip", 2)
-            _same_device(clip, "clip", self.device)
-        lr = self.lr if lr is None else lr
-        lr_device = None
-        if isinstance(lr, torch.Tensor):
-            _req(lr, _F64, "lr", 1)
-            _same_device(lr, "lr", self.device)
-            lr, lr_device = 0.0, lr
-        _enqueue(dev.index, "ccnn_adamw_step", self._table, at, kinds, count, self.state_bits, self.m.data_ptr(),
-                 self.v.data_ptr(), _at(self.m_scale), _at(self.v_scale), _at(self.master), self._clock.data_ptr(), float(lr),
-                 _at(lr_device), self.betas[0], self.betas[1], self.eps, _at(clip))
+        _refuse_list(grads, "gradient", _TYPES)
+        for i, (g, p) in enumerate(zip(grads, self.params)):
+            _same_device(g, f"gradient {i}", self.device)
+            if g.numel() != p.numel():
+                raise ValueError(f"gradient {i} has {g.numel()} elements, its parameter {p.numel()}")
+            _on_device(g, f"gradient {i}", (p.dtype, _F32) if p.element_size() == 2 else (p.dtype,))
+        for t, name, n in ((clip, "clip", 2), (lr if isinstance(lr, torch.Tensor) else None, "lr", 1)):
+            if t is not None:
+                _req(t, _F64, name, n)
+                _same_device(t, name, self.device)
+        raise ValueError("the gradients cannot be used")
 
     def moments(self):
         """(m, v), flat in the order of the parameters: the optimiser's own tensors with 32 bits, the values
@@ -675,8 +633,9 @@ class AdamW:
         if self.state_bits == 32:
             return self.m, self.v
         m, v = (torch.empty(self.numel, dtype=_F32, device=self.device) for _ in range(2))
-        _enqueue(self.device.index, "ccnn_adamw_moments", self._table, len(self.params), self.m.data_ptr(), self.v.data_ptr(),
-                 self.m_scale.data_ptr(), self.v_scale.data_ptr(), m.data_ptr(), v.data_ptr())
+        with torch.cuda.device(self.device):
+            _l.check(_l.load().ccnn_adamw_moments(self._table, len(self.params), _ptr(self.m), _ptr(self.v), _ptr(self.m_scale),
+                                                  _ptr(self.v_scale), _ptr(m), _ptr(v), _stream()), "ccnn_adamw_moments")
         return m, v
 
     def state_dict(self):

@@ -21,4 +21,8 @@ for s in $SRCS; do
 done
 for p in "${pids[@]}"; do wait "$p"; done
 $HIPCC --offload-arch=gfx950 -shared -fPIC -o "$ROOT/gcn_amd/lib/libccnn_hip.so" $(for s in $SRCS; do echo "$OBJ/${s%.*}.o"; done)
+C="$ROOT/gcn_amd/lib/ccnn_torch_calls.so"
+if [ "$CSRC/torch_calls.cpp" -nt "$C" ] || [ "$ROOT/include/ccnn.h" -nt "$C" ]; then
+    (cd "$ROOT" && python3 -c 'import __graft_entry__ as g; g.build_calls()')
+fi
 echo "built $ROOT/gcn_amd/lib/libccnn_hip.so"

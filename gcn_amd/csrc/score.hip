@@ -121,15 +121,29 @@ template <typename A> struct KeyOf { typedef unsigned long long type; };
 template <> struct KeyOf<double> { typedef unsigned __int128 type; };
 template <typename A> using Key = typename KeyOf<A>::type;
 
-__device__ __forceinline__ unsigned long long key_of(float v, unsigned i)
+// A number's order as a signed whole number, above its lowest value.
+__device__ __forceinline__ int order_of(float v)
 {
     const int u = __float_as_int(v + 0.0f);
-    return (unsigned long long)(unsigned)(u ^ ((u >> 31) | (int)0x80000000)) << 32 | (unsigned)~i;
+    return u ^ ((u >> 31) & 0x7fffffff);
 }
-__device__ __forceinline__ unsigned __int128 key_of(double v, unsigned i)
+__device__ __forceinline__ long long order_of(double v)
 {
     const long long u = __double_as_longlong(v + 0.0);
-    return (unsigned __int128)(unsigned long long)(u ^ ((u >> 63) | (long long)0x8000000000000000ull)) << 32 | (unsigned)~i;
+    return u ^ ((u >> 63) & 0x7fffffffffffffffll);
+}
+__device__ __forceinline__ unsigned long long order_key(int order, unsigned i)
+{
+    return (unsigned long long)((unsigned)order ^ 0x80000000u) << 32 | (unsigned)~i;
+}
+__device__ __forceinline__ unsigned __int128 order_key(long long order, unsigned i)
+{
+    return (unsigned __int128)((unsigned long long)order ^ 0x8000000000000000ull) << 32 | (unsigned)~i;
+}
+template <typename A>
+__device__ __forceinline__ Key<A> key_of(A v, unsigned i)
+{
+    return order_key(order_of(v), i);
 }
 __device__ __forceinline__ unsigned key_index(unsigned long long k) { return ~(unsigned)k; }
 __device__ __forceinline__ unsigned key_index(unsigned __int128 k) { return ~(unsigned)k; }
@@ -157,7 +171,7 @@ __device__ __forceinline__ void put_top(const ScoreOut<A> &o, long r, int place,
 // by value, the largest left, all elements that equal it placed in the order of their classes and struck out.
 // With several rows to a wave: one by one, the lane whose best was taken looking for its next - what one row needs
 // all rows of the wave wait for, and equal values of one row would be looked for in all (20000 x 1000 bf16, 20
-// alternatives: 54 us the first way, 101 the second; 207400 x 13 fp32, 3 alternatives: 11.7 and 8.7).
+// alternatives: 54 us the first way, 101 the second; 207400 x 13 fp32, 3 alternatives: 11.7 and 8.1).
 template <typename T, int G, int E>
 __global__ __launch_bounds__(256) void log_probs_small(const T *__restrict__ logits, long rows, int classes, long stride,
                                                        Targets targets, ScoreOut<Wide<T>> o)
@@ -227,22 +241,29 @@ __global__ __launch_bounds__(256) void log_probs_small(const T *__restrict__ log
             }
         }
     } else {
-        unsigned taken = 0;
-        auto next = [&]() {                     // the first of the lane's largest elements not taken yet
-            A v = ninf(A());
-            int at = -1;
+        typedef decltype(order_of(A())) Order;
+        const Order gone = sizeof(Order) == 4 ? (Order)0x80000000u : (Order)0x8000000000000000ull;     // below every number
+        Order left[E];
 #pragma unroll
-            for (int e = 0; e < E; e++)
-                if (!(taken >> e & 1) && place_of(e) < classes && (at < 0 || x[e] > v)) v = x[e], at = e;
-            return at < 0 ? Key<A>(0) : key_of(v, place_of(at));
+        for (int e = 0; e < E; e++) left[e] = place_of(e) < classes ? order_of(x[e]) : gone;
+        Key<A> best;
+        int at;
+        auto next = [&]() {                     // the first of the lane's largest elements not taken yet
+            Order v = left[0];
+            at = 0;
+#pragma unroll
+            for (int e = 1; e < E; e++)
+                if (left[e] > v) v = left[e], at = e;
+            best = order_key(v, place_of(at));
         };
-        Key<A> best = next();
+        next();
         for (int k = 0; k < o.top; k++) {
             const Key<A> high = lanes_max<G>(best);
             if (lane == 0) put_top(o, r, k, key_value(high), (int)key_index(high), m, l);
             if (best == high && k + 1 < o.top) {
-                taken |= 1u << (key_index(high) / (G * W) * W + key_index(high) % W);
-                best = next();
+#pragma unroll
+                for (int e = 0; e < E; e++) left[e] = e == at ? gone : left[e];
+                next();
             }
         }
     }
@@ -658,9 +679,9 @@ int score_impl(const void *logits, long rows, int classes, long stride, Targets 
     if (classes <= SMALL_CLASSES) {
         typedef void (*Kern)(const T *, long, int, long, Targets, ScoreOut<A>);
         // Few lanes to a row while there are rows enough for the device, more where latency counts: 100000 x 50
-        // bf16 with 5 alternatives takes 15.7 us with 8 lanes, 34.5 with 32, 1000 x 50 takes 5.7 and 3.8;
-        // 50000 x 250 takes 26.5 us with 16, 31.7 with 64, 1000 x 250 (20 alternatives) 20.5 and 6.9.
-        const bool many = rows >= 16384;
+        // bf16 with 5 alternatives takes 13.8 us with 8 lanes, 30 with 32, 8000 x 50 4.8 and 5.2, 1000 x 50 5.0 and
+        // 3.9; 100000 x 250 takes 37.6 us with 16, 68.7 with 64, 8000 x 250 7.0 and 8.6, 1000 x 250 6.9 and 4.4.
+        const bool many = rows >= 8192;
         const int group = classes <= 16 ? 2 : classes <= 64 ? (many ? 8 : 32) : classes <= 256 ? (many ? 16 : 64) : 64;
         const Kern kern = classes <= 16    ? log_probs_small<T, 2, 8>
                           : classes <= 64  ? (many ? log_probs_small<T, 8, 8> : log_probs_small<T, 32, 2>)

@@ -1,0 +1,60 @@
+"""CPU: the module between torch tensors and the library answers None to what it cannot take, before anything of the
+library is called, and ops says what it was."""
+import ctypes as C
+
+import pytest
+import torch
+
+from gcn_amd import lib as L
+from gcn_amd import ops
+
+
+@pytest.fixture(scope="module")
+def calls():
+    return L.calls()
+
+
+def test_tensors_in_host_memory_are_not_taken(calls):
+    x, y, d = torch.zeros(4, 13), torch.zeros(4, dtype=torch.int32), torch.zeros(4)
+    table = (L.AdamwTensor * 1)((d.data_ptr(), 4, 0, 0, 0.0, L.TYPE_F32))
+    for device in (0, -1, 7):
+        assert calls.log_probs(0, device, x, y, 0, True) is None
+        assert calls.log_probs_grad(0, device, x, y, torch.zeros(4, 4), d, d, None, None) is None
+        assert calls.grad_norm(0, device, [d], 1.0) is None
+        assert calls.adamw_step(0, device, [d], [d], C.addressof(table), 32, d, d, None, None, None, d, 1e-3, 0.9, 0.999,
+                                1e-8, None) is None
+
+
+def test_what_is_not_a_tensor_is_not_taken(calls):
+    for odd in (None, 3, "x", [1.0], object()):
+        assert calls.log_probs(0, 0, odd, odd, 0, True) is None
+        assert calls.log_probs_grad(0, 0, odd, odd, odd, odd, odd, odd, odd) is None
+        assert calls.grad_norm(0, 0, odd, 1.0) is None
+        assert calls.grad_norm(0, 0, [odd], 1.0) is None
+        assert calls.adamw_step(0, 0, odd, odd, 0, 32, odd, odd, odd, odd, odd, odd, 1e-3, 0.9, 0.999, 1e-8, odd) is None
+        assert calls.adamw_step(0, 0, [odd], [odd], 0, 32, odd, odd, odd, odd, odd, odd, 1e-3, 0.9, 0.999, 1e-8, odd) is None
+    assert calls.grad_norm(0, 0, [], 1.0) is None
+
+
+def test_arguments_are_counted_and_numbers_are_numbers(calls):
+    x, y = torch.zeros(4, 13), torch.zeros(4, dtype=torch.int32)
+    for name in ("bind", "log_probs", "log_probs_grad", "grad_norm", "adamw_step"):
+        with pytest.raises(TypeError):
+            getattr(calls, name)(1)
+    with pytest.raises(TypeError):
+        calls.log_probs(0, 0, x, y, "many", True)
+    with pytest.raises(TypeError):
+        calls.grad_norm(0, 0, [x], "much")
+
+
+def test_ops_says_what_is_wrong():
+    x, y = torch.zeros(4, 13), torch.zeros(4, dtype=torch.int32)
+    scored = ops.LogProbs(x[:, 0], x[:, 0], None, None, torch.zeros(4, 4))
+    for call in (lambda: ops.log_probs(x, y), lambda: ops.log_probs(None, y), lambda: ops.log_probs_grad(x, y, scored, x[:, 0]),
+                 lambda: ops.grad_norm([x]), lambda: ops.grad_norm([3]), lambda: ops.AdamW([x])):
+        with pytest.raises(TypeError, match="must be a CUDA tensor"):
+            call()
+    with pytest.raises(ValueError, match="at least one"):
+        ops.grad_norm([])
+    with pytest.raises(ValueError, match="max_norm"):
+        ops.grad_norm([x], -1.0)

@@ -145,6 +145,8 @@ __device__ __forceinline__ Key<A> key_of(A v, unsigned i)
 {
     return order_key(order_of(v), i);
 }
+__device__ __forceinline__ unsigned key_high(unsigned long long k) { return (unsigned)(k >> 32); }
+__device__ __forceinline__ unsigned long long key_high(unsigned __int128 k) { return (unsigned long long)(k >> 32); }
 __device__ __forceinline__ unsigned key_index(unsigned long long k) { return ~(unsigned)k; }
 __device__ __forceinline__ unsigned key_index(unsigned __int128 k) { return ~(unsigned)k; }
 __device__ __forceinline__ float key_value(unsigned long long k)
@@ -292,7 +294,8 @@ struct SliceOut {
 template <typename A, int NT>
 struct SliceLds {
     static constexpr int MOST = NT == 64 ? 512 : 1024;    // candidates: 64 alternatives are expected to bring 300
-    Key<A> key[NT];
+    Key<A> key[64];                         // largest of each group of NT / 64 threads
+    decltype(key_high(Key<A>())) high[64];
     Key<A> found[MOST];
     A m[NT / 64], s[NT / 64], t[NT / 64];
     Key<A> bar;
@@ -300,21 +303,32 @@ struct SliceLds {
     int n_owners, n_found;
 };
 
-// k-th largest (k >= 1) of the wave's 64 keys; equal keys count one by one.
-template <typename K>
-__device__ __forceinline__ K wave_kth(K mine, int k, K *lds)
+// k-th largest (k >= 1) of the wave's 64 keys, 0 if fewer are not 0.  Ranked by the values alone, a compare and an add
+// each; of the lanes that share the k-th value the one whose index comes next is looked for then.
+template <typename K, typename H>
+__device__ __forceinline__ K wave_kth(K mine, int k, H *lds)
 {
     const int lane = threadIdx.x & 63;
-    lds[lane] = mine;
+    const H high = key_high(mine);
+    lds[lane] = high;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
     __builtin_amdgcn_wave_barrier();
     int rank = 0;
-    for (int j = 0; j < 64; j++) {
-        const K w = lds[j];
-        rank += w > mine || (w == mine && j < lane);
+#pragma unroll
+    for (int j = 0; j < 64; j++) rank += lds[j] > high;
+    unsigned long long same = 0;
+    int r = k;
+    while (!same) same = __ballot(rank == --r);         // rank 0 is there
+    const unsigned index = key_index(mine);
+    for (unsigned long long left = same; left; left &= left - 1) {
+        const int one = __ffsll(left) - 1;
+        const unsigned at = __builtin_amdgcn_readlane(index, one);
+        if (__popcll(same & __ballot(index < at)) == k - 1 - r) {
+            const H value = lds[one];
+            return value == 0 ? K(0) : (K)value << 32 | (unsigned)~at;
+        }
     }
-    const unsigned long long at = __ballot(rank == k - 1);
-    return lds[__ffsll((unsigned long long)at) - 1];
+    return K(0);
 }
 
 // The first `top` of n keys in LDS, handed to put(place, key) in falling order.
@@ -426,7 +440,10 @@ __global__ __launch_bounds__(NT) void log_probs_slice(const T *__restrict__ logi
     shift(sums, best);
     sums = over_wave(sums);
     if (lane == 0) lds.m[wave] = sums.m, lds.s[wave] = sums.s, lds.t[wave] = sums.t;
-    if (o.top) lds.key[tid] = best_at < 0 ? Key<A>(0) : key_of(best, best_at);
+    if (o.top) {
+        const Key<A> group = lanes_max<NT / 64>(best_at < 0 ? Key<A>(0) : key_of(best, best_at));
+        if (tid % (NT / 64) == 0) lds.key[tid / (NT / 64)] = group;
+    }
     if (tid == 0) lds.n_owners = lds.n_found = 0;
     __syncthreads();
     A all = lds.m[0];
@@ -451,9 +468,7 @@ __global__ __launch_bounds__(NT) void log_probs_slice(const T *__restrict__ logi
         else put_top(o, r, place, key_value(k), (int)key_index(k), sums.m, l);
     };
     if (wave == 0) {
-        Key<A> high = lds.key[lane];
-        for (int w = 1; w < NT / 64; w++) high = lds.key[w * 64 + lane] > high ? lds.key[w * 64 + lane] : high;
-        const Key<A> bar = wave_kth(high, o.top, lds.found);
+        const Key<A> bar = wave_kth(lds.key[lane], o.top, lds.high);
         if (lane == 0) lds.bar = bar;
     }
     __syncthreads();
@@ -497,7 +512,8 @@ __global__ __launch_bounds__(256) void log_probs_join(const T *__restrict__ logi
                                                       ScoreOut<Wide<T>> o, SliceOut<Wide<T>> part)
 {
     typedef Wide<T> A;
-    __shared__ Key<A> keys[JOIN_KEYS], found[CANDIDATES], high_of[64];
+    __shared__ Key<A> keys[JOIN_KEYS], found[CANDIDATES], high_of[4];
+    __shared__ decltype(key_high(Key<A>())) order[64];
     __shared__ Key<A> bar;
     __shared__ int n_found;
     const long r = blockIdx.x;
@@ -526,7 +542,7 @@ __global__ __launch_bounds__(256) void log_probs_join(const T *__restrict__ logi
     if (tid < 64) {
         Key<A> high = 0;
         for (int k = lane; k < n; k += 64) high = keys[k] > high ? keys[k] : high;
-        const Key<A> b = n < 64 ? Key<A>(0) : wave_kth(high, o.top, high_of);
+        const Key<A> b = n < 64 ? Key<A>(0) : wave_kth(high, o.top, order);
         if (lane == 0) bar = b;
     }
     __syncthreads();

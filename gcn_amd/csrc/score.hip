@@ -279,7 +279,8 @@ __global__ __launch_bounds__(256) void log_probs_small(const T *__restrict__ log
 // Without entropy and alternatives the memory bounds it: 4096 x 128000 bf16 in 167 us, 6.3 TB/s.  With both it is the
 // vector units (10.5 operations an element and an exponential that counts for four): 2048 x 128000 bf16 in 101 us;
 // x L - c in one multiply-add in place of (x - m) L changes nothing there and costs short rows 8 %.
-// One row of 128000 takes 7.4 us in slices and 5.5 to join them, most of it the four waits of the selection.
+// One row of 128000 with 20 alternatives takes 11.4 us, half of it to join the slices; of 61 x 50251 fp16 the alternatives
+// are a third of 9.9 us: the bar, what reaches it read again, its order.
 constexpr int SLICE_THREADS = 512;   // or 64: see wave_rows
 constexpr int CANDIDATES = 1024;      // of the joining workgroup
 
@@ -650,14 +651,18 @@ constexpr int PACKED_CLASSES = 1024;    // gradient: 16 bytes a thread up to her
                                         // 126 and 90 us; 200000 x 200: 43 us, a wave to a row took 96)
 constexpr long ROWS_AT_ONCE = 1 << 24, SLICED_AT_ONCE = 1 << 22;   // 64 or 512 threads each stay below a launch's 2^32
 
-// A wave to a row, in place of a workgroup, for short rows if there are enough of them: 100000 x 1025 bf16 takes 68 us
-// instead of 303, 16384 x 16384 93 instead of 116, 1024 x 4096 5.1 instead of 6.1; 3001 x 32003 fp32 with 5
-// alternatives would take 100 instead of 73.
-inline bool wave_rows(long rows, int classes) { return rows >= 512 && classes <= 16384; }
+// A wave to a row, in place of a workgroup, for short rows if there are enough of them, the more the longer they are: 100000 x
+// 1025 bf16 takes 68 us instead of 303, 16384 x 16384 94 instead of 115, 1024 x 4096 with 5 alternatives 7.2 instead of 9.4,
+// 1024 x 8192 9.6 instead of 10.4; 512 x 8192 would take 9.3 instead of 7.9, 1024 x 16384 15.4 instead of 12.5, and of fp32
+// 1024 x 8192 12.3 instead of 10.3, 3001 x 32003 100 instead of 73.
+inline bool wave_rows(long rows, int classes, int size)
+{
+    return rows >= 512 && classes <= 16384 && (long)classes * size <= 16 * rows;
+}
 
 // Slices of a row: one up to UNSPLIT classes, where a workgroup ends with the row before a second launch could join
-// slices (one row of 50000 bf16 with 20 alternatives: 10.3 us whole, 12.0 in slices; of 128000: 17.0 and 12.7;
-// 61 rows of 50251 fp16: 13.1 and 14.5).  Beyond, enough of them to give every CU two workgroups, none shorter
+// slices (one row of 50000 bf16 with 20 alternatives: 9.4 us whole, 10.7 in slices; of 65536: 10.2 and 11.0;
+// 61 rows of 50251 fp16: 9.9 and 12.8).  Beyond, enough of them to give every CU two workgroups, none shorter
 // than a load per thread, and their lists short enough for the LDS of the workgroup that joins them.
 constexpr int UNSPLIT = 65536;
 
@@ -719,7 +724,7 @@ int score_impl(const void *logits, long rows, int classes, long stride, Targets 
         part.sums = c.take<Sums<A>>(rows * part.slices);
         part.keys = c.take<Key<A>>(rows * part.slices * (size_t)top);
     }
-    const bool waves = wave_rows(rows, classes);
+    const bool waves = wave_rows(rows, classes, sizeof(T));
     const auto kern = waves ? (want_entropy ? log_probs_slice<T, true, 64> : log_probs_slice<T, false, 64>)
                             : (want_entropy ? log_probs_slice<T, true, SLICE_THREADS> : log_probs_slice<T, false, SLICE_THREADS>);
     const int threads = waves ? 64 : SLICE_THREADS;

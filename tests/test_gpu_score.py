@@ -88,7 +88,7 @@ def weights(rows, kind, seed=1):
 
 
 SHAPES = [(1, 1), (1, 2), (3, 13), (257, 13), (5, 16), (7, 17), (130, 31), (4, 64), (3, 65), (9, 255), (2, 1000), (5, 1024),
-          (16385, 13), (16400, 41), (16390, 200), (20000, 5), (3, 1025), (2, 2049), (3, 4097), (1, 32003), (4, 50251), (520, 1025), (513, 1037), (600, 8190), (3, 65536), (2, 65537), (1, 128000), (2, 131073), (70, 8191), (600, 70001)]
+          (16385, 13), (16400, 41), (16390, 200), (20000, 5), (3, 1025), (2, 2049), (3, 4097), (1, 32003), (4, 50251), (520, 1025), (513, 1037), (600, 8190), (3, 65536), (2, 65537), (1, 128000), (2, 131073), (70, 8191), (600, 70001), (2050, 8190)]
 
 
 @pytest.mark.parametrize("kind", KINDS, ids=str)
@@ -163,7 +163,7 @@ def test_masked_and_odd_values(classes, kind):
 
 
 @pytest.mark.parametrize("kind", KINDS, ids=str)
-@pytest.mark.parametrize("classes,times", [(13, 1400), (50, 1400), (200, 1400), (1500, 45), (9001, 43)])
+@pytest.mark.parametrize("classes,times", [(13, 1400), (50, 1400), (200, 1400), (1500, 45), (9001, 43), (4096, 90)])
 def test_masked_and_odd_values_in_many_rows(classes, times, kind):
     """The row counts from which other shapes of the kernels take over."""
     x, y = odd_rows(classes, kind)
@@ -221,7 +221,7 @@ def test_ties_and_clustered_alternatives(classes, kind):
 
 
 @pytest.mark.parametrize("kind", KINDS, ids=str)
-@pytest.mark.parametrize("classes,times", [(16, 1640), (50, 1640), (200, 1640), (1025, 52), (4096, 52), (16384, 52)])
+@pytest.mark.parametrize("classes,times", [(16, 1640), (50, 1640), (200, 1640), (1025, 52), (4096, 52), (16384, 52), (4096, 105)])
 def test_ties_and_clustered_alternatives_in_many_rows(classes, times, kind):
     top = min(64, classes)
     x, y = clustered_rows(classes, top)

@@ -295,7 +295,7 @@ struct SliceOut {
 template <typename A, int NT>
 struct SliceLds {
     static constexpr int MOST = NT == 64 ? 512 : 1024;    // candidates: 64 alternatives are expected to bring 300
-    Key<A> key[64];                         // largest of each group of NT / 64 threads
+    Key<A> key[NT];
     decltype(key_high(Key<A>())) high[64];
     Key<A> found[MOST];
     A m[NT / 64], s[NT / 64], t[NT / 64];
@@ -441,10 +441,7 @@ __global__ __launch_bounds__(NT) void log_probs_slice(const T *__restrict__ logi
     shift(sums, best);
     sums = over_wave(sums);
     if (lane == 0) lds.m[wave] = sums.m, lds.s[wave] = sums.s, lds.t[wave] = sums.t;
-    if (o.top) {
-        const Key<A> group = lanes_max<NT / 64>(best_at < 0 ? Key<A>(0) : key_of(best, best_at));
-        if (tid % (NT / 64) == 0) lds.key[tid / (NT / 64)] = group;
-    }
+    if (o.top) lds.key[tid] = best_at < 0 ? Key<A>(0) : key_of(best, best_at);
     if (tid == 0) lds.n_owners = lds.n_found = 0;
     __syncthreads();
     A all = lds.m[0];
@@ -469,7 +466,11 @@ __global__ __launch_bounds__(NT) void log_probs_slice(const T *__restrict__ logi
         else put_top(o, r, place, key_value(k), (int)key_index(k), sums.m, l);
     };
     if (wave == 0) {
-        const Key<A> bar = wave_kth(lds.key[lane], o.top, lds.high);
+        // groups of every 64th thread: what lies together in the row, as in one that is in order, is in different ones
+        Key<A> high = lds.key[lane];
+#pragma unroll
+        for (int w = 1; w < NT / 64; w++) high = lds.key[w * 64 + lane] > high ? lds.key[w * 64 + lane] : high;
+        const Key<A> bar = wave_kth(high, o.top, lds.high);
         if (lane == 0) lds.bar = bar;
     }
     __syncthreads();

@@ -283,6 +283,10 @@ __global__ __launch_bounds__(256) void log_probs_small(const T *__restrict__ log
 // are a third of 9.9 us: the bar, what reaches it read again, its order.
 constexpr int SLICE_THREADS = 512;   // or 64: see wave_rows
 constexpr int CANDIDATES = 1024;      // of the joining workgroup
+// The bar is the k-th of the groups up to here: 52 of them are expected to bring 107 elements, enough for the most
+// alternatives, and all 64 some 300 or, now and then, far more (2000 x 4096 bf16 with 64: 422 us).  Where it brings too few, k
+// is used after all.
+constexpr int BAR_RANK = 52;
 
 template <typename A>
 struct SliceOut {
@@ -294,7 +298,7 @@ struct SliceOut {
 
 template <typename A, int NT>
 struct SliceLds {
-    static constexpr int MOST = NT == 64 ? 512 : 1024;    // candidates: 64 alternatives are expected to bring 300
+    static constexpr int MOST = NT == 64 ? 512 : 1024;    // candidates
     Key<A> key[NT];
     decltype(key_high(Key<A>())) high[64];
     Key<A> found[MOST];
@@ -465,39 +469,44 @@ __global__ __launch_bounds__(NT) void log_probs_slice(const T *__restrict__ logi
         if (part.sums) part.keys[(r * part.slices + slice) * o.top + place] = k;
         else put_top(o, r, place, key_value(k), (int)key_index(k), sums.m, l);
     };
-    if (wave == 0) {
-        // groups of every 64th thread: what lies together in the row, as in one that is in order, is in different ones
-        Key<A> high = lds.key[lane];
-#pragma unroll
-        for (int w = 1; w < NT / 64; w++) high = lds.key[w * 64 + lane] > high ? lds.key[w * 64 + lane] : high;
-        const Key<A> bar = wave_kth(high, o.top, lds.high);
-        if (lane == 0) lds.bar = bar;
-    }
-    __syncthreads();
-    const Key<A> bar = lds.bar;
-    if (best_at >= 0 && key_of(best, best_at) >= bar) lds.owners[atomicAdd(&lds.n_owners, 1)] = tid;
-    __syncthreads();
     const int turns = (loads + (rest > 0) + NT - 1) / NT;
-    for (int task = tid; task < lds.n_owners * turns; task += NT) {
-        const int at = lds.owners[task / turns] + (task % turns) * NT;
-        const int count = at < loads ? W : at == loads ? rest : 0;
-        Pack<T, W> p;
-        if (count == W) p = load_pack<W>(row + (long)at * W);
-        else {
+    for (int rank = min(o.top, BAR_RANK);; rank = o.top) {
+        if (wave == 0) {
+            // groups of every 64th thread: what lies together in the row, as in one that is in order, is in different ones
+            Key<A> high = lds.key[lane];
 #pragma unroll
-            for (int e = 0; e < W; e++)
-                if (e < count) p.v[e] = row[(long)at * W + e];
+            for (int w = 1; w < NT / 64; w++) high = lds.key[w * 64 + lane] > high ? lds.key[w * 64 + lane] : high;
+            const Key<A> bar = wave_kth(high, rank, lds.high);
+            if (lane == 0) lds.bar = bar;
         }
+        __syncthreads();
+        const Key<A> bar = lds.bar;
+        if (best_at >= 0 && key_of(best, best_at) >= bar) lds.owners[atomicAdd(&lds.n_owners, 1)] = tid;
+        __syncthreads();
+        for (int task = tid; task < lds.n_owners * turns; task += NT) {
+            const int at = lds.owners[task / turns] + (task % turns) * NT;
+            const int count = at < loads ? W : at == loads ? rest : 0;
+            Pack<T, W> p;
+            if (count == W) p = load_pack<W>(row + (long)at * W);
+            else {
 #pragma unroll
-        for (int e = 0; e < W; e++) {
-            const A x = widen(p.v[e]);
-            if (e < count && key_of(x, at) >= bar) {
-                const int place = atomicAdd(&lds.n_found, 1);
-                if (place < MOST) lds.found[place] = key_of(x, (unsigned)(begin + (long)at * W + e));
+                for (int e = 0; e < W; e++)
+                    if (e < count) p.v[e] = row[(long)at * W + e];
+            }
+#pragma unroll
+            for (int e = 0; e < W; e++) {
+                const A x = widen(p.v[e]);
+                if (e < count && key_of(x, at) >= bar) {
+                    const int place = atomicAdd(&lds.n_found, 1);
+                    if (place < MOST) lds.found[place] = key_of(x, (unsigned)(begin + (long)at * W + e));
+                }
             }
         }
+        __syncthreads();
+        if (lds.n_found >= o.top || rank == o.top) break;
+        __syncthreads();
+        if (tid == 0) lds.n_owners = lds.n_found = 0;
     }
-    __syncthreads();
     if (lds.n_found <= MOST) {
         in_order(lds.found, lds.n_found, o.top, put);
         if (part.sums)     // a last slice shorter than the list: nothing behind its elements
@@ -514,13 +523,13 @@ __global__ __launch_bounds__(256) void log_probs_join(const T *__restrict__ logi
                                                       ScoreOut<Wide<T>> o, SliceOut<Wide<T>> part)
 {
     typedef Wide<T> A;
-    __shared__ Key<A> keys[JOIN_KEYS], found[CANDIDATES], high_of[4];
+    __shared__ Key<A> keys[JOIN_KEYS + CCNN_MAX_TOP], found[CANDIDATES], high_of[4];
     __shared__ decltype(key_high(Key<A>())) order[64];
     __shared__ Key<A> bar;
     __shared__ int n_found;
     const long r = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63;
-    const int n = part.slices * o.top;
+    const int pitch = part.slices | 1, n = pitch * o.top;
     long y = -1;
     A given = A(0);
     if (tid == 0) {
@@ -528,10 +537,11 @@ __global__ __launch_bounds__(256) void log_probs_join(const T *__restrict__ logi
         if (y >= 0 && y < classes) given = widen(logits[r * stride + y]);
         n_found = 0;
     }
+    // Place by place of all slices, an odd number to a place: among groups of every 64th key both a row's first
+    // alternatives and those of one slice, which may be all, are in different ones.
     for (int k = tid; k < n; k += 256) {
-        // place by place of all slices, so that groups of every 64th key share a row's first alternatives
-        // unevenly only if few slices hold them all
-        keys[k % o.top * part.slices + k / o.top] = part.keys[r * n + k];
+        const int place = k / pitch, slice = k - place * pitch;
+        keys[k] = slice < part.slices ? part.keys[(r * part.slices + slice) * o.top + place] : Key<A>(0);
     }
     const Sums<A> *in = part.sums + r * part.slices;
     Sums<A> sums = {ninf(A()), A(0), A(0)};

@@ -228,6 +228,21 @@ def test_ties_and_clustered_alternatives_in_many_rows(classes, times, kind):
     check_scores(x.to(kind).cuda().repeat(times, 1), y.cuda().repeat(times), top)
 
 
+@pytest.mark.parametrize("kind", KINDS, ids=str)
+@pytest.mark.parametrize("rows,classes", [(3, 1025), (3, 4096), (1100, 4096), (3, 20000), (2, 128000)])
+@pytest.mark.parametrize("count", [1, 40, 51, 52, 53, 60, 63, 64, 65])
+def test_few_large_values_each_in_a_load_of_its_own(rows, classes, kind, count):
+    """With 64 alternatives: as many groups hold large values, one each, as there are, and the rest of the row is equal."""
+    if rows > 3 and kind == torch.float64:
+        rows = 2100
+    x = torch.zeros(rows, classes, dtype=torch.float64)
+    width = 128 // torch.finfo(kind).bits
+    at = torch.randperm(min(classes // width, 512), generator=torch.Generator().manual_seed(count))[:count] * width
+    x[:, at] = 2.0 + torch.arange(count, dtype=torch.float64) / 64
+    x[0, at] = 2.0
+    check_scores(x.to(kind).cuda(), torch.zeros(rows, dtype=torch.int64, device="cuda"), 64)
+
+
 SIGNALLING = {torch.float32: (torch.int32, 0x7f800001), torch.float64: (torch.int64, 0x7ff0000000000001),
               torch.bfloat16: (torch.int16, 0x7f81), torch.float16: (torch.int16, 0x7c01)}
 

@@ -108,8 +108,10 @@ __global__ __launch_bounds__(TOTAL_THREADS) void norm_total(const double *__rest
 }
 
 // Few gradients, of any types: one workgroup for all of them, each of its waves taking every 16th piece, in place of two
-// launches and a workspace (47 k fp32 gradients: 5.2 us).
-constexpr long PIECE = 2048, ONE_PIECES = 64;
+// launches and a workspace.  Its one CU's fp64 conversions and sums bound it: 47 k fp32 gradients take 5.1 us of the device
+// and 5.0 a call (two launches: 5.8 and 8.2), 80 k 6.7 and 6.6 (6.0 and 8.2), 130 k 9.5 and 9.4 (6.0 and 8.0).  Pieces of
+// 1024 are 3 % slower at 47 k, of 512 17 %.
+constexpr long PIECE = 2048, ONE_PIECES = 40;
 
 struct FewList : NormList<FEW_TENSORS> {
     int type[FEW_TENSORS];

@@ -302,7 +302,7 @@ def test_types_mixed_in_one_list():
 
 
 @pytest.mark.parametrize("kind", [F32, F64, BF16, F16], ids=str)
-@pytest.mark.parametrize("sizes", [[1], [0, 5], [16384], [16385, 3, 100000], [3000001]])
+@pytest.mark.parametrize("sizes", [[1], [0, 5], [16384], [16385, 3, 100000], [3000001], [81920], [81921], [5121] * 16, [100] * 17])
 def test_norm(kind, sizes):
     grads = tensors(sizes, kind, 9, 2.0)
     want = float(torch.cat([g.cpu().double() for g in grads]).norm())

@@ -465,6 +465,11 @@ __global__ __launch_bounds__(NT) void log_probs_slice(const T *__restrict__ logi
     }
     if (!o.top) return;
     const A l = sums.m == ninf(A()) && sums.s == A(0) ? ninf(A()) : logw(sums.s);
+    if (l != l) {      // a NaN is no number's largest, so what follows may find nothing
+        if (!part.sums)                                     // else the row's join says so, from the sums
+            for (int place = tid; place < o.top; place += NT) put_top(o, r, place, sums.m, -1, sums.m, l);
+        return;
+    }
     auto put = [&](int place, Key<A> k) {
         if (part.sums) part.keys[(r * part.slices + slice) * o.top + place] = k;
         else put_top(o, r, place, key_value(k), (int)key_index(k), sums.m, l);
@@ -550,6 +555,10 @@ __global__ __launch_bounds__(256) void log_probs_join(const T *__restrict__ logi
     if (tid == 0) finish_row(sums, r, given, y, classes, o);
     if (!o.top) return;
     const A l = sums.m == ninf(A()) && sums.s == A(0) ? ninf(A()) : logw(sums.s);
+    if (l != l) {      // of the slices that hold it there are no keys
+        for (int place = tid; place < o.top; place += 256) put_top(o, r, place, sums.m, -1, sums.m, l);
+        return;
+    }
     __syncthreads();
     if (tid < 64) {
         Key<A> high = 0;

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import wide_ref as ref
+from gcn_amd import lib as L
 from gcn_amd import ops
 
 pytestmark = pytest.mark.gpu
@@ -420,3 +421,41 @@ def test_empty_and_refused():
     x64, _ = problem(70, 70, torch.float32)
     with pytest.raises(ValueError):
         ops.log_probs(x64, torch.zeros(70, dtype=torch.int32, device="cuda"), top=65)
+
+
+def scored_into(x, y, top, fill):
+    """ccnn_log_probs into results that hold `fill` before -> (logp, entropy, top_logp, top_index)."""
+    rows, classes = x.shape
+    stats, top_logp = (torch.full((n, rows), fill, dtype=wide(x.dtype), device="cuda") for n in (4, top))
+    index = torch.full((rows, top), int(fill), dtype=torch.int32, device="cuda")
+    kind = ops._TYPES[x.dtype]
+    need = L.load().ccnn_log_probs_workspace_bytes(rows, classes, top, kind)
+    ws = torch.full((need + 1,), 7, dtype=torch.uint8, device="cuda")
+    L.check(L.load().ccnn_log_probs(x.data_ptr(), kind, rows, classes, classes, y.data_ptr(), 4, top, 1, stats.data_ptr(),
+                                    top_logp.data_ptr(), index.data_ptr(), ws.data_ptr() if need else None, need,
+                                    torch.cuda.current_stream().cuda_stream), "ccnn_log_probs")
+    return stats[0], stats[1], top_logp.view(rows, top), index
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=str)
+@pytest.mark.parametrize("rows,classes", [(6, 13), (6, 700), (6, 1025), (6, 1030), (6, 2047), (6, 4095), (6, 40001), (6, 70003), (600, 1025),
+                                          (600, 4095)])
+@pytest.mark.parametrize("top", [1, 2, 13])
+def test_rows_of_negative_nans_have_no_alternatives(rows, classes, kind, top):
+    """A NaN with its sign bit set orders below -inf, so no element may reach the bar; every place says so, whatever
+    the memory held before."""
+    x, y = problem(rows, classes, kind, seed=12)
+    x = x.contiguous()
+    bits = {2: torch.int16, 4: torch.int32, 8: torch.int64}[x.element_size()]
+    part = classes % (16 // x.element_size()) or 1
+    x.view(bits)[0::6] = -1
+    x.view(bits)[1::6, classes - part:] = -1           # all of the last, partial load
+    x.view(bits)[2::6, 1:] = -1
+    x[3::6] = math.nan
+    x[4::6, classes - 1] = INF
+    logp, entropy, top_logp, index = scored_into(x, y, top, 5.0)
+    bad = torch.arange(rows, device="cuda") % 6 != 5
+    assert torch.isnan(logp[bad]).all() and torch.isnan(entropy[bad]).all()
+    assert (index[bad] == -1).all() and torch.isnan(top_logp[bad]).all()
+    want = ref.log_probs(x[~bad], y[~bad], top)
+    assert torch.equal(index[~bad].cpu(), want["top_index"]) and torch.isfinite(logp[~bad]).all()

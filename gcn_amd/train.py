@@ -124,9 +124,10 @@ def fit_mbgd(params, cubes, onehot, z, batch=100, lr=None, min_err=None, max_ite
     mean is taken over its own size (hyper_version_MBGD.cu:780, 794-796) instead of being
     dropped (gcn_mbgd_fp64.cu:895).
     optimizer: an ops.AdamW over views of `params` (train.adamw makes one) that takes the steps instead of the
-    trainers' own rule, from the gradient summed over the batch (and the ranks); lr is then its own unless
-    given, and falls by the same schedule.  max_norm: the norm the batch's mean gradient is clipped to; a step
-    whose norm is not finite is left out.
+    trainers' own rule, from the gradient summed over the batch (and the ranks; keep_tail's short last batch as
+    `batch` times its mean, so that it weighs as much in the moments); lr is then its own unless given, and
+    falls by the same schedule.  max_norm: the norm the batch's mean gradient is clipped to; a step whose norm
+    is not finite is left out.
     """
     f32 = params.dtype == torch.float32
     if max_norm is not None and optimizer is None:
@@ -173,10 +174,10 @@ def fit_mbgd(params, cubes, onehot, z, batch=100, lr=None, min_err=None, max_ite
         for i0, (first, nb) in enumerate(steps):
             if optimizer is not None:
                 g = comm.all_reduce(st.grad(first, nb, loss_d[i0]))
+                if nb != sub_b:
+                    g = g * (batch / nb)                     # a short batch's mean, as a sum over `batch` like the others
                 grads = [g[a:b] for a, b in places]
-                clip = None
-                if max_norm is not None:
-                    clip = ops.grad_norm(grads, max_norm * (batch if nb == sub_b else nb))
+                clip = ops.grad_norm(grads, max_norm * batch) if max_norm is not None else None
                 optimizer.step(grads, lr=lr, clip=clip)
             elif comm.world == 1 and stepper is None:
                 st.step_fused(first, nb, lr, loss_d[i0])

@@ -162,3 +162,34 @@ def test_training_with_adamw_runs_end_to_end():
     assert len(hist.loss) == 3 and np.isfinite(hist.loss).all()
     r = train.score(got["params"], got["test_cubes"], got["test_labels"], z)
     assert torch.isfinite(r.logp).all() and torch.isfinite(r.entropy).all()
+
+
+@pytest.mark.parametrize("dtype,bits", [(np.float32, 32), (np.float32, 8), (np.float64, 32)])
+@pytest.mark.parametrize("max_norm", [None, 1e-3])
+def test_the_short_last_batch_weighs_as_much_as_the_others(dtype, bits, max_norm):
+    """keep_tail: a batch of ten after four of 25 enters the moments as its mean does beside theirs."""
+    params, cubes, onehot, geom = network(dtype, n=110)
+    start = params.clone()
+    d, B, lr, epochs = L.dims(geom), 25, 1e-3, 2
+    opt = train.adamw(params, geom, lr=lr, weight_decay=0.1, state_bits=bits)
+    train.fit_mbgd(params, cubes, onehot, geom, batch=B, min_err=0.0, max_iter=epochs, optimizer=opt, max_norm=max_norm,
+                   keep_tail=True)
+    assert opt.step_count == epochs * 5
+    p, keep = start.clone(), [0, 2, 3, 4, 5] if dtype == np.float32 else list(range(6))
+    views = [ops.param_views(p, geom)[i] for i in keep]
+    want = ref.AdamW(views, lr, decays=[[0.1, 0.0] * 3][0] if len(keep) == 6 else [0.1, 0.1, 0.0, 0.1, 0.0], bits=bits)
+    for _ in range(epochs):
+        for first, nb in [(0, 25), (25, 25), (50, 25), (75, 25), (100, 10)]:
+            g, _ = ops.mbgd_grad(p, cubes, onehot, first, nb, geom)
+            grads = [ops.param_views(g, geom)[i].cpu().double() * (B / nb) for i in keep]
+            scale = 1.0
+            if max_norm is not None:
+                scale = min(1.0, max_norm * B / float(torch.cat(grads).norm()))
+            want.step(grads, scale=scale)
+            for v, w in zip(views, want.p):
+                v.copy_(w.to(p.dtype))
+            want.p = [v.cpu().double() for v in views]
+    # as for whole batches: a step moves a parameter by at most 40 lr, rounding stays far below 1e-3 of it in fp32 and
+    # 1e-10 in fp64, a code on the other side of a border is an eighth of its moment
+    tol = 40 * lr * ({32: 1e-3, 8: 0.02}[bits] if dtype == np.float32 else 1e-10)
+    assert (params - p).abs().max().item() <= tol

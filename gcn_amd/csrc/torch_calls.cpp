@@ -134,13 +134,10 @@ PyObject *log_probs(PyObject *, PyObject *const *a, Py_ssize_t n)
     }
     PyObject *out = PyTuple_New(5);
     if (!out) return nullptr;
-    Py_INCREF(Py_None);
-    Py_INCREF(Py_None);
-    Py_INCREF(Py_None);
     PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(stats.select(0, 0)));
-    PyTuple_SET_ITEM(out, 1, want_entropy ? THPVariable_Wrap(stats.select(0, 1)) : Py_None);
-    PyTuple_SET_ITEM(out, 2, top ? THPVariable_Wrap(top_logp) : Py_None);
-    PyTuple_SET_ITEM(out, 3, top ? THPVariable_Wrap(top_index) : Py_None);
+    PyTuple_SET_ITEM(out, 1, want_entropy ? THPVariable_Wrap(stats.select(0, 1)) : none());
+    PyTuple_SET_ITEM(out, 2, top ? THPVariable_Wrap(top_logp) : none());
+    PyTuple_SET_ITEM(out, 3, top ? THPVariable_Wrap(top_index) : none());
     PyTuple_SET_ITEM(out, 4, THPVariable_Wrap(stats));
     return out;
     END_HANDLE_TH_ERRORS

@@ -1,6 +1,7 @@
 """GPU: log_probs and log_probs_grad against their 64-bit restatement, at the sizes, strides, masks and
 values where they can go wrong."""
 import math
+import sys
 
 import pytest
 import torch
@@ -459,3 +460,14 @@ def test_rows_of_negative_nans_have_no_alternatives(rows, classes, kind, top):
     assert (index[bad] == -1).all() and torch.isnan(top_logp[bad]).all()
     want = ref.log_probs(x[~bad], y[~bad], top)
     assert torch.equal(index[~bad].cpu(), want["top_index"]) and torch.isfinite(logp[~bad]).all()
+
+
+def test_calls_keep_no_references_to_none():
+    """An absent result is one reference to None, given back with the result."""
+    x, y = problem(4, 13, torch.float32)
+    for top, want_entropy in [(0, False), (0, True), (2, False), (2, True)]:
+        ops.log_probs(x, y, top=top, want_entropy=want_entropy)
+        before = sys.getrefcount(None)
+        for _ in range(1000):
+            ops.log_probs(x, y, top=top, want_entropy=want_entropy)
+        assert abs(sys.getrefcount(None) - before) < 100, (top, want_entropy)

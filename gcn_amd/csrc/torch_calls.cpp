@@ -235,27 +235,41 @@ PyObject *grad_norm(PyObject *, PyObject *const *a, Py_ssize_t n)
     END_HANDLE_TH_ERRORS
 }
 
+// The bytes of an object that has them (a ctypes array), none of any other.
+struct Bytes {
+    Py_buffer view = {};
+    explicit Bytes(PyObject *o)
+    {
+        if (PyObject_CheckBuffer(o) && PyObject_GetBuffer(o, &view, PyBUF_SIMPLE)) PyErr_Clear(), view = {};
+    }
+    ~Bytes() { PyBuffer_Release(&view); }
+    Bytes(const Bytes &) = delete;
+};
+
 // adamw_step(stream, device, params, grads, table, bits, m, v, m_scale, v_scale, master, clock, lr, beta1, beta2, eps, clip)
-// -> 0.  params: still where the table (ccnn_adamw_tensor_t) has them; the state's tensors are the optimiser's own.
+// -> 0.  table: an array of ccnn_adamw_tensor_t, one for each parameter, which is still what it says; the state's tensors
+// are the optimiser's own.
 PyObject *adamw_step(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
     HANDLE_TH_ERRORS
     if (!count_is(n, 17)) return nullptr;
     void *stream = address(a[0]);
     const long device = PyLong_AsLong(a[1]);
-    const auto *table = (const ccnn_adamw_tensor_t *)address(a[4]);
     const long bits = PyLong_AsLong(a[5]);
     const double beta1 = PyFloat_AsDouble(a[13]), beta2 = PyFloat_AsDouble(a[14]), eps = PyFloat_AsDouble(a[15]);
     if (PyErr_Occurred()) return nullptr;
+    const Bytes held(a[4]);
+    const auto *table = (const ccnn_adamw_tensor_t *)held.view.buf;
     List g;
     if (!PyList_Check(a[2]) || !list_of(a[3], device, &g) || (Py_ssize_t)g.n.size() != PyList_GET_SIZE(a[2])) return none();
     const int count = (int)g.n.size();
+    if (held.view.len != (Py_ssize_t)(count * sizeof *table)) return none();
     for (int i = 0; i < count; i++) {
         const at::Tensor *p = tensor(PyList_GET_ITEM(a[2], i), device);
         const ccnn_adamw_tensor_t &t = table[i];
         const bool half = t.type == CCNN_TYPE_BF16 || t.type == CCNN_TYPE_F16;
-        if (!p || p->const_data_ptr() != t.param || g.n[i] != t.n || (g.types[i] != t.type && !(half && g.types[i] == CCNN_TYPE_F32)))
-            return none();
+        if (!p || p->const_data_ptr() != t.param || p->numel() != t.n || type_of(*p) != t.type) return none();
+        if (g.n[i] != t.n || (g.types[i] != t.type && !(half && g.types[i] == CCNN_TYPE_F32))) return none();
     }
     void *state[6];
     for (int i = 0; i < 6; i++) {

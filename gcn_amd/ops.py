@@ -568,7 +568,6 @@ class AdamW:
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise ValueError("parameter tensors overlap")
         self.numel, self.blocks = first, block
-        self._table_at = C.addressof(self._table)
         wide = _F64 if self.params[0].dtype == _F64 else _F32
         if state_bits == 32:
             self.m, self.v = (torch.zeros(first, dtype=wide, device=self.device) for _ in range(2))
@@ -605,16 +604,20 @@ class AdamW:
         for bf16 / fp16).  lr: instead of self.lr.  clip: grad_norm's result; its factor scales every
         gradient, and a factor that is not finite leaves everything as it is, the step count too."""
         grads, lr = list(grads), self.lr if lr is None else lr
-        got = _called("adamw_step", self.params[0], self.params, grads, self._table_at, self.state_bits, self.m, self.v,
+        got = _called("adamw_step", self._clock, self.params, grads, self._table, self.state_bits, self.m, self.v,
                       self.m_scale, self.v_scale, self.master, self._clock, lr, self.betas[0], self.betas[1], self.eps, clip)
         if got is None:
             self._refuse_step(grads, lr, clip)
 
     def _refuse_step(self, grads, lr, clip):
+        if not isinstance(self.params, list) or len(self.params) != len(self._table):
+            raise ValueError(f"params must be the list of the {len(self._table)} parameters that the optimiser was made for")
         if len(grads) != len(self.params):
             raise ValueError(f"{len(grads)} gradients for {len(self.params)} parameters")
-        if any(p.data_ptr() != (t.param or 0) for p, t in zip(self.params, self._table)):
-            raise ValueError("a parameter's memory is not what it was when the optimiser was made")
+        for i, (p, t) in enumerate(zip(self.params, self._table)):
+            _on_device(p, f"parameter {i}", _TYPES)
+            if (p.data_ptr(), p.numel(), _TYPES[p.dtype]) != (t.param or 0, t.n, t.type):
+                raise ValueError(f"parameter {i} is not what or where it was when the optimiser was made")
         _refuse_list(grads, "gradient", _TYPES)
         for i, (g, p) in enumerate(zip(grads, self.params)):
             _same_device(g, f"gradient {i}", self.device)
@@ -634,7 +637,7 @@ class AdamW:
             return self.m, self.v
         m, v = (torch.empty(self.numel, dtype=_F32, device=self.device) for _ in range(2))
         with torch.cuda.device(self.device):
-            _l.check(_l.load().ccnn_adamw_moments(self._table, len(self.params), _ptr(self.m), _ptr(self.v), _ptr(self.m_scale),
+            _l.check(_l.load().ccnn_adamw_moments(self._table, len(self._table), _ptr(self.m), _ptr(self.v), _ptr(self.m_scale),
                                                   _ptr(self.v_scale), _ptr(m), _ptr(v), _stream()), "ccnn_adamw_moments")
         return m, v
 

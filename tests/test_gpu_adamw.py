@@ -462,3 +462,37 @@ def test_refused():
     moved.data = torch.zeros(10, device="cuda")           # the memory the optimiser knew is gone
     with pytest.raises(ValueError):
         other.step([g])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_parameters_are_those_that_the_optimiser_was_made_for(bits):
+    """The list, the memory, the size and the type are looked at before a step; what is read out does not hang on the list."""
+    p, g = torch.zeros(512, device="cuda"), torch.full((512,), 0.5, device="cuda")
+    more = torch.zeros(512, device="cuda")
+    opt = ops.AdamW([p], state_bits=bits)
+    opt.step([g])
+    m, v = opt.moments()
+    for change, back in [(lambda: opt.params.append(more), lambda: opt.params.pop()),
+                         (lambda: opt.params.extend([more] * 200), lambda: opt.params.__delitem__(slice(1, None))),
+                         (lambda: opt.params.clear(), lambda: opt.params.append(p)),
+                         (lambda: setattr(opt, "params", (p,)), lambda: setattr(opt, "params", [p]))]:
+        change()
+        for grads in ([g], [g] * len(opt.params), [g] * 2):
+            with pytest.raises(ValueError):
+                opt.step(grads)
+        assert all(torch.equal(a, b) for a, b in zip(opt.moments(), (m, v)))
+        back()
+    whole = p.data
+    for other in (whole[:500], whole.view(torch.bfloat16), whole.view(torch.bfloat16)[:512], whole.view(torch.int32)):
+        p.data = other
+        for grads in ([g], [g[:500]], [g.bfloat16()]):
+            with pytest.raises((ValueError, TypeError)):
+                opt.step(grads)
+        p.data = whole
+    opt.params[0] = None
+    with pytest.raises(TypeError):
+        opt.step([g])
+    opt.params[0] = p
+    assert opt.step_count == 1 and not more.any()
+    opt.step([g])
+    assert opt.step_count == 2

@@ -58,3 +58,13 @@ def test_ops_says_what_is_wrong():
         ops.grad_norm([])
     with pytest.raises(ValueError, match="max_norm"):
         ops.grad_norm([x], -1.0)
+
+
+def test_the_table_of_a_step_is_an_array_with_a_length(calls):
+    """Its entries are looked at up to its own length, which has to be that of the lists."""
+    d = torch.zeros(4)
+    table = (L.AdamwTensor * 1)((d.data_ptr(), 4, 0, 0, 0.0, L.TYPE_F32))
+    for count in (1, 2, 500):
+        for odd in (table, bytes(table), memoryview(b"")[::1], b"", "x", None, 3.5, 1 << 70, [table]):
+            assert calls.adamw_step(0, 0, [d] * count, [d] * count, odd, 32, d, d, None, None, None, d, 1e-3, 0.9, 0.999,
+                                    1e-8, None) is None

@@ -247,8 +247,8 @@ struct Bytes {
 };
 
 // adamw_step(stream, device, params, grads, table, bits, m, v, m_scale, v_scale, master, clock, lr, beta1, beta2, eps, clip)
-// -> 0.  table: an array of ccnn_adamw_tensor_t, one for each parameter, which is still what it says; the state's tensors
-// are the optimiser's own.
+// -> 0.  table: an array of ccnn_adamw_tensor_t, one for each parameter, which is still what it says, with their places
+// one after the other; the state's tensors hold what it counts.
 PyObject *adamw_step(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
     HANDLE_TH_ERRORS
@@ -264,21 +264,28 @@ PyObject *adamw_step(PyObject *, PyObject *const *a, Py_ssize_t n)
     if (!PyList_Check(a[2]) || !list_of(a[3], device, &g) || (Py_ssize_t)g.n.size() != PyList_GET_SIZE(a[2])) return none();
     const int count = (int)g.n.size();
     if (held.view.len != (Py_ssize_t)(count * sizeof *table)) return none();
+    long elements = 0, blocks = 0;
+    bool any_half = false;
     for (int i = 0; i < count; i++) {
         const at::Tensor *p = tensor(PyList_GET_ITEM(a[2], i), device);
         const ccnn_adamw_tensor_t &t = table[i];
         const bool half = t.type == CCNN_TYPE_BF16 || t.type == CCNN_TYPE_F16;
         if (!p || p->const_data_ptr() != t.param || p->numel() != t.n || type_of(*p) != t.type) return none();
         if (g.n[i] != t.n || (g.types[i] != t.type && !(half && g.types[i] == CCNN_TYPE_F32))) return none();
+        elements += t.n;
+        blocks += (t.n + CCNN_MOMENT_BLOCK - 1) / CCNN_MOMENT_BLOCK;
+        any_half |= half;
     }
+    const bool coded = bits == 8;
+    const auto moments = coded ? at::kByte : table[0].type == CCNN_TYPE_F64 ? at::kDouble : at::kFloat;
+    const long held_moments = coded ? blocks * CCNN_MOMENT_BLOCK : elements;
     void *state[6];
-    for (int i = 0; i < 6; i++) {
-        state[i] = nullptr;
-        if (a[6 + i] == Py_None) continue;
-        const at::Tensor *t = tensor(a[6 + i], device);
-        if (!t) return none();
-        state[i] = t->data_ptr();
-    }
+    if (!plain(a[6], device, moments, held_moments, &state[0]) || !plain(a[7], device, moments, held_moments, &state[1])
+        || !plain(a[8], device, at::kFloat, blocks, &state[2]) || !plain(a[9], device, at::kFloat, blocks, &state[3])
+        || !plain(a[10], device, at::kFloat, elements, &state[4]) || !plain(a[11], device, at::kDouble, CCNN_ADAMW_CLOCK, &state[5])
+        || a[6] == Py_None || a[7] == Py_None || a[11] == Py_None || (a[8] == Py_None) == coded || (a[9] == Py_None) == coded
+        || (a[10] == Py_None) == any_half)
+        return none();
     double lr = 0;
     void *lr_device = nullptr, *clip;
     if (THPVariable_Check(a[12])) {

@@ -624,17 +624,33 @@ class AdamW:
             if g.numel() != p.numel():
                 raise ValueError(f"gradient {i} has {g.numel()} elements, its parameter {p.numel()}")
             _on_device(g, f"gradient {i}", (p.dtype, _F32) if p.element_size() == 2 else (p.dtype,))
+        self._refuse_state()
         for t, name, n in ((clip, "clip", 2), (lr if isinstance(lr, torch.Tensor) else None, "lr", 1)):
             if t is not None:
                 _req(t, _F64, name, n)
                 _same_device(t, name, self.device)
-        raise ValueError("the gradients cannot be used")
+        raise ValueError("the gradients or the optimiser's state cannot be used")
+
+    def _refuse_state(self):
+        """Raises unless the state's tensors are what the optimiser made them."""
+        types, n = {t.type for t in self._table}, self.numel
+        wide = _F64 if _l.TYPE_F64 in types else _F32
+        want = [("m", wide, n), ("v", wide, n)]
+        if self.state_bits == 8:
+            codes = self.blocks * _l.MOMENT_BLOCK
+            want = [("m", torch.uint8, codes), ("v", torch.uint8, codes), ("m_scale", _F32, self.blocks), ("v_scale", _F32, self.blocks)]
+        if types & {_l.TYPE_BF16, _l.TYPE_F16}:
+            want.append(("master", _F32, n))
+        for k, dtype, size in want:
+            _req(getattr(self, k), dtype, k, size)
+            _same_device(getattr(self, k), k, self.device)
 
     def moments(self):
         """(m, v), flat in the order of the parameters: the optimiser's own tensors with 32 bits, the values
         the codes stand for (fp32) with 8."""
         if self.state_bits == 32:
             return self.m, self.v
+        self._refuse_state()
         m, v = (torch.empty(self.numel, dtype=_F32, device=self.device) for _ in range(2))
         with torch.cuda.device(self.device):
             _l.check(_l.load().ccnn_adamw_moments(self._table, len(self._table), _ptr(self.m), _ptr(self.v), _ptr(self.m_scale),

@@ -496,3 +496,28 @@ def test_parameters_are_those_that_the_optimiser_was_made_for(bits):
     assert opt.step_count == 1 and not more.any()
     opt.step([g])
     assert opt.step_count == 2
+
+
+@pytest.mark.parametrize("kind,bits", [(F32, 32), (F64, 32), (BF16, 32), (F32, 8), (BF16, 8)], ids=str)
+def test_state_of_another_size_or_type_is_refused(kind, bits):
+    """The state is in public attributes; a step writes to no tensor that is too small for it."""
+    params, grads = tensors([700, 0, 300], kind, 60, 0.5), tensors([700, 0, 300], kind, 61, 1e-2)
+    opt = ops.AdamW(params, state_bits=bits)
+    opt.step(grads)
+    for name in ("m", "v", "m_scale", "v_scale", "master", "_clock"):
+        own = getattr(opt, name)
+        if own is None:
+            others = [torch.zeros(4, device="cuda")]
+        else:
+            others = [own[:-1], own.cpu(), own.to(torch.float16), torch.cat([own, own])[::2], torch.cat([own, own]), None, 3]
+        for other in others:
+            setattr(opt, name, other)
+            with pytest.raises((ValueError, TypeError)):
+                opt.step(grads)
+            if bits == 8 and name != "_clock" and own is not None:
+                with pytest.raises((ValueError, TypeError)):
+                    opt.moments()
+        setattr(opt, name, own)
+    assert opt.step_count == 1
+    opt.step(grads)
+    assert opt.step_count == 2

@@ -329,9 +329,10 @@ __device__ __forceinline__ unsigned encode8(double y)
     return (unsigned)(u >> 49) - ((1023u - 7u) << 3);
 }
 
-// Four codes of x / scale; positive: no sign, and what v says is above 0 keeps at least the smallest code.
+// Four codes of x / scale; positive: no sign, and what v says is above 0 keeps at least the smallest code.  `in` of them, or
+// more, are in the tensor: of a scale that is NaN all codes are, but for those behind its end, which stay 0.
 template <bool POSITIVE>
-__device__ __forceinline__ unsigned exact_codes(const double (&x)[4], const double (&v)[4], float scale)
+__device__ __forceinline__ unsigned exact_codes(const double (&x)[4], const double (&v)[4], float scale, long in)
 {
     if (scale == 0) return 0;
     unsigned w = 0;
@@ -343,6 +344,7 @@ __device__ __forceinline__ unsigned exact_codes(const double (&x)[4], const doub
         if (!POSITIVE && x[e] < 0) c |= 0x80;
         w |= c << (8 * e);
     }
+    if (scale != scale && in < 4) w &= in > 0 ? (1u << (8 * in)) - 1 : 0;
     return w;
 }
 
@@ -351,7 +353,7 @@ __device__ __forceinline__ unsigned exact_codes(const double (&x)[4], const doub
 // exact quotient.  Blocks with an undecided element or a root to be kept above 0, and scales outside the range
 // where that holds, go the way above.
 template <bool POSITIVE>
-__device__ __forceinline__ unsigned codes(const double (&x)[4], const double (&v)[4], const float (&x32)[4], float scale)
+__device__ __forceinline__ unsigned codes(const double (&x)[4], const double (&v)[4], const float (&x32)[4], float scale, long in)
 {
     const float inv = __builtin_amdgcn_rcpf(scale), more = inv * (1.0f + 0x1p-21f), less = inv * (1.0f - 0x1p-21f);
     unsigned up = 0, down = 0;
@@ -361,7 +363,7 @@ __device__ __forceinline__ unsigned codes(const double (&x)[4], const double (&v
     down = __builtin_amdgcn_cvt_pk_fp8_f32(x32[2] * less, x32[3] * less, down, true);
     bool open = up != down;
     if (POSITIVE) open |= ((down - 0x01010101u) & ~down & 0x80808080u) != 0;     // a byte of 0
-    if (!(scale > 1e-30f && scale < 1e30f) || __any(open)) return exact_codes<POSITIVE>(x, v, scale);
+    if (!(scale > 1e-30f && scale < 1e30f) || __any(open)) return exact_codes<POSITIVE>(x, v, scale, in);
     return up;
 }
 
@@ -467,8 +469,8 @@ __global__ __launch_bounds__(256) void adamw_coded(StepList<STEP_TENSORS> list, 
         const bool lost = high_v >= 0x7f800000u || high_m >= 0x7f800000u;
         const float sm = lost ? __builtin_nanf("") : scale_of(__uint_as_float(high_m));
         const float sv = lost ? __builtin_nanf("") : scale_of(__uint_as_float(high_v));
-        ((unsigned *)a.m)[(blk0 + u) * (BLOCK / 4) + lane] = codes<false>(m, v, m32, sm);
-        ((unsigned *)a.v)[(blk0 + u) * (BLOCK / 4) + lane] = codes<true>(root, v, root32, sv);
+        ((unsigned *)a.m)[(blk0 + u) * (BLOCK / 4) + lane] = codes<false>(m, v, m32, sm, n - k);
+        ((unsigned *)a.v)[(blk0 + u) * (BLOCK / 4) + lane] = codes<true>(root, v, root32, sv, n - k);
         if (lane == 0) a.m_scale[blk0 + u] = sm, a.v_scale[blk0 + u] = sv;
     }
     if (ALONE) arrive<256>(a, tick);

@@ -521,3 +521,21 @@ def test_state_of_another_size_or_type_is_refused(kind, bits):
     assert opt.step_count == 1
     opt.step(grads)
     assert opt.step_count == 2
+
+
+@pytest.mark.parametrize("kinds", [[F32], [F32, BF16]], ids=str)
+def test_bytes_behind_a_tensor_stay_0_in_a_block_that_is_not_finite(kinds):
+    """One launch (one type) and several."""
+    n = 300
+    params = [torch.zeros(n, dtype=k, device="cuda") for k in kinds]
+    opt = ops.AdamW(params, state_bits=8)
+    for value in (math.nan, 0.1, math.inf):
+        grads = [torch.full((n,), 0.1, dtype=k, device="cuda") for k in kinds]
+        for g in grads:
+            g[290] = value
+        opt.step(grads)
+        for codes, scale in ((opt.m, opt.m_scale), (opt.v, opt.v_scale)):
+            for i in range(len(kinds)):
+                c, s = codes[i * 512:(i + 1) * 512].cpu(), scale[2 * i:2 * i + 2].cpu()
+                assert torch.isfinite(s[0]) and torch.isnan(s[1])
+                assert (c[256:300] == 0x7f).all() and not c[300:].any() and (c[:256] == 0x7e).all()

@@ -17,8 +17,11 @@ constexpr int NORM_TENSORS = 192, STEP_TENSORS = 64, FEW_TENSORS = 16;
 constexpr int BLOCK = CCNN_MOMENT_BLOCK;
 
 // ---------------------------------------------------------------------------- gradient norm
-// Squares are summed in fp64 (no square of an fp32 gradient overflows it, and 2e8 of them lose nothing), in an order
-// that the sizes alone fix.  A wave to a chunk: short ones while they are needed to fill the device, long ones beyond
+// Squares are summed in fp64, in an order that the sizes alone fix: those of fp32 and 16-bit gradients are exact there and fit, and
+// the sum of n of them is off by at most (n / 64 + 40) 2^-53 of itself, a rounding for each addition.  Squares of fp64 gradients
+// may not fit: where a sum of theirs shows that, what is beyond 2^480 or below 2^-480 is summed apart, brought near 1 by a
+// power of two.  The look costs 47 k fp64 gradients 0.15 us (4.8 of the device) and 210 M nothing (247 us, 6.8 TB/s).
+// A wave to a chunk: short ones while they are needed to fill the device, long ones beyond
 // (202 M bf16 gradients: 69 us, 5.9 TB/s; 78 with workgroups of 256 to 16 K, 73 with a wave to 16 K).
 inline long norm_chunk(long total) { return total < (1L << 25) ? 4096 : 32768; }
 constexpr int NORM_THREADS = 64;
@@ -58,15 +61,54 @@ __device__ __forceinline__ double block_sum(double v, double *lds)
     return v;
 }
 
+// Sums of squares: of numbers within 2^480 and 2^-480, of those beyond times 2^-600, of those below times 2^600.
+struct Squares {
+    double mid = 0, big = 0, tiny = 0;
+};
+constexpr double FAR = 0x1p480, BACK = 0x1p600;
+
+// A sum of squares that stands for Squares::mid as it is: none was lost then but some below 2^-1022.  So does that of zeros.
+__device__ __forceinline__ bool stands(double s) { return s >= 0x1p-900 && s < 0x1p960; }
+
+// Squares of fp64 numbers one by one, those of packs [k, n) of W, `step` apart.
+template <int W>
+__device__ __forceinline__ void add_apart(Squares &s, const double *p, long k, long n, long step)
+{
+#pragma unroll 1
+    for (; k < n; k += step)
+#pragma unroll 1
+        for (long j = k; j < min(k + W, n); j++) {
+            const double a = fabs(p[j]), b = a * (1 / BACK), t = a * BACK;
+            if (a > FAR) s.big += b * b;
+            else if (a < 1 / FAR) s.tiny += t * t;
+            else s.mid += a * a;
+        }
+}
+
+// mid, with a sign where something is apart.
+__device__ __forceinline__ double marked(const Squares &s)
+{
+    return s.big > 0 || s.tiny > 0 ? -fabs(s.mid) : fabs(s.mid);
+}
+
 template <typename T>
-__global__ __launch_bounds__(NORM_THREADS) void norm_partial(NormList<NORM_TENSORS> list, int chunk, double *__restrict__ partial)
+__global__ __launch_bounds__(NORM_THREADS) void norm_partial(NormList<NORM_TENSORS> list, int chunk, double *__restrict__ partial,
+                                                             double *__restrict__ apart, long apart_stride)
 {
     constexpr int W = 16 / sizeof(T), U = 8, STRIDE = NORM_THREADS * W;
     const int i = find(list, blockIdx.x);
     const long at = (long)(blockIdx.x - list.chunk0[i]) * chunk;
     const T *p = (const T *)list.data[i] + at;
     const int n = (int)min(list.n[i] - at, (long)chunk);
-    double s = 0;
+    double sum = 0;
+    unsigned high = 0, low = 0;       // bits of any fp64 number: without one they are zeros
+    auto add = [&](T x) {
+        sum += (double)widen(x) * (double)widen(x);
+        if constexpr (sizeof(T) == 8) {
+            const unsigned long long b = __double_as_longlong(x);
+            high |= (unsigned)(b >> 32), low |= (unsigned)b;
+        }
+    };
     for (int k = threadIdx.x * W; k < n; k += U * STRIDE) {
         Pack<T, W> x[U];
 #pragma unroll
@@ -77,33 +119,57 @@ __global__ __launch_bounds__(NORM_THREADS) void norm_partial(NormList<NORM_TENSO
             const int j0 = k + u * STRIDE;
             if (j0 + W <= n) {
 #pragma unroll
-                for (int e = 0; e < W; e++) s += (double)widen(x[u].v[e]) * (double)widen(x[u].v[e]);
+                for (int e = 0; e < W; e++) add(x[u].v[e]);
             } else {
-                for (int j = j0; j < n; j++) s += (double)widen(p[j]) * (double)widen(p[j]);
+                for (int j = j0; j < n; j++) add(p[j]);
             }
         }
     }
-    s = lanes_sum<64>(s);
-    if (threadIdx.x == 0) partial[blockIdx.x] = s;
+    Squares s = {sum};
+    if constexpr (sizeof(T) == 8)
+        if (!stands(sum) && (high << 1 | low) != 0) s = {}, add_apart<W>(s, p, threadIdx.x * W, n, STRIDE);
+    s.mid = lanes_sum<64>(s.mid);
+    if (__any(s.big > 0 || s.tiny > 0)) s.big = lanes_sum<64>(s.big), s.tiny = lanes_sum<64>(s.tiny);
+    if (threadIdx.x == 0) {
+        partial[blockIdx.x] = marked(s);
+        if (signbit(marked(s))) apart[blockIdx.x] = s.big, apart[apart_stride + blockIdx.x] = s.tiny;
+    }
 }
 
-__device__ __forceinline__ void put_norm(double squares, double max_norm, double *out)
+__device__ __forceinline__ void put_norm(const Squares &s, double max_norm, double *out)
 {
-    const double norm = sqrt(squares);
+    double squares = s.mid, unit = 1;
+    if (__builtin_expect(s.big > 0, 0)) squares = s.big + s.mid * (1 / BACK) * (1 / BACK), unit = BACK;
+    else if (s.mid == 0) squares = s.tiny, unit = 1 / BACK;
+    else squares += s.tiny * (1 / BACK) * (1 / BACK);
+    const double norm = sqrt(squares) * unit;
     out[0] = norm;
     out[1] = !(norm < __builtin_huge_val()) ? __builtin_nan("") : norm > max_norm ? max_norm / norm : 1.0;
 }
 
 constexpr int TOTAL_THREADS = 1024;
 
-__global__ __launch_bounds__(TOTAL_THREADS) void norm_total(const double *__restrict__ partial, int n, double max_norm,
-                                                  double *__restrict__ out)
+template <bool F64>
+__global__ __launch_bounds__(TOTAL_THREADS) void norm_total(const double *__restrict__ partial, int n, const double *__restrict__ apart,
+                                                            long apart_stride, double max_norm, double *__restrict__ out)
 {
-    __shared__ double lds[TOTAL_THREADS / 64];
-    double s = 0;
+    __shared__ double lds[F64 ? 3 : 1][TOTAL_THREADS / 64];
+    Squares s;
+    bool any = false;
 #pragma unroll 4
-    for (int k = threadIdx.x; k < n; k += TOTAL_THREADS) s += partial[k];
-    s = block_sum<TOTAL_THREADS>(s, lds);
+    for (int k = threadIdx.x; k < n; k += TOTAL_THREADS) {
+        const double mid = partial[k];
+        s.mid += F64 ? fabs(mid) : mid;
+        any |= F64 && signbit(mid);
+    }
+    s.mid = block_sum<TOTAL_THREADS>(s.mid, lds[0]);
+    if constexpr (F64)
+        if (__syncthreads_or(any)) {
+            for (int k = threadIdx.x; k < n; k += TOTAL_THREADS)
+                if (signbit(partial[k])) s.big += apart[k], s.tiny += apart[apart_stride + k];
+            s.big = block_sum<TOTAL_THREADS>(s.big, lds[1]);
+            s.tiny = block_sum<TOTAL_THREADS>(s.tiny, lds[2]);
+        }
     if (threadIdx.x == 0) put_norm(s, max_norm, out);
 }
 
@@ -132,19 +198,40 @@ __device__ __forceinline__ double piece_squares(const void *data, long at, long 
     return s;
 }
 
+// Whether the plain sum of all stands is seen at the end; where it does not, the fp64 pieces are read again.
+template <bool F64>
 __global__ __launch_bounds__(TOTAL_THREADS) void norm_one(FewList list, double max_norm, double *__restrict__ out)
 {
-    __shared__ double lds[TOTAL_THREADS / 64];
-    double s = 0;
+    __shared__ double lds[F64 ? 4 : 1][TOTAL_THREADS / 64];
+    Squares s;
+    double s64 = 0;
     for (int c = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); c < list.chunk0[list.count]; c += TOTAL_THREADS / 64) {
         const int i = find(list, c), type = list.type[i];
         const long at = (c - list.chunk0[i]) * PIECE, n = list.n[i];
-        s += type == CCNN_TYPE_F32    ? piece_squares<float>(list.data[i], at, n)
-             : type == CCNN_TYPE_F64  ? piece_squares<double>(list.data[i], at, n)
-             : type == CCNN_TYPE_BF16 ? piece_squares<Bf16>(list.data[i], at, n)
-                                      : piece_squares<F16>(list.data[i], at, n);
+        if (F64 && type == CCNN_TYPE_F64) s64 += piece_squares<double>(list.data[i], at, n);
+        else
+            s.mid += type == CCNN_TYPE_F32    ? piece_squares<float>(list.data[i], at, n)
+                     : type == CCNN_TYPE_BF16 ? piece_squares<Bf16>(list.data[i], at, n)
+                                              : piece_squares<F16>(list.data[i], at, n);
     }
-    s = block_sum<TOTAL_THREADS>(s, lds);
+    if constexpr (F64) {
+        const double all = block_sum<TOTAL_THREADS>(s.mid + s64, lds[0]);
+        if (stands(all)) {
+            s.mid = all;
+        } else {
+            for (int c = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); c < list.chunk0[list.count]; c += TOTAL_THREADS / 64) {
+                const int i = find(list, c);
+                const long at = (c - list.chunk0[i]) * PIECE;
+                if (list.type[i] == CCNN_TYPE_F64)
+                    add_apart<1>(s, (const double *)list.data[i], at + (threadIdx.x & 63), min(at + PIECE, list.n[i]), 64);
+            }
+            s.mid = block_sum<TOTAL_THREADS>(s.mid, lds[1]);
+            s.big = block_sum<TOTAL_THREADS>(s.big, lds[2]);
+            s.tiny = block_sum<TOTAL_THREADS>(s.tiny, lds[3]);
+        }
+    } else {
+        s.mid = block_sum<TOTAL_THREADS>(s.mid, lds[0]);
+    }
     if (threadIdx.x == 0) put_norm(s, max_norm, out);
 }
 
@@ -576,7 +663,7 @@ size_t ccnn_grad_norm_workspace_bytes(const long *n, int count)
     size_t chunks = 1;
     for (int i = 0; i < count; i++)
         if (n[i] > 0) chunks += (size_t)(n[i] / chunk + (n[i] % chunk != 0));
-    return chunks * sizeof(double);
+    return chunks * sizeof(Squares);
 }
 
 int ccnn_grad_norm(const void *const *data, const long *n, const int *types, int count, double max_norm, double *out,
@@ -589,7 +676,7 @@ int ccnn_grad_norm(const void *const *data, const long *n, const int *types, int
         used[types[i]] = true;
     }
     const size_t need = ccnn_grad_norm_workspace_bytes(n, count);
-    if (need / sizeof(double) > 0x7fffffffu) return CCNN_E_RANGE;
+    if (need / sizeof(Squares) > 0x7fffffffu) return CCNN_E_RANGE;
     if (workspace_bytes < need || (need && !workspace)) return CCNN_E_WORKSPACE;
     hipStream_t st = (hipStream_t)stream;
     if (norm_in_one(n, count)) {
@@ -603,11 +690,12 @@ int ccnn_grad_norm(const void *const *data, const long *n, const int *types, int
             list.type[c] = types[i];
             list.chunk0[c + 1] = list.chunk0[c] + (int)((n[i] + PIECE - 1) / PIECE);
         }
-        launch("norm_one", norm_one, dim3(1), dim3(TOTAL_THREADS), 0, st, list, max_norm, out);
+        launch("norm_one", used[CCNN_TYPE_F64] ? norm_one<true> : norm_one<false>, dim3(1), dim3(TOTAL_THREADS), 0, st, list, max_norm, out);
         CCNN_LAUNCH_CHECK();
         return 0;
     }
-    double *partial = (double *)workspace;
+    const long apart_stride = (long)(need / sizeof(Squares));
+    double *partial = (double *)workspace, *apart = partial + apart_stride;
     const long chunk = norm_chunk(sum_of(n, count));
     int done = 0;
     auto take = [&](auto &list, int i, int type) -> long {
@@ -629,14 +717,15 @@ int ccnn_grad_norm(const void *const *data, const long *n, const int *types, int
                                        : type == CCNN_TYPE_F64  ? norm_partial<double>
                                        : type == CCNN_TYPE_BF16 ? norm_partial<Bf16>
                                                                 : norm_partial<F16>,
-                       dim3((unsigned)chunks), dim3(NORM_THREADS), 0, st, list, (int)chunk, partial + done);
+                       dim3((unsigned)chunks), dim3(NORM_THREADS), 0, st, list, (int)chunk, partial + done, apart + done, apart_stride);
                 CCNN_LAUNCH_CHECK();
                 done += chunks;
                 return 0;
             });
         if (e) return e;
     }
-    launch("norm_total", norm_total, dim3(1), dim3(TOTAL_THREADS), 0, st, partial, done, max_norm, out);
+    launch("norm_total", used[CCNN_TYPE_F64] ? norm_total<true> : norm_total<false>, dim3(1), dim3(TOTAL_THREADS), 0, st, partial, done, apart, apart_stride,
+           max_norm, out);
     CCNN_LAUNCH_CHECK();
     return 0;
 }

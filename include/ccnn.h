@@ -422,8 +422,8 @@ int ccnn_log_probs_grad(const void *logits, int type, long rows, int classes, lo
 
 /* Norm of many gradient tensors taken as one vector, and the factor that limits it.
  * data, n, types: HOST arrays of `count` pointers, element counts (0 allowed) and CCNN_TYPE_*.
- * out [2] device doubles: sqrt(sum g^2), summed in fp64 in a fixed order; and min(1, max_norm / norm),
- * NaN when the norm is not finite.  workspace: ccnn_grad_norm_workspace_bytes() bytes (0 for few and
+ * out [2] device doubles: sqrt(sum g^2), summed in fp64 in a fixed order, also where squares of fp64 gradients
+ * leave that range; and min(1, max_norm / norm), NaN when the norm is not finite.  workspace: ccnn_grad_norm_workspace_bytes() bytes (0 for few and
  * small tensors), not initialised; calls that share one must be ordered by one stream. */
 size_t ccnn_grad_norm_workspace_bytes(const long *n, int count);
 int ccnn_grad_norm(const void *const *data, const long *n, const int *types, int count,

@@ -539,3 +539,53 @@ def test_bytes_behind_a_tensor_stay_0_in_a_block_that_is_not_finite(kinds):
                 c, s = codes[i * 512:(i + 1) * 512].cpu(), scale[2 * i:2 * i + 2].cpu()
                 assert torch.isfinite(s[0]) and torch.isnan(s[1])
                 assert (c[256:300] == 0x7f).all() and not c[300:].any() and (c[:256] == 0x7e).all()
+
+
+def scaled_norm(tensors):
+    """The norm of fp64 gradients of any size: of the values over their largest, summed without rounding."""
+    flat = torch.cat([t.cpu().double().reshape(-1) for t in tensors])
+    high = 2.0 ** math.floor(math.log2(float(flat.abs().max())))
+    return math.sqrt(math.fsum(((flat / high) ** 2).tolist())), high
+
+
+@pytest.mark.parametrize("sizes", [[1], [1000], [81921, 5], [300001], [100] * 40 + [7]], ids=str)
+@pytest.mark.parametrize("scale,other", [(1e200, 1.0), (1e200, 1e200), (1e-200, 0.0), (1e-200, 1e-200), (1e-310, 0.0), (1e-170, 1e-130),
+                                         (3e153, 1e154), (1e300, 1e-300)])
+def test_norm_of_doubles_whose_squares_leave_the_range(sizes, scale, other):
+    """A finite norm is found whatever its squares do: sums of n terms of one size, and a rounding of each square."""
+    grads = tensors(sizes, F64, 12, 1.0)
+    for g in grads:
+        g.clamp_(-4, 4)
+        g.mul_(scale)
+        g[1::3] = other
+    norm, high = scaled_norm(grads)
+    limit = 1e-3 * high
+    out = ops.grad_norm(grads, limit).tolist()
+    rel = 2.0 ** -53 * (sum(sizes) / 256 + 40) + 2.0 ** -1074 / (norm * high)
+    assert out[0] / high == pytest.approx(norm, rel=rel)
+    assert out[1] == pytest.approx(min(1.0, limit / high / norm), rel=1e-12 + rel)
+
+
+@pytest.mark.parametrize("n", [1000, 300001])
+def test_norm_beyond_doubles_and_a_step_just_below(n):
+    g = torch.full((n,), 1.7e308, dtype=F64, device="cuda")
+    norm, factor = ops.grad_norm([g], 1.0).tolist()
+    assert norm == math.inf and math.isnan(factor)
+    g.fill_(1e300)
+    mixed = [g, torch.full((50,), 3e38, device="cuda")]
+    clip = ops.grad_norm(mixed, 1.0)
+    assert clip[0].item() == pytest.approx(1e300 * math.sqrt(n), rel=1e-12)
+    for others in (1e300, 1.0, 1e-200, 0.0):
+        g.fill_(others)
+        g[5] = math.nan
+        assert all(map(math.isnan, ops.grad_norm([g], 1.0).tolist()))
+        g[5] = -0.0
+        assert ops.grad_norm([g], 1.0)[0].item() == pytest.approx(others * math.sqrt(n - 1), rel=1e-12)
+    g[5] = -math.inf
+    assert math.isnan(ops.grad_norm([g], 1.0)[1].item())
+    g.fill_(1e300)
+    p = torch.zeros(n, dtype=F64, device="cuda")
+    opt = ops.AdamW([p])
+    opt.step([g], clip=ops.grad_norm([g], 1.0))
+    assert opt.step_count == 1
+    assert (opt.moments()[0] * (10 * math.sqrt(n)) - 1).abs().max() < 1e-12

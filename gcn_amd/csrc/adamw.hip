@@ -294,20 +294,30 @@ __global__ void adamw_clock(StepArgs a)
     a.clock[6] = tick.skip ? __builtin_nan("") : tick.scale;
 }
 
+// The gradient factor in two: one that is no normal number of A - large gradients clipped to a small norm - would lose
+// what the product keeps, or be 0.
 template <typename A>
 struct Rates {
-    A scale, lr_decay, rate, root, eps;
+    A scale, scale2, lr_decay, rate, root, eps;
     bool skip;
+    __device__ Rates(double factor, double lr, double decay, double rate, double root, double eps, bool skip)
+        : scale((A)factor), scale2(1), lr_decay((A)(lr * decay)), rate((A)rate), root((A)root), eps((A)eps), skip(skip)
+    {
+        if constexpr (sizeof(A) == 4) {
+            const double size = fabs(factor);
+            if (size < 0x1p-126) scale = 0x1p-126f, scale2 = (A)(factor * 0x1p126);
+            if (size > 0x1p127) scale = 0x1p127f, scale2 = (A)(factor * 0x1p-127);
+        }
+    }
     __device__ Rates(const StepArgs &a, double decay)
-        : scale((A)a.clock[6]), lr_decay((A)(a.clock[3] * decay)), rate((A)a.clock[4]), root((A)a.clock[5]), eps((A)a.eps),
-          skip(!(a.clock[6] == a.clock[6]))
+        : Rates(a.clock[6], a.clock[3], decay, a.clock[4], a.clock[5], a.eps, !(a.clock[6] == a.clock[6]))
     {
     }
     __device__ Rates(const StepArgs &a, const Tick &tick, double decay)
-        : scale((A)tick.scale), lr_decay((A)(tick.lr * decay)), rate((A)tick.rate), root((A)tick.root), eps((A)a.eps),
-          skip(tick.skip)
+        : Rates(tick.scale, tick.lr, decay, tick.rate, tick.root, a.eps, tick.skip)
     {
     }
+    __device__ __forceinline__ A of(A g) const { return sizeof(A) == 4 ? g * scale * scale2 : g * scale; }
 };
 
 // A launch that is the whole step moves the clock itself: every wave has read it when its workgroup arrives here, the
@@ -387,7 +397,7 @@ __global__ __launch_bounds__(WIDE_THREADS) void adamw_wide(StepList<U == 1 ? FEW
         Pack<P, W> out;
 #pragma unroll
         for (int e = 0; e < W; e++) {
-            const A g = (A)widen(gk[u].v[e]) * r.scale;
+            const A g = r.of((A)widen(gk[u].v[e]));
             mk[u].v[e] += b1 * (g - mk[u].v[e]);
             const A old_v = vk[u].v[e];
             vk[u].v[e] += b2 * (g * g - (old_v == -ninf(A()) ? A(0) : old_v));   // what is beyond the type stays infinite

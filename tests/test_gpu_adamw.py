@@ -589,3 +589,32 @@ def test_norm_beyond_doubles_and_a_step_just_below(n):
     opt.step([g], clip=ops.grad_norm([g], 1.0))
     assert opt.step_count == 1
     assert (opt.moments()[0] * (10 * math.sqrt(n)) - 1).abs().max() < 1e-12
+
+
+@pytest.mark.parametrize("kind,grad_kind", [(F32, F32), (BF16, F32), (BF16, BF16), (F64, F64)], ids=str)
+@pytest.mark.parametrize("n", [1000, 200001, 1500001])
+@pytest.mark.parametrize("limit", [1e-3, 1e-9])
+def test_a_clip_factor_below_fp32(kind, grad_kind, n, limit):
+    """Gradients near the largest fp32 clipped to a small norm: the factor is no normal fp32 number, the clipped
+    gradient is.  m rounds g * factor (twice, a factor of two numbers) and its own two operations: 4 half steps."""
+    grads = [g.mul_(3e37) for g in tensors([n], grad_kind, 40, 1.0)]
+    params = tensors([n], kind, 41, 0.5)
+    opt = ops.AdamW(params)
+    clip = ops.grad_norm(grads, limit)
+    assert 0 < clip[1].item() < 1e-39
+    opt.step(grads, clip=clip)
+    want = 0.1 * (grads[0].cpu().double() * clip[1].item())
+    wide = F64 if kind == F64 else F32
+    off = (opt.moments()[0].cpu().double() - want).abs()
+    # products that are no normal fp32 numbers are off by half their distance, m by that of its own
+    assert (off <= 6 * ref.half_step(wide) * want.abs() + 3 * 2.0 ** -149).all()
+    assert want.abs().max() > 1e-8 * limit
+
+
+@pytest.mark.parametrize("n", [1000, 200001])
+def test_a_clip_factor_above_fp32(n):
+    """A factor from elsewhere that brings tiny gradients up."""
+    g = torch.full((n,), 2.0 ** -140, device="cuda")
+    opt = ops.AdamW([torch.zeros(n, device="cuda")])
+    opt.step([g], clip=torch.tensor([1.0, 2.0 ** 140], dtype=F64, device="cuda"))
+    assert (opt.moments()[0] * 10 - 1).abs().max() < 1e-6

@@ -294,15 +294,21 @@ __global__ void adamw_clock(StepArgs a)
     a.clock[6] = tick.skip ? __builtin_nan("") : tick.scale;
 }
 
-// The gradient factor in two: one that is no normal number of A - large gradients clipped to a small norm - would lose
+// In fp32 the gradient factor is two: one that is no normal number - large gradients clipped to a small norm - would lose
 // what the product keeps, or be 0.
-template <typename A>
+// FITS: lr m is within A whatever the moments hold.
+template <typename A, bool FITS>
 struct Rates {
     A scale, scale2, lr_decay, rate, root, eps;
     bool skip;
     __device__ Rates(double factor, double lr, double decay, double rate, double root, double eps, bool skip)
         : scale((A)factor), scale2(1), lr_decay((A)(lr * decay)), rate((A)rate), root((A)root), eps((A)eps), skip(skip)
     {
+        if constexpr (!FITS) {      // lr m may be beyond the type where m is not: the power of two in an lr of 1 or more goes below the line
+            const int down = -max(__builtin_amdgcn_frexp_exp(lr), 0);
+            this->rate = (A)ldexp(rate, down), this->root = (A)ldexp(root, down);
+            this->eps = (A)fmax(ldexp(eps, down), sizeof(A) == 4 ? 0x1p-149 : 0x1p-1074);
+        }
         if constexpr (sizeof(A) == 4) {
             const double size = fabs(factor);
             if (size < 0x1p-126) scale = 0x1p-126f, scale2 = (A)(factor * 0x1p126);
@@ -317,7 +323,6 @@ struct Rates {
         : Rates(tick.scale, tick.lr, decay, tick.rate, tick.root, a.eps, tick.skip)
     {
     }
-    __device__ __forceinline__ A of(A g) const { return sizeof(A) == 4 ? g * scale * scale2 : g * scale; }
 };
 
 // A launch that is the whole step moves the clock itself: every wave has read it when its workgroup arrives here, the
@@ -350,7 +355,7 @@ __device__ __forceinline__ void arrive(const StepArgs &a, const Tick &tick)
 }
 
 template <typename A>
-__device__ __forceinline__ A stepped(A p, A m, A v_root, const Rates<A> &r)
+__device__ __forceinline__ A stepped(A p, A m, A v_root, const Rates<A, false> &r)
 {
     return p - (r.lr_decay * p + r.rate * m / (v_root * r.root + r.eps));
 }
@@ -388,17 +393,18 @@ __global__ __launch_bounds__(WIDE_THREADS) void adamw_wide(StepList<U == 1 ? FEW
     }
     const bool alone = U == 1 || a.alone;
     const Tick tick = alone ? Tick(a) : Tick();
-    const Rates<A> r = alone ? Rates<A>(a, tick, list.decay[i]) : Rates<A>(a, list.decay[i]);
+    typedef Rates<A, false> R;
+    const R r = alone ? R(a, tick, list.decay[i]) : R(a, list.decay[i]);
     if (r.skip) return;
-    const A b1 = (A)(1 - a.beta1), b2 = (A)(1 - a.beta2);
+    const A b1 = (A)(1 - a.beta1), b2 = (A)(1 - a.beta2), twice_b1 = 2 * b1, half2 = A(0.5) * r.scale2;
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const long k = k0 + u * WIDE_THREADS * W;
         Pack<P, W> out;
 #pragma unroll
         for (int e = 0; e < W; e++) {
-            const A g = r.of((A)widen(gk[u].v[e]));
-            mk[u].v[e] += b1 * (g - mk[u].v[e]);
+            const A x = (A)widen(gk[u].v[e]) * r.scale, g = sizeof(A) == 4 ? x * r.scale2 : x;
+            mk[u].v[e] += twice_b1 * (x * half2 - A(0.5) * mk[u].v[e]);     // g - m may be beyond the type, half of it is not
             const A old_v = vk[u].v[e];
             vk[u].v[e] += b2 * (g * g - (old_v == -ninf(A()) ? A(0) : old_v));   // what is beyond the type stays infinite
             pk[u].v[e] = stepped((A)pk[u].v[e], mk[u].v[e], (A)sqrt(vk[u].v[e]), r);
@@ -531,7 +537,8 @@ __global__ __launch_bounds__(256) void adamw_coded(StepList<STEP_TENSORS> list, 
         vs[u] = a.v_scale[blk0 + u];
     }
     const Tick tick = ALONE ? Tick(a) : Tick();
-    const Rates<double> r = ALONE ? Rates<double>(a, tick, list.decay[i]) : Rates<double>(a, list.decay[i]);
+    typedef Rates<double, true> R;
+    const R r = ALONE ? R(a, tick, list.decay[i]) : R(a, list.decay[i]);
     if (r.skip) return;
 #pragma unroll
     for (int u = 0; u < U; u++) {

@@ -618,3 +618,43 @@ def test_a_clip_factor_above_fp32(n):
     opt = ops.AdamW([torch.zeros(n, device="cuda")])
     opt.step([g], clip=torch.tensor([1.0, 2.0 ** 140], dtype=F64, device="cuda"))
     assert (opt.moments()[0] * 10 - 1).abs().max() < 1e-6
+
+
+@pytest.mark.parametrize("kind", [F32, F64, BF16], ids=str)
+@pytest.mark.parametrize("n", [1000, 200001])
+@pytest.mark.parametrize("beta1,lr", [(0.9, 1e-3), (0.0, 1e-3), (0.9, 100.0)])
+def test_gradients_near_the_largest_number_of_both_signs(kind, n, beta1, lr):
+    """Finite gradients leave m finite, and an element whose v is beyond the type where it is, also where g - m or
+    lr * m is beyond it too; one that is not finite is seen."""
+    big = 0.95 * torch.finfo(kind).max
+    p = torch.zeros(n, dtype=kind, device="cuda")
+    g = torch.full((n,), 0.1, dtype=kind, device="cuda")
+    opt, m = ops.AdamW([p], lr=lr, betas=(beta1, 0.999), weight_decay=0.0), 0.0
+    for k in range(40):
+        g[n - 7] = big if k < 30 else -big
+        opt.step([g])
+        m = beta1 * m + (1 - beta1) * (g[n - 7].item() / big)
+    got = opt.moments()[0][n - 7].double().item() / big
+    assert abs(got - m) <= 1e-5
+    assert p[n - 7] == 0 and torch.isfinite(p).all() and torch.count_nonzero(p < 0) == n - 1
+    g[n - 7] = math.inf
+    opt.step([g])
+    assert torch.isnan(p[n - 7]) and torch.count_nonzero(torch.isfinite(p)) == n - 1
+
+
+@pytest.mark.parametrize("kind", [F32, F64, BF16], ids=str)
+@pytest.mark.parametrize("lr", [1.0, 3.0, 1e6, -5.0])
+def test_rates_of_one_or_more(kind, lr):
+    """The quotient is that of the formula, and of an element without a gradient still 0 with the smallest eps."""
+    u = ref.half_step(F64 if kind == F64 else F32)
+    params, grads = tensors([3000, 70], kind, 70, 0.5), tensors([3000, 70], kind, 71, 1e-2)
+    opt, want = ops.AdamW(params, lr=lr, weight_decay=0.0), ref.AdamW(params, lr, decays=[0.0, 0.0])
+    opt.step(grads)
+    want.step(grads)
+    held = opt.master if opt.master is not None else torch.cat(params)
+    # the first step is of size lr; its quotient, roots and products round 16 times at most, p once
+    assert ((held.cpu().double() - torch.cat(want.p)).abs() <= 16 * u * abs(lr) + u * torch.cat(want.p).abs()).all()
+    p = torch.ones(500, dtype=kind, device="cuda")
+    still = ops.AdamW([p], lr=lr, eps=5e-324 if kind == F64 else 1e-45, weight_decay=0.0)
+    still.step([torch.zeros_like(p)])
+    assert (p == 1).all()

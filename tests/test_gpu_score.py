@@ -471,3 +471,56 @@ def test_calls_keep_no_references_to_none():
         for _ in range(1000):
             ops.log_probs(x, y, top=top, want_entropy=want_entropy)
         assert abs(sys.getrefcount(None) - before) < 100, (top, want_entropy)
+
+
+def tight_bound(logits, want, dtype):
+    """How far the log sum may be off where a row has 512 parts at least (64 with 512 rows or more), u half a step.
+
+    A thread adds n / parts terms, then 6 + 8 + 6 steps join lanes, waves and slices, and the slices of a lane: n / parts
+    + 64 additions, u each.  A term e^d at d from a reference carries 3u|d| + 2u; the reference is at most 4
+    above or below the largest element's neighbourhood, so on average over the sum that is 3u (E|x - m| + 4) + 2u.  A thread's
+    reference moves up by more than 4 at a time, at most R / 4 + 1 times over the row's range R, and each
+    joining step moves a sum once: 3u of every distance, which add up to R + 4, and 3u of each of the at most
+    R / 4 + 8 moves.  The logarithm and its argument: 4u of it."""
+    x = logits.detach().cpu().double()
+    u = ref.half_step(dtype)
+    d = (x - torch.where(want["m"] == -INF, 0.0, want["m"])[:, None]).abs()
+    span = torch.where(torch.isfinite(d), d, 0.0).clamp(max=120.0 if dtype == torch.float32 else 760.0).amax(1).nan_to_num(0.0)
+    near = torch.where(want["p"] > 0, want["p"] * d, 0.0).sum(1).nan_to_num(0.0)
+    parts = 64 if x.shape[0] >= 512 else 512
+    adds = x.shape[1] / parts + 64
+    return u * (adds + 3 * (near + 4) + 2 + 3 * (span + 4) + 3 * (span / 4 + 8) + 4 * want["l"].abs().nan_to_num(0.0, 0.0, 0.0)), near
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=str)
+@pytest.mark.parametrize("rows,classes", [(4, 1027), (4, 4099), (513, 1037), (4, 32003), (4, 65543), (4, 70003), (3, 131077), (2, 200005)])
+def test_no_element_is_lost_from_a_long_row(rows, classes, kind):
+    """Sums within the bound that the real number of additions gives, at sizes that end inside a load; the last elements of
+    some rows, or the only ones of all slices but one, carry the whole sum."""
+    width = 128 // torch.finfo(kind).bits
+    x, y = problem(rows, classes, kind, seed=13)
+    x = x.contiguous()
+    u = ref.half_step(wide(kind))
+
+    def check():
+        r, want = check_scores(x, y, min(classes, 3))
+        b, near = tight_bound(x, want, wide(kind))
+        close(r.stats[3], want["l"], b, "l")
+        close(r.logp, want["logp"], b + 4 * u * want["logp"].abs().nan_to_num(0, 0, 0), "logp")
+        # l is off by b; t / s, with the reference at most 4 above and 4 below where it ends, by b (near + 8), and s takes b near more
+        close(r.entropy, want["entropy"], b * (9 + 2 * near) + 4 * u * want["entropy"].abs(), "entropy")
+
+    check()
+    x[:] = 1.0
+    check()
+    rest = classes % width or 1
+    x[:] = -INF
+    x[:, classes - rest:] = torch.arange(rest, dtype=torch.float64).to(kind).cuda() / 4
+    y[:] = classes - 1
+    check()
+    x[:] = -20.0
+    x[:, classes - rest:] = 5.0
+    check()
+    x[:, 0] = 5.0
+    y[:] = 0
+    check()

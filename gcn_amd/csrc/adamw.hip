@@ -21,8 +21,9 @@ constexpr int BLOCK = CCNN_MOMENT_BLOCK;
 // the sum of n of them is off by at most (n / 64 + 40) 2^-53 of itself, a rounding for each addition.  Squares of fp64 gradients
 // may not fit: where a sum of theirs shows that, what is beyond 2^480 or below 2^-480 is summed apart, brought near 1 by a
 // power of two.  The look costs 47 k fp64 gradients 0.15 us (4.8 of the device) and 210 M nothing (247 us, 6.8 TB/s).
-// A wave to a chunk: short ones while they are needed to fill the device, long ones beyond
-// (202 M bf16 gradients: 69 us, 5.9 TB/s; 78 with workgroups of 256 to 16 K, 73 with a wave to 16 K).
+// A wave to a chunk: short ones while they are needed to fill the device, long ones beyond (202 M bf16 gradients: 65 us, 6.2 TB/s;
+// 78 with workgroups of 256 to 16 K, 73 with a wave to 16 K).  Just beyond the border the long ones are too few waves: fp32, 31 M
+// take 24 us, 36 M 49, 52 M 53, 105 M 70 (6.0 TB/s) and 210 M 127 (6.6); bf16 19, 39, 41, 49 (4.3) and 66 (6.4).
 inline long norm_chunk(long total) { return total < (1L << 25) ? 4096 : 32768; }
 constexpr int NORM_THREADS = 64;
 
@@ -361,7 +362,7 @@ __device__ __forceinline__ A stepped(A p, A m, A v_root, const Rates<A, false> &
 }
 
 // A wave to a chunk, U packs of four elements in flight per lane.  Bound by the memory: 202 M bf16 parameters with fp32
-// master copy and moments (28 bytes each) in 970 us, 5.8 TB/s; with workgroups of 256 4 % slower, with three packs
+// master copy and moments (28 bytes each) in 951 us, 5.9 TB/s; with workgroups of 256 4 % slower, with three packs
 // 5, with eight 20.
 constexpr int WIDE_THREADS = 64;
 
@@ -502,9 +503,9 @@ __device__ __forceinline__ float scale_of(float h)
 }
 
 // One wave per block of 256 elements, four to a lane, two blocks in flight (one costs 6 % at 100 M parameters, four
-// 2 %; a small step has one, 100 k bf16 parameters in 5.3 us instead of 6.1).  Moments, root and step in fp64, so that codes, scales and steps are those of the definition whatever the
-// order of operations.  101 M bf16 parameters with fp32 master copy (16 bytes each) in 299 us, 5.4 TB/s; the vector
-// units are busy for some 60 % of it (342 operations a block and lane in an earlier form were 75 % and 4 % slower).
+// 2 %; a small step has one, 100 k bf16 parameters in 5.3 us instead of 6.1).  Moments, root and step in fp64, so that codes,
+// scales and steps are those of the definition whatever the order of operations.  101 M bf16 parameters with fp32 master copy (16 bytes each) in 297 us, 5.4 TB/s; the vector
+// units are busy for 84 % of the CUs' cycles meanwhile (561 operations a wave for two blocks), so that both bound it.
 template <typename P, typename G, bool ALONE>
 __global__ __launch_bounds__(256) void adamw_coded(StepList<STEP_TENSORS> list, StepArgs a)
 {

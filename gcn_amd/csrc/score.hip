@@ -276,10 +276,12 @@ __global__ __launch_bounds__(256) void log_probs_small(const T *__restrict__ log
 // largest element with the load it came in.  The k-th largest of 64 groups' largest is a bar that the
 // top k elements all reach and few others do; only the threads that hold such an element look at their part
 // again, what reaches the bar is collected in LDS and put in order by counting.
-// Without entropy and alternatives the memory bounds it: 4096 x 128000 bf16 in 167 us, 6.3 TB/s.  With both it is the
-// vector units (10.5 operations an element and an exponential that counts for four): 2048 x 128000 bf16 in 101 us;
-// x L - c in one multiply-add in place of (x - m) L changes nothing there and costs short rows 8 %.
-// One row of 128000 with 20 alternatives takes 11.4 us, half of it to join the slices; of 61 x 50251 fp16 the alternatives
+// Of 16-bit logits the vector units bound it, busy for 92 % of the CUs' cycles without entropy (8 operations an element and an
+// exponential that counts for four) and for 93 % with it (10.5): 4096 x 128000 bf16 in 161 us, 6.5 TB/s, and 2048 x 128000 with
+// 5 alternatives in 92 us; x L - c in one multiply-add in place of (x - m) L changes nothing there and costs short rows 8 %.
+// Of fp32 it is the memory (63 %): 3001 x 32003 in 65 us, 5.9 TB/s; of fp64 the vector units again (80 %): 1024 x 128000 in 195 us,
+// 5.4 TB/s.
+// One row of 128000 with 20 alternatives takes 10.9 us, two fifths of it to join the slices; of 61 x 50251 fp16 the alternatives
 // are a third of 9.9 us: the bar, what reaches it read again, its order.
 constexpr int SLICE_THREADS = 512;   // or 64: see wave_rows
 constexpr int CANDIDATES = 1024;      // of the joining workgroup
@@ -613,7 +615,8 @@ struct GradRow {
     }
 };
 
-// A thread to each 16 bytes of a row, rows one after the other: 200000 x 1000 bf16 in 190 us, 4.2 TB/s read and written.
+// A thread to each 16 bytes of a row, rows one after the other: 200000 x 1000 bf16 in 190 us, 4.2 TB/s read and written; 20000 x
+// 1000 fp64 in 66 us, 4.9 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void log_probs_grad_packs(const T *logits, unsigned rows, int classes, long stride,
                                                             Targets targets, GradIn<Wide<T>> in, T *d_logits, long d_stride,
@@ -633,8 +636,9 @@ __global__ __launch_bounds__(256) void log_probs_grad_packs(const T *logits, uns
 
 constexpr int GRAD_LOADS = 2;   // 1 and 4 are a few per cent slower over 1 GB of logits
 
-// A tile of a row to a workgroup, two loads to a thread, under way while the row's values come.  Bound by the memory:
-// 4096 x 128000 bf16 in 370 to 390 us, 5.5 TB/s read and written; 3001 x 32003 fp32 in 127 us, 6.0 TB/s.
+// A tile of a row to a workgroup, two loads to a thread, under way while the row's values come.  4096 x 128000 bf16 in 345 us,
+// 6.1 TB/s read and written, with the vector units busy for 95 % of the CUs' cycles (19 operations an element): both bounds at
+// once.  fp32 is bound by the memory (42 %): 3001 x 32003 in 128 us, 6.0 TB/s; fp64 too (52 %): 1024 x 128000 in 328 us, 6.4 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void log_probs_grad_wide(const T *logits, int classes, long stride, Targets targets,
                                                            GradIn<Wide<T>> in, T *d_logits, long d_stride)

@@ -125,8 +125,8 @@ def fit_mbgd(params, cubes, onehot, z, batch=100, lr=None, min_err=None, max_ite
     dropped (gcn_mbgd_fp64.cu:895).
     optimizer: an ops.AdamW over views of `params` (train.adamw makes one) that takes the steps instead of the
     trainers' own rule, from the gradient summed over the batch (and the ranks; keep_tail's short last batch as
-    `batch` times its mean, so that it weighs as much in the moments); lr is then its own unless given, and
-    falls by the same schedule.  max_norm: the norm the batch's mean gradient is clipped to; a step whose norm
+    `batch` times its mean, so that it weighs as much in the moments), which is what its eps acts on; lr is then
+    its own unless given, and falls by the same schedule.  max_norm: the norm the batch's mean gradient is clipped to; a step whose norm
     is not finite is left out.
     """
     f32 = params.dtype == torch.float32

@@ -524,3 +524,52 @@ def test_no_element_is_lost_from_a_long_row(rows, classes, kind):
     x[:, 0] = 5.0
     y[:] = 0
     check()
+
+
+@pytest.mark.parametrize("rows,classes,kind", [((1 << 24) + 77, 3, torch.float32), ((1 << 22) + 67, 1025, torch.bfloat16), (70001, 1027, torch.float32),
+                                               (70001, 1025, torch.float64), ((1 << 22) + 67, 1000, torch.float64)], ids=str)
+def test_more_rows_than_one_launch_takes(rows, classes, kind):
+    """Rows that repeat every 61 have results that do, whichever launch they are in; some against 64 bits."""
+    base, by = problem(61, classes, kind, seed=14)
+    at = torch.arange(rows, device="cuda") % 61
+    x, y = base[at], by[at]
+    r = ops.log_probs(x, y, top=2)
+    picked = [0, 1, 60, 61, 65534, 65535, 65536, (1 << 22) - 1, 1 << 22, (1 << 24) - 1, 1 << 24, rows - 1]
+    some = torch.tensor([i for i in picked if i < rows], device="cuda")
+    part = ops.LogProbs(*(t[some] for t in r[:4]), r.stats[:, some].contiguous())
+    _, want = check_scores(x[some], y[some], 2, got=part)
+    for t in r[:4]:
+        assert torch.equal(t, t[:61][at])
+    dl, dh = (w[at] for w in weights(61, kind))
+    g = ops.log_probs_grad(x, y, r, dl, dh, out=x)
+    assert g.data_ptr() == x.data_ptr()
+    exact = ref.log_probs_grad(want, y[some], dl[some], dh[some])
+    # probabilities within the bound of the sums, the result rounded once
+    off = (g[some].cpu().double() - exact).abs()
+    assert (off <= 8 * ref.score_bound(base, ref.log_probs(base, by), wide(kind)).max() + ref.half_step(kind) * exact.abs()).all()
+    first = g[:61].clone()
+    for a in range(0, rows, 1 << 20):
+        assert torch.equal(g[a:a + (1 << 20)], first[at[a:a + (1 << 20)]])
+
+
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16], ids=str)
+def test_the_longest_row(kind):
+    """2^30 classes: equal ones but for a few, so that the sums are known."""
+    classes = 1 << 30
+    x = torch.zeros((1, classes), dtype=kind, device="cuda")
+    at = torch.tensor([classes - 1, 0, (1 << 29) + 5], device="cuda")
+    x[0, at] = torch.tensor([12.0, 11.0, 10.0], dtype=kind, device="cuda")
+    y = torch.tensor([classes - 1], device="cuda")
+    r = ops.log_probs(x, y, top=5)
+    total = math.fsum([classes - 3, math.exp(12), math.exp(11), math.exp(10)])
+    weighed = math.fsum([12 * math.exp(12), 11 * math.exp(11), 10 * math.exp(10)])
+    u = ref.half_step(torch.float32)
+    # 512 slices of 512 threads: 4096 additions each and 64 to join; the terms' own errors and the log's as in score_bound
+    bound = u * (4096 + 64 + 6 * 12 + 30 + 4 * math.log(total))
+    assert abs(r.logp.item() - (12 - math.log(total))) <= bound
+    assert abs(r.entropy.item() - (math.log(total) - weighed / total)) <= 30 * bound
+    assert r.top_index.tolist() == [[classes - 1, 0, (1 << 29) + 5, 1, 2]]
+    d = ops.log_probs_grad(x, y, r, torch.ones(1, device="cuda"), None, out=x)
+    want = -1.0 / total
+    assert abs(d[0, 7].item() / want - 1) < 0.01 and abs(d[0, classes - 2].item() / want - 1) < 0.01
+    assert abs(d[0, classes - 1].item() - (1 - math.exp(12) / total)) < 2 ** -8 and abs(d[0, 0].item() / (math.exp(11) * want) - 1) < 0.01

@@ -22,6 +22,7 @@ decltype(&ccnn_log_probs_grad) log_probs_grad_fn;
 decltype(&ccnn_grad_norm_workspace_bytes) grad_norm_bytes_fn;
 decltype(&ccnn_grad_norm) grad_norm_fn;
 decltype(&ccnn_adamw_step) adamw_step_fn;
+decltype(&ccnn_adamw_moments) adamw_moments_fn;
 
 int type_of(const at::Tensor &t)
 {
@@ -88,16 +89,17 @@ bool count_is(Py_ssize_t n, Py_ssize_t want)
     return n == want;
 }
 
-// bind(six addresses, in the order of their names above)
+// bind(seven addresses, in the order of their names above)
 PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
-    if (!count_is(n, 6)) return nullptr;
+    if (!count_is(n, 7)) return nullptr;
     log_probs_bytes_fn = (decltype(log_probs_bytes_fn))address(a[0]);
     log_probs_fn = (decltype(log_probs_fn))address(a[1]);
     log_probs_grad_fn = (decltype(log_probs_grad_fn))address(a[2]);
     grad_norm_bytes_fn = (decltype(grad_norm_bytes_fn))address(a[3]);
     grad_norm_fn = (decltype(grad_norm_fn))address(a[4]);
     adamw_step_fn = (decltype(adamw_step_fn))address(a[5]);
+    adamw_moments_fn = (decltype(adamw_moments_fn))address(a[6]);
     return PyErr_Occurred() ? nullptr : none();
 }
 
@@ -304,8 +306,49 @@ PyObject *adamw_step(PyObject *, PyObject *const *a, Py_ssize_t n)
     END_HANDLE_TH_ERRORS
 }
 
+// adamw_moments(stream, device, table, m, v, m_scale, v_scale, master) -> (m, v) of 8-bit moments, as the values they stand for,
+// of a state that is whole
+PyObject *adamw_moments(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    if (!count_is(n, 8)) return nullptr;
+    void *stream = address(a[0]);
+    const long device = PyLong_AsLong(a[1]);
+    if (PyErr_Occurred()) return nullptr;
+    const Bytes held(a[2]);
+    const auto *table = (const ccnn_adamw_tensor_t *)held.view.buf;
+    const int count = (int)(held.view.len / (Py_ssize_t)sizeof *table);
+    if (count == 0 || held.view.len != (Py_ssize_t)(count * sizeof *table)) return none();
+    long elements = 0, blocks = 0;
+    bool any_half = false;
+    for (int i = 0; i < count; i++) {
+        elements += table[i].n;
+        blocks += (table[i].n + CCNN_MOMENT_BLOCK - 1) / CCNN_MOMENT_BLOCK;
+        any_half |= table[i].type == CCNN_TYPE_BF16 || table[i].type == CCNN_TYPE_F16;
+    }
+    void *state[4], *master;
+    if (!plain(a[7], device, at::kFloat, elements, &master) || (a[7] == Py_None) == any_half) return none();
+    for (int i = 0; i < 4; i++)
+        if (!plain(a[3 + i], device, i < 2 ? at::kByte : at::kFloat, i < 2 ? blocks * CCNN_MOMENT_BLOCK : blocks, &state[i])
+            || a[3 + i] == Py_None)
+            return none();
+    const auto wide = at::TensorOptions().device(at::Device(at::kCUDA, (c10::DeviceIndex)device)).dtype(at::kFloat);
+    const at::Tensor m = at::empty({elements}, wide), v = at::empty({elements}, wide);
+    const int rc = unlocked([&] {
+        return adamw_moments_fn(table, count, state[0], state[1], (const float *)state[2], (const float *)state[3],
+                                (float *)m.data_ptr(), (float *)v.data_ptr(), stream);
+    });
+    if (rc) return PyLong_FromLong(rc);
+    PyObject *out = PyTuple_New(2);
+    if (!out) return nullptr;
+    PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(m));
+    PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(v));
+    return out;
+    END_HANDLE_TH_ERRORS
+}
+
 #define CALL(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {CALL(bind), CALL(log_probs), CALL(log_probs_grad), CALL(grad_norm), CALL(adamw_step),
+PyMethodDef methods[] = {CALL(bind), CALL(log_probs), CALL(log_probs_grad), CALL(grad_norm), CALL(adamw_step), CALL(adamw_moments),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "ccnn_torch_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -149,7 +149,7 @@ def load():
 _calls = None
 # what the module beside the library calls, in the order of its bind()
 _CALLED = ("ccnn_log_probs_workspace_bytes", "ccnn_log_probs", "ccnn_log_probs_grad", "ccnn_grad_norm_workspace_bytes",
-           "ccnn_grad_norm", "ccnn_adamw_step")
+           "ccnn_grad_norm", "ccnn_adamw_step", "ccnn_adamw_moments")
 
 
 def calls():

@@ -650,12 +650,11 @@ class AdamW:
         the codes stand for (fp32) with 8."""
         if self.state_bits == 32:
             return self.m, self.v
-        self._refuse_state()
-        m, v = (torch.empty(self.numel, dtype=_F32, device=self.device) for _ in range(2))
-        with torch.cuda.device(self.device):
-            _l.check(_l.load().ccnn_adamw_moments(self._table, len(self._table), _ptr(self.m), _ptr(self.v), _ptr(self.m_scale),
-                                                  _ptr(self.v_scale), _ptr(m), _ptr(v), _stream()), "ccnn_adamw_moments")
-        return m, v
+        got = _called("adamw_moments", self.m, self._table, self.m, self.v, self.m_scale, self.v_scale, self.master)
+        if got is None:
+            self._refuse_state()
+            raise ValueError("the optimiser's state cannot be used")
+        return got
 
     def state_dict(self):
         """Copies of everything a later run continues from (waits for the device)."""

@@ -68,3 +68,15 @@ def test_the_table_of_a_step_is_an_array_with_a_length(calls):
         for odd in (table, bytes(table), memoryview(b"")[::1], b"", "x", None, 3.5, 1 << 70, [table]):
             assert calls.adamw_step(0, 0, [d] * count, [d] * count, odd, 32, d, d, None, None, None, d, 1e-3, 0.9, 0.999,
                                     1e-8, None) is None
+
+
+def test_a_read_out_takes_an_array_and_tensors_of_its_sizes(calls):
+    d = torch.zeros(4)
+    table = (L.AdamwTensor * 2)((d.data_ptr(), 4, 0, 0, 0.0, L.TYPE_F32), (d.data_ptr(), 4, 4, 1, 0.0, L.TYPE_F32))
+    codes, scales = torch.zeros(512, dtype=torch.uint8), torch.zeros(2)
+    for odd in (table, bytes(table)[:-1], b"", None, 3, "x"):
+        for device in (0, -1):
+            assert calls.adamw_moments(0, device, odd, codes, codes, scales, scales, None) is None
+            assert calls.adamw_moments(0, device, odd, None, None, None, None, None) is None
+    with pytest.raises(TypeError):
+        calls.adamw_moments(0, 0, table)

@@ -20,7 +20,8 @@ constexpr int BLOCK = CCNN_MOMENT_BLOCK;
 // Squares are summed in fp64, in an order that the sizes alone fix: those of fp32 and 16-bit gradients are exact there and fit, and
 // the sum of n of them is off by at most (n / 64 + 40) 2^-53 of itself, a rounding for each addition.  Squares of fp64 gradients
 // may not fit: where a sum of theirs shows that, what is beyond 2^480 or below 2^-480 is summed apart, brought near 1 by a
-// power of two.  The look costs 47 k fp64 gradients 0.15 us (4.8 of the device) and 210 M nothing (247 us, 6.8 TB/s).
+// power of two.  The look costs 47 k fp64 gradients 0.1 us (4.9 of the device), 131 k to 8 M 0.4 (7.5 to 16.2) and 210 M
+// nothing (247 us, 6.8 TB/s).
 // A wave to a chunk: short ones while they are needed to fill the device, long ones beyond (202 M bf16 gradients: 65 us, 6.2 TB/s;
 // 78 with workgroups of 256 to 16 K, 73 with a wave to 16 K).  Just beyond the border the long ones are too few waves: fp32, 31 M
 // take 24 us, 36 M 49, 52 M 53, 105 M 70 (6.0 TB/s) and 210 M 127 (6.6); bf16 19, 39, 41, 49 (4.3) and 66 (6.4).
@@ -86,12 +87,6 @@ __device__ __forceinline__ void add_apart(Squares &s, const double *p, long k, l
         }
 }
 
-// mid, with a sign where something is apart.
-__device__ __forceinline__ double marked(const Squares &s)
-{
-    return s.big > 0 || s.tiny > 0 ? -fabs(s.mid) : fabs(s.mid);
-}
-
 template <typename T>
 __global__ __launch_bounds__(NORM_THREADS) void norm_partial(NormList<NORM_TENSORS> list, int chunk, double *__restrict__ partial,
                                                              double *__restrict__ apart, long apart_stride)
@@ -126,15 +121,22 @@ __global__ __launch_bounds__(NORM_THREADS) void norm_partial(NormList<NORM_TENSO
             }
         }
     }
-    Squares s = {sum};
-    if constexpr (sizeof(T) == 8)
-        if (!stands(sum) && (high << 1 | low) != 0) s = {}, add_apart<W>(s, p, threadIdx.x * W, n, STRIDE);
-    s.mid = lanes_sum<64>(s.mid);
-    if (__any(s.big > 0 || s.tiny > 0)) s.big = lanes_sum<64>(s.big), s.tiny = lanes_sum<64>(s.tiny);
-    if (threadIdx.x == 0) {
-        partial[blockIdx.x] = marked(s);
-        if (signbit(marked(s))) apart[blockIdx.x] = s.big, apart[apart_stride + blockIdx.x] = s.tiny;
+    if constexpr (sizeof(T) == 8) {
+        const bool falls = !stands(sum) && (high << 1 | low) != 0;
+        if (__builtin_expect(__any(falls), 0)) {
+            Squares s;
+            if (falls) add_apart<W>(s, p, threadIdx.x * W, n, STRIDE);
+            else s.mid = sum;
+            s = {lanes_sum<64>(s.mid), lanes_sum<64>(s.big), lanes_sum<64>(s.tiny)};
+            if (threadIdx.x == 0) {                 // a sign: something is apart
+                partial[blockIdx.x] = -s.mid;
+                apart[blockIdx.x] = s.big, apart[apart_stride + blockIdx.x] = s.tiny;
+            }
+            return;
+        }
     }
+    sum = lanes_sum<64>(sum);
+    if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
 
 __device__ __forceinline__ void put_norm(const Squares &s, double max_norm, double *out)
@@ -156,21 +158,30 @@ __global__ __launch_bounds__(TOTAL_THREADS) void norm_total(const double *__rest
 {
     __shared__ double lds[F64 ? 3 : 1][TOTAL_THREADS / 64];
     Squares s;
-    bool any = false;
+    bool any = false;       // a sign in memory or, from wave to wave, in LDS: something is apart
 #pragma unroll 4
     for (int k = threadIdx.x; k < n; k += TOTAL_THREADS) {
         const double mid = partial[k];
         s.mid += F64 ? fabs(mid) : mid;
         any |= F64 && signbit(mid);
     }
-    s.mid = block_sum<TOTAL_THREADS>(s.mid, lds[0]);
-    if constexpr (F64)
-        if (__syncthreads_or(any)) {
+    if constexpr (F64) {
+        s.mid = lanes_sum<64>(s.mid);
+        any = __any(any);
+        if ((threadIdx.x & 63) == 0) lds[0][threadIdx.x >> 6] = any ? -s.mid : s.mid;
+        __syncthreads();
+        s.mid = 0;
+#pragma unroll
+        for (int w = 0; w < TOTAL_THREADS / 64; w++) s.mid += fabs(lds[0][w]), any |= signbit(lds[0][w]);
+        if (any) {
             for (int k = threadIdx.x; k < n; k += TOTAL_THREADS)
                 if (signbit(partial[k])) s.big += apart[k], s.tiny += apart[apart_stride + k];
             s.big = block_sum<TOTAL_THREADS>(s.big, lds[1]);
             s.tiny = block_sum<TOTAL_THREADS>(s.tiny, lds[2]);
         }
+    } else {
+        s.mid = block_sum<TOTAL_THREADS>(s.mid, lds[0]);
+    }
     if (threadIdx.x == 0) put_norm(s, max_norm, out);
 }
 
